@@ -37,7 +37,7 @@ def lib() -> C.CDLL:
         L = C.CDLL(LIB_PATH)
         L.gs4d_last_error.restype = C.c_char_p
         for name in ("gs4d_geometry_bytes", "gs4d_binning_bytes", "gs4d_image_bytes", "gs4d_backward_scratch_bytes",
-                     "gs4d_l1_loss_scratch_bytes"):
+                     "gs4d_l1_loss_scratch_bytes", "gs4d_linear8_keep_bytes", "gs4d_linear8_scratch_bytes"):
             getattr(L, name).restype = C.c_size_t
         L.gs4d_thread_state_release.restype = None
         L.gs4d_mailbox_stats.restype = None

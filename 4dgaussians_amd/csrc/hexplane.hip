@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include "deform_hexplane.h"
+#include "lowbit.h"
 
 namespace {
 
@@ -163,6 +164,48 @@ __global__ __launch_bounds__(256) void hexplane_forward_shared_kernel(
             acc.w *= f00.w * cw.x + f01.w * cw.y + f10.w * cw.z + f11.w * cw.w;
         }
         reinterpret_cast<float4*>(feat + (size_t)p * ldf + l * C)[sub] = acc;
+    }
+}
+
+// The features of a frame from a cache of the spatial planes' product (gs4d_frame_features): three bilinear samples per level
+// over (axis, t) and one 8-bit row, instead of six samples.  C / 4 lanes per point, 4 channels each.
+struct FramePlanes { const float* p[GS4D_MAX_LEVELS * 3]; int w[GS4D_MAX_LEVELS * 3]; int h[GS4D_MAX_LEVELS * 3]; };
+
+template <int FMT>
+__global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L, int C, int lpp_shift, FramePlanes T,
+                                                             const float* __restrict__ aabb, const float* __restrict__ xyz,
+                                                             const float* __restrict__ t, int t_stride, long long P,
+                                                             float* __restrict__ out, long long ld)
+{
+    const long long gtid = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long p = gtid >> lpp_shift;
+    const int sub = (int)(gtid & ((1 << lpp_shift) - 1));
+    if (p >= P) return;
+    float u[3];
+#pragma unroll
+    for (int a = 0; a < 3; a++) {
+        const float lo = aabb[a], hi = aabb[3 + a];
+        u[a] = (xyz[3 * p + a] - lo) * (2.0f / (hi - lo)) - 1.0f;
+    }
+    const float tt = t[p * t_stride];
+    const int ng = (c.width + c.group - 1) / c.group, q = C >> 2;
+    for (int l = 0; l < L; l++) {
+        const int col = l * C + 4 * sub;
+        const float s = c.scales[p * ng + col / c.group];
+        const float4 k = lb_decode4<FMT>(*reinterpret_cast<const unsigned*>(c.codes + (size_t)p * c.pitch + col));
+        float4 acc = make_float4(s * k.x, s * k.y, s * k.z, s * k.w);
+#pragma unroll
+        for (int a = 0; a < 3; a++) {
+            const Corner n = corner_of(u[a], tt, T.w[3 * l + a], T.h[3 * l + a]);
+            const float4* __restrict__ base = reinterpret_cast<const float4*>(T.p[3 * l + a]) + sub;
+            const float4 f00 = base[(size_t)n.i00 * q], f01 = base[(size_t)n.i01 * q];
+            const float4 f10 = base[(size_t)n.i10 * q], f11 = base[(size_t)n.i11 * q];
+            acc.x *= f00.x * n.w00 + f01.x * n.w01 + f10.x * n.w10 + f11.x * n.w11;
+            acc.y *= f00.y * n.w00 + f01.y * n.w01 + f10.y * n.w10 + f11.y * n.w11;
+            acc.z *= f00.z * n.w00 + f01.z * n.w01 + f10.z * n.w10 + f11.z * n.w11;
+            acc.w *= f00.w * n.w00 + f01.w * n.w01 + f10.w * n.w10 + f11.w * n.w11;
+        }
+        reinterpret_cast<float4*>(out + p * ld + l * C)[sub] = acc;
     }
 }
 
@@ -910,5 +953,38 @@ int gs4d_hex_launch_backward(const gs4d_deform_desc* d, const gs4d_deform_grads*
         GS4D_LAUNCH_CHECK("hexplane_coord_reduce", 0, s);
     }
     *ft_done = fold_ft ? 1 : 0;
+    return GS4D_OK;
+}
+
+extern "C" int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const float* const* planes, const int* plane_w,
+                                   const int* plane_h, const float* aabb, const float* points, const float* t, int t_stride,
+                                   long long P, float* out, long long ld, void* stream)
+{
+    GS4D_TRACE_SCOPE("gs4d_frame_features");
+    hipStream_t s = (hipStream_t)stream;
+    if (!c || L < 1 || L > GS4D_MAX_LEVELS || C < 4 || C > 256 || (C & (C - 1)) || c->width != L * C || P < 0 || P > c->capacity ||
+        !c->codes || !c->scales || c->pitch < c->width || (c->pitch & 15) || ((uintptr_t)c->codes & 15) ||
+        (c->group != 32 && c->group != 64 && c->group != 128) || c->fmt < GS4D_FMT_INT8 || c->fmt > GS4D_FMT_E5M2) {
+        gs4d_set_error("gs4d_frame_features: bad cache, levels or channels (rows of L * C values, C a power of two in [4, 256], at least P rows)");
+        return GS4D_EINVAL;
+    }
+    if (P == 0) return GS4D_OK;
+    if (!planes || !plane_w || !plane_h || !aabb || !points || !t || !out || ((uintptr_t)out & 15) || (ld & 3) || ld < c->width ||
+        (t_stride != 0 && t_stride != 1)) {
+        gs4d_set_error("gs4d_frame_features: null or misaligned pointer, or a row pitch that is too small or no multiple of 4");
+        return GS4D_EINVAL;
+    }
+    FramePlanes T = {};
+    for (int i = 0; i < L * 3; i++) {
+        if (!planes[i] || ((uintptr_t)planes[i] & 15) || plane_w[i] < 1 || plane_h[i] < 1) { gs4d_set_error("gs4d_frame_features: plane %d null, empty or not 16-byte aligned", i); return GS4D_EINVAL; }
+        T.p[i] = planes[i]; T.w[i] = plane_w[i]; T.h[i] = plane_h[i];
+    }
+    int lpp_shift = 0;
+    while ((1 << lpp_shift) < C / 4) lpp_shift++;
+    const size_t threads = (size_t)P << lpp_shift;
+    if (threads > 0xffffff00ull) { gs4d_set_error("gs4d_frame_features: %lld points are too many for one call", P); return GS4D_EINVAL; }
+    auto k = c->fmt == GS4D_FMT_INT8 ? frame_features_kernel<GS4D_FMT_INT8> : c->fmt == GS4D_FMT_E4M3 ? frame_features_kernel<GS4D_FMT_E4M3> : frame_features_kernel<GS4D_FMT_E5M2>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, *c, L, C, lpp_shift, T, aabb, points, t, t_stride, P, out, ld);
+    GS4D_LAUNCH_CHECK("frame_features", 0, s);
     return GS4D_OK;
 }

@@ -610,6 +610,70 @@ int gs4d_temporal_regulation_backward(int n, int k, int sh_floats, const float* 
                                       const float* packed, float* scratch, const float* g6, float* const* grad13,
                                       void* stream);
 
+/*
+ * Rows in 8 bits, one float32 scale per group of columns (no counterpart in the reference, which keeps everything in float32):
+ *   a = max |x| of the group, s = a / Q, code = round_half_even(x * (Q / a)) in the format, value = s * code,
+ * Q = 127 (int8), 448 (e4m3), 57344 (e5m2); the quotients and the product are rounded to float32.  s below 2^-126: the group
+ * is stored as zero.  A group with an infinity or a NaN reads as NaN.
+ */
+#define GS4D_F32 0
+#define GS4D_BF16 1
+#define GS4D_F16 2
+#define GS4D_FMT_INT8 0
+#define GS4D_FMT_E4M3 1
+#define GS4D_FMT_E5M2 2
+#define GS4D_FMT_UINT8 3        /* 0..255: what gs4d_linear8 keeps of a rectified input in place of int8 */
+#define GS4D_ROWS8_SCAN 256     /* up to this many rows at given slots are written without `owner` */
+
+/* A cache of rows: codes [capacity][pitch] bytes (16-byte aligned, pitch a multiple of 16, at least width), scales
+ * [capacity][ceil(width / group)].  owner: [capacity] ints, all zero, or NULL; gs4d_rows8_write leaves them zero. */
+typedef struct gs4d_rows8 {
+    unsigned char* codes;
+    float* scales;
+    int* owner;
+    long long capacity;
+    int width, pitch, group, fmt;      /* group: 32, 64 or 128 columns */
+} gs4d_rows8;
+
+/* rows [n] of `dtype` with a pitch of ld elements -> the cache.  slots: device [n] ints of slot_bytes (4 or 8) bytes each, or
+ * NULL for the slots start .. start + n - 1.  A row whose slot lies outside [0, capacity) is padding and not stored.  A slot
+ * that several rows of the call name keeps the last of them. */
+int gs4d_rows8_write(const gs4d_rows8* c, const void* rows, int dtype, long long ld, long long n, const void* slots, int slot_bytes,
+                     long long start, void* stream);
+/* The inverse: out[i][0 .. width) = the values of row slots[i] (zeros where it lies outside the cache), rounded to dtype. */
+int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, long long n, const void* slots, int slot_bytes,
+                    long long start, void* stream);
+
+/*
+ * y [N][M] = act(x) w^T + b, x [N] rows of K with a pitch of ldx elements, w [M][K], b [M] or NULL, act = relu or nothing; all
+ * of one dtype, sums in float32.  The backward does not need x: `keep` (gs4d_linear8_keep_bytes, 256-byte aligned) receives
+ *   GS4D_KEEP_CODES  act(x) in 8 bits in groups of 64 columns (int8 becomes uint8 with relu): the weight gradient's operand
+ *   GS4D_KEEP_SIGNS  a bit per value, x > 0 (relu only): the input gradient's mask
+ * as `what` says (0: nothing, keep may be NULL).
+ */
+#define GS4D_KEEP_CODES 1
+#define GS4D_KEEP_SIGNS 2
+size_t gs4d_linear8_keep_bytes(long long N, int K, int what);
+int gs4d_linear8_forward(int dtype, long long N, int K, int M, const void* x, long long ldx, const void* w, const void* b, int relu,
+                         int fmt, void* y, char* keep, int what, void* stream);
+/* dy [N][M] -> dx [N][K], dw [M][K], db [M], each of which may be NULL (written, not accumulated); dtype, relu, fmt, keep and
+ * what as in the forward.  scratch: gs4d_linear8_scratch_bytes, 256-byte aligned. */
+size_t gs4d_linear8_scratch_bytes(long long N, int K, int M);
+int gs4d_linear8_backward(int dtype, long long N, int K, int M, const void* dy, const void* w, int relu, int fmt, char* keep, int what,
+                          void* dx, void* dw, void* db, char* scratch, void* stream);
+
+/*
+ * The plane features of one frame from a cache of the spatial planes' product (rows of L * C values):
+ *   out[p][l * C + c] = value(cache row p) * product over a = x, y, z of the bilinear sample of planes[3 l + a] at
+ *   (normalised coordinate a of point p, t)
+ * planes[3 l + a]: channels-last [plane_h][plane_w][C], the axis along the width and t along the height; aabb, points and the
+ * border rule as in gs4d_deform_forward.  t: device, one normalised value for all points (t_stride 0) or one per point
+ * (t_stride 1).  out: P rows with a pitch of ld floats, 16-byte aligned, ld a multiple of 4.  The cache holds at least P rows.
+ */
+int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const float* const* planes, const int* plane_w, const int* plane_h,
+                        const float* aabb, const float* points, const float* t, int t_stride, long long P, float* out,
+                        long long ld, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
