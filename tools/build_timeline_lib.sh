@@ -4,7 +4,7 @@
 set -e
 cd 4dgaussians_amd/csrc
 make -s
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -I../../include -DGS4D_TIMELINE $TL_EXTRA"
+F="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -I../../include -DGS4D_TIMELINE $TL_EXTRA"
 /opt/rocm/bin/hipcc $F -c blend_bwd.hip -o /tmp/blend_bwd_tl.o
 /opt/rocm/bin/hipcc $F -c blend_fwd.hip -o /tmp/blend_fwd_tl.o
 /opt/rocm/bin/hipcc $F -ffp-contract=off -c binning.hip -o /tmp/binning_tl.o
