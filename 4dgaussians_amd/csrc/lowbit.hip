@@ -111,130 +111,608 @@ static Keep carve_keep(char* base, long long N, int K, int what, size_t* bytes)
     return k;
 }
 
-// relu that keeps a NaN
-__device__ __forceinline__ float lb_relu(float x) { return x < 0.f ? 0.f : x; }
-
-template <int FMT, bool RELU, typename T>
-__global__ __launch_bounds__(256) void linear8_keep_kernel(Keep kp, const T* __restrict__ x, long long ldx, long long N, int K)
+template <typename F> static int by_type(int dtype, F f)
 {
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;       // 8 lanes per group of 64
-    const int cpr = kp.kp / 8;
-    const long long i = t / cpr;
-    const int col = (int)(t % cpr) * 8;
-    if (i >= N) return;
-    float v[8];
-    unsigned m = 0, bits = 0;
-#pragma unroll
-    for (int q = 0; q < 8; q++) {
-        v[q] = col + q < K ? lb_load(x[i * ldx + col + q]) : 0.f;
-        if (RELU) {
-            bits |= (v[q] <= 0.f ? 0u : 1u) << q;
-            v[q] = lb_relu(v[q]);
-        }
-        m = max(m, lb_abs_bits(v[q]));
-    }
-    if (RELU && kp.bits) kp.bits[i * cpr + (col >> 3)] = (unsigned char)bits;
-    if (!kp.codes) return;
-#pragma unroll
-    for (int s = 1; s < 8; s <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, s, 64));
-    const LbScale sc = lb_scale<FMT>(m);
-    uint2 w;
-    w.x = lb_encode4<FMT>(v[0] * sc.inv, v[1] * sc.inv, v[2] * sc.inv, v[3] * sc.inv);
-    w.y = lb_encode4<FMT>(v[4] * sc.inv, v[5] * sc.inv, v[6] * sc.inv, v[7] * sc.inv);
-    *reinterpret_cast<uint2*>(kp.codes + (size_t)i * kp.kp + col) = w;
-    if ((col & 63) == 0) kp.scales[(size_t)i * (kp.kp / 64) + (col >> 6)] = sc.s;
+    return dtype == GS4D_F32 ? f(float()) : dtype == GS4D_BF16 ? f(LbBf16()) : f(LbF16());
+}
+template <int V> struct Int { static constexpr int value = V; };
+template <typename F> static int by_fmt(int fmt, F f)
+{
+    return fmt == GS4D_FMT_INT8 ? f(Int<GS4D_FMT_INT8>()) : fmt == GS4D_FMT_E4M3 ? f(Int<GS4D_FMT_E4M3>()) :
+           fmt == GS4D_FMT_E5M2 ? f(Int<GS4D_FMT_E5M2>()) : f(Int<GS4D_FMT_UINT8>());
 }
 
-// The three products, simplest form: a 64 x 64 tile of the result per workgroup, 16 steps of the contraction at a time through
-// LDS, 4 x 4 results per thread in float32.  LA(row, k) and LB(col, k) give the operands, out-of-range ones as zero.
-template <typename LA, typename LB, typename ST>
-__device__ __forceinline__ void tile_product(long long k0, long long k1, LA la, LB lb, ST st)
+// What the matrix cores work on: 8 consecutive elements of a row per lane (lane & 31: the row of the operand, lane >> 5: which
+// half of 16), as 16-bit numbers.  A float32 number is the sum of three bfloat16 numbers -- its leading 8 significant bits, the
+// next 8 and the last 8, by truncation, so the sum is exact above 2^-110 -- and a product of two of them is taken from the six
+// largest of the nine term products; the three left out are below 2^-23 of it together.  Six bfloat16 MFMAs against the
+// float32 one: 2.7 times its rate.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> constexpr int kTerms = 1;
+template <> constexpr int kTerms<float> = 3;
+
+template <typename T> __device__ __forceinline__ f32x16 mfma(const uint4& a, const uint4& b, const f32x16& c)
 {
-    __shared__ float sa[16][65], sb[16][65];
-    const int tid = threadIdx.x, tr = (tid >> 4) * 4, tc = (tid & 15) * 4;
-    float acc[4][4] = {};
-    for (long long k = k0; k < k1; k += 16) {
-        for (int e = tid; e < 1024; e += 256) {
-            const int r = e >> 4, q = e & 15;
-            sa[q][r] = la(r, k + q);
-            sb[q][r] = lb(r, k + q);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 16; q++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sa[q][tr + i], sb[q][tc + j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) st(tr + i, tc + j, acc[i][j]);
+    if constexpr (__is_same(T, LbF16))
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <bool RELU, typename T>
-__global__ __launch_bounds__(256) void linear8_forward_kernel(long long N, int K, int M, const T* __restrict__ x, long long ldx,
-                                                              const T* __restrict__ w, const T* __restrict__ b, T* __restrict__ y)
+// the upper halves of two words
+__device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ float top8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
+// two numbers -> their TERMS bfloat16 parts, packed.  SAFE: also for infinities (whose remainder would be a NaN)
+template <int TERMS, bool SAFE>
+__device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
 {
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64;
-    tile_product(0, K,
-        [&](int r, long long k) { const float v = r0 + r < N && k < K ? lb_load(x[(r0 + r) * ldx + k]) : 0.f; return RELU ? lb_relu(v) : v; },
-        [&](int c, long long k) { return c0 + c < M && k < K ? lb_load(w[(long long)(c0 + c) * K + k]) : 0.f; },
-        [&](int r, int c, float v) { if (r0 + r < N && c0 + c < M) y[(r0 + r) * M + c0 + c] = lb_store<T>(v + (b ? lb_load(b[c0 + c]) : 0.f)); });
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) {
+        o[t] = hi16(__float_as_uint(a), __float_as_uint(b));
+        if (t + 1 < TERMS) {
+            const float ra = a - top8(a), rb = b - top8(b);
+            a = SAFE && lb_abs_bits(a) == 0x7f800000u ? 0.f : ra;
+            b = SAFE && lb_abs_bits(b) == 0x7f800000u ? 0.f : rb;
+        }
+    }
+}
+
+template <int TERMS, bool SAFE>
+__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
+{
+    unsigned w[4][TERMS];
+#pragma unroll
+    for (int q = 0; q < 4; q++) split2<TERMS, SAFE>(v[2 * q], v[2 * q + 1], w[q]);
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) o[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+}
+
+// relu on the bits: a number with its sign bit set is a negative integer.  lowest = 0: relu, INT_MIN / -32768: nothing.
+__device__ __forceinline__ unsigned relu_bits(unsigned x, int lowest) { return (unsigned)max((int)x, lowest); }
+__device__ __forceinline__ unsigned relu_bits2(unsigned x, unsigned lowest2)
+{
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(s16x2, x), __builtin_bit_cast(s16x2, lowest2)));
+}
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b)
+{
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <typename T> __device__ __forceinline__ float low16(unsigned w)
+{
+    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)w);
+    else return __uint_as_float(w << 16);
+}
+template <typename T> __device__ __forceinline__ float high16(unsigned w)
+{
+    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+    else return __uint_as_float(w & 0xffff0000u);
+}
+
+// A lane's share of a row's group of 64 columns: 4 steps of 8 elements, at columns 16 t + 8 h.
+template <typename T> struct Group { uint4 w[4]; };
+template <> struct Group<float> { uint4 w[8]; };
+
+// VEC: rows start on 16 bytes and C is a multiple of 8.  Columns past C are read somewhere inside the row; the caller clears them.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_group(Group<T>& g, const T* __restrict__ row, int c0, int C)
+{
+    constexpr int PER = 16 / (int)sizeof(T);              // elements per 16 bytes
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        if constexpr (VEC) {
+            const T* p = row + min(c0 + 16 * t, C - 8);
+#pragma unroll
+            for (int q = 0; q < 8 / PER; q++) g.w[t * (8 / PER) + q] = reinterpret_cast<const uint4*>(p)[q];
+        } else if constexpr (sizeof(T) == 4) {
+            unsigned e[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) e[q] = __float_as_uint(row[min(c0 + 16 * t + q, C - 1)]);
+            g.w[2 * t] = make_uint4(e[0], e[1], e[2], e[3]);
+            g.w[2 * t + 1] = make_uint4(e[4], e[5], e[6], e[7]);
+        } else {
+            unsigned e[8];
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+            for (int q = 0; q < 8; q++) e[q] = p[min(c0 + 16 * t + q, C - 1)];
+            g.w[t] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void linear8_dx_kernel(long long N, int K, int M, const T* __restrict__ dy, const T* __restrict__ w,
-                                                         Keep kp, T* __restrict__ dx)
+__device__ __forceinline__ void clear_past(Group<T>& g, int c0, int C)
 {
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64;
-    tile_product(0, M,
-        [&](int r, long long m) { return r0 + r < N && m < M ? lb_load(dy[(r0 + r) * M + m]) : 0.f; },
-        [&](int c, long long m) { return c0 + c < K && m < M ? lb_load(w[m * K + c0 + c]) : 0.f; },
-        [&](int r, int c, float v) {
-            if (r0 + r >= N || c0 + c >= K) return;
-            const int k = c0 + c;
-            if (kp.bits && !(kp.bits[(r0 + r) * (kp.kp / 8) + (k >> 3)] >> (k & 7) & 1)) v = 0.f;
-            dx[(r0 + r) * K + k] = lb_store<T>(v);
-        });
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const int left = C - c0 - 16 * t;                 // elements of this step inside the row
+        if constexpr (sizeof(T) == 4) {
+            unsigned* e = reinterpret_cast<unsigned*>(&g.w[2 * t]);
+#pragma unroll
+            for (int q = 0; q < 8; q++) e[q] = q < left ? e[q] : 0u;
+        } else {
+            unsigned* e = reinterpret_cast<unsigned*>(&g.w[t]);
+#pragma unroll
+            for (int q = 0; q < 4; q++) e[q] = 2 * q + 1 < left ? e[q] : 2 * q < left ? e[q] & 0xffffu : 0u;
+        }
+    }
 }
 
-// partial[chunk][m][kc]: kc < K the weight gradient of the chunk's rows, kc == K the bias gradient
-template <int FMT, typename T>
-__global__ __launch_bounds__(256) void linear8_dw_kernel(long long N, int K, int M, const T* __restrict__ dy, Keep kp,
-                                                         long long per, float* __restrict__ partial)
-{
-    const int m0 = blockIdx.y * 64, c0 = blockIdx.z * 64;
-    const long long n0 = (long long)blockIdx.x * per, n1 = min(N, n0 + per);
-    tile_product(n0, n1,
-        [&](int r, long long n) { return m0 + r < M && n < n1 ? lb_load(dy[n * M + m0 + r]) : 0.f; },
-        [&](int c, long long n) {
-            const int k = c0 + c;
-            if (n >= n1 || k > K) return 0.f;
-            if (k == K) return 1.f;
-            const unsigned wd = kp.codes[(size_t)n * kp.kp + k];
-            return lb_decode4<FMT>(wd).x * kp.scales[(size_t)n * (kp.kp / 64) + (k >> 6)];
-        },
-        [&](int r, int c, float v) { if (m0 + r < M && c0 + c <= K) partial[((size_t)blockIdx.x * M + m0 + r) * (K + 1) + c0 + c] = v; });
-}
-
+// a NaN with its sign bit set would be rectified away
 template <typename T>
-__global__ __launch_bounds__(256) void linear8_dw_sum_kernel(int K, int M, int chunks, const float* __restrict__ partial,
-                                                             T* __restrict__ dw, T* __restrict__ db)
+__device__ __forceinline__ void positive_nans(Group<T>& g)
 {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x, total = (long long)M * (K + 1);
-    if (e >= total) return;
+    unsigned* e = reinterpret_cast<unsigned*>(&g);
+#pragma unroll
+    for (int q = 0; q < (int)(sizeof(g) / 4); q++) {
+        if constexpr (sizeof(T) == 4) {
+            if ((e[q] & 0x7fffffffu) > 0x7f800000u) e[q] &= 0x7fffffffu;
+        } else {
+            constexpr unsigned kInf = __is_same(T, LbF16) ? 0x7c00u : 0x7f80u;
+            if ((e[q] & 0x7fffu) > kInf) e[q] &= 0xffff7fffu;
+            if ((e[q] >> 16 & 0x7fffu) > kInf) e[q] &= 0x7fffffffu;
+        }
+    }
+}
+
+struct RowsArgs {
+    long long N; int C, F;                // rows, contraction length, features of the result
+    const void* x; long long ldx;
+    const void* w; long long wf, wc;      // element (feature f, contraction c) of the weight: w[f * wf + c * wc]
+    const void* bias;
+    void* y;                              // [N][F]
+    int lowest;                           // relu_bits()
+    Keep keep; int fmt;                   // forward: what to keep; dx: keep.bits masks the result
+    int ncb, nwg, groups, chunk;          // column blocks, workgroups per column block, groups of 64 of the contraction, groups in LDS at once
+};
+
+// Both products over the rows, y^T[feature][row] = W x^T (+ bias) and dx^T = W^T dy^T: a wave owns 32 rows, which are the columns
+// of v_mfma_f32_32x32x16, and NT tiles of 32 features; a lane streams its row from memory in groups of 64 columns (the next group
+// is in flight while this one is multiplied) and ends up with quads of neighbouring features of that row.  The weight lies in LDS
+// as MFMA operands, split once per workgroup, for as many groups as fit; a workgroup of 8 waves walks the rows in steps of
+// 8 * nwg tiles.  What the backward needs of x is quantised on the way, from the registers that feed the product: x is read once.
+template <typename T, int NT, bool VEC, bool DX>
+__global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
+{
+    constexpr int TERMS = kTerms<T>;
+    extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane]
+    __shared__ float s_bias[NT * 32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
+    // workgroups that share rows differ by 8 in their number, i.e. run on one XCD behind one L2
+    int cb, wg;
+    if ((a.nwg & 7) == 0) {
+        const int rest = blockIdx.x >> 3;
+        cb = rest % a.ncb;
+        wg = (rest / a.ncb) * 8 + (blockIdx.x & 7);
+    } else {
+        cb = blockIdx.x % a.ncb;
+        wg = blockIdx.x / a.ncb;
+    }
+    const int f0 = cb * NT * 32, C = a.C, F = a.F;
+    const T* __restrict__ X = (const T*)a.x;
+    const T* __restrict__ W = (const T*)a.w;
+    if (tid < NT * 32) s_bias[tid] = !DX && a.bias && f0 + tid < F ? lb_load(((const T*)a.bias)[f0 + tid]) : 0.f;
+    auto stage = [&](int g0, int n) {                     // groups g0 .. g0 + n - 1 of the weight
+        for (int e = tid; e < n * 4 * NT * 64; e += 512) {
+            const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
+            const int f = f0 + nt * 32 + (l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
+            const T* p = W + (long long)min(f, F - 1) * a.wf;
+            if constexpr (sizeof(T) == 4) {
+                float v[8];
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const float u = p[(long long)min(c + q, C - 1) * a.wc];
+                    v[q] = f < F && c + q < C ? u : 0.f;
+                }
+                uint4 o[TERMS];
+                split8<TERMS, true>(v, o);
+#pragma unroll
+                for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
+            } else {
+                unsigned v[8];
+                const unsigned short* ps = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const unsigned u = ps[(long long)min(c + q, C - 1) * a.wc];
+                    v[q] = f < F && c + q < C ? u : 0u;
+                }
+                s_w[(step * NT + nt) * 64 + l] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+            }
+        }
+    };
+    if (a.chunk >= a.groups) stage(0, a.groups);
+    __syncthreads();
+
+    const int ntile = (int)((a.N + 31) >> 5);
+    const bool keeping = !DX && cb == 0 && (a.keep.codes || a.keep.bits);
+    auto row_of = [&](long long tile) { const long long r = tile * 32 + j; return X + (r < a.N ? r : a.N - 1) * a.ldx; };
+    Group<T> cur, nxt;
+    long long tile = (long long)wave * a.nwg + wg;
+    load_group<T, VEC>(cur, row_of(tile), 8 * h, C);
+    for (long long base = 0; base * a.nwg < ntile; base += 8, tile += 8ll * a.nwg) {      // uniform: every wave takes part in the barriers
+        const long long row = tile * 32 + j;
+        const bool live = row < a.N;
+        f32x16 acc[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[nt][r] = s_bias[nt * 32 + (r & 3) + 8 * (r >> 2) + 4 * h];
+        for (int g = 0; g < a.groups; g++) {
+            if (a.chunk < a.groups && g % a.chunk == 0) {
+                __syncthreads();
+                stage(g, min(a.chunk, a.groups - g));
+                __syncthreads();
+            }
+            load_group<T, VEC>(nxt, g + 1 < a.groups ? row_of(tile) : row_of(tile + 8ll * a.nwg), g + 1 < a.groups ? (g + 1) * 64 + 8 * h : 8 * h, C);
+            if (g * 64 + 64 > C) clear_past(cur, g * 64 + 8 * h, C);
+            const uint4* __restrict__ wl = s_w + (size_t)(g % a.chunk) * 4 * NT * TERMS * 64 + lane;
+            // the group's largest number (of the kept values) and whether anything in it is no finite number
+            unsigned m = 0, odd = 0;
+            float v[4][8];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int t = 0; t < 8; t++) odd = max(max(odd, max(cur.w[t].x & 0x7fffffffu, cur.w[t].y & 0x7fffffffu)), max(cur.w[t].z & 0x7fffffffu, cur.w[t].w & 0x7fffffffu));
+                odd = odd >= 0x7f800000u;
+            } else {
+                unsigned o2 = 0;
+#pragma unroll
+                for (int t = 0; t < 4; t++) o2 = max_u16x2(max_u16x2(o2, max_u16x2(cur.w[t].x & 0x7fff7fffu, cur.w[t].y & 0x7fff7fffu)), max_u16x2(cur.w[t].z & 0x7fff7fffu, cur.w[t].w & 0x7fff7fffu));
+                odd = max(o2 & 0xffffu, o2 >> 16) >= (__is_same(T, LbF16) ? 0x7c00u : 0x7f80u);
+            }
+            const bool rare = __builtin_amdgcn_ballot_w64(odd) != 0;
+            if (rare && !DX) positive_nans(cur);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const unsigned* e = reinterpret_cast<const unsigned*>(&cur.w[2 * t]);
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const unsigned r = DX ? e[q] : relu_bits(e[q], a.lowest);
+                        m = max(m, r & 0x7fffffffu);
+                        v[t][q] = __uint_as_float(r);
+                    }
+                }
+            } else if constexpr (!DX) {
+                const unsigned low2 = a.lowest ? 0x80008000u : 0u;
+                unsigned m2 = 0;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    unsigned* e = reinterpret_cast<unsigned*>(&cur.w[t]);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        e[q] = relu_bits2(e[q], low2);
+                        m2 = max_u16x2(m2, e[q] & 0x7fff7fffu);
+                    }
+                }
+                m = __float_as_uint(low16<T>(max(m2 & 0xffffu, m2 >> 16)));
+            }
+            if (keeping) {
+                unsigned bits = 0;
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const unsigned* e = reinterpret_cast<const unsigned*>(&cur.w[t]);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) { v[t][2 * q] = low16<T>(e[q]); v[t][2 * q + 1] = high16<T>(e[q]); }
+                    }
+                }
+                if (a.keep.bits) {                        // relu: every number is at least 0 here
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int q = 0; q < 8; q++) bits |= min(__float_as_uint(v[t][q]), 1u) << (8 * t + q);
+                    // byte 2 t + h of the group's 8 holds step t: the halves' bytes alternate
+                    const unsigned other = (unsigned)__shfl_xor((int)bits, 32, 64);
+                    const unsigned ev = h ? other : bits, od = h ? bits : other;
+                    uint2 w;
+                    w.x = (ev & 255u) | (od & 255u) << 8 | (ev >> 8 & 255u) << 16 | (od >> 8 & 255u) << 24;
+                    w.y = (ev >> 16 & 255u) | (od >> 16 & 255u) << 8 | (ev >> 24) << 16 | (od >> 24) << 24;
+                    if (live && h == 0) *reinterpret_cast<uint2*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + g * 8) = w;
+                }
+                if (a.keep.codes) {
+                    m = max(m, (unsigned)__shfl_xor((int)m, 32, 64));
+                    unsigned char* code = a.keep.codes + (size_t)row * a.keep.kp + g * 64 + 8 * h;
+                    auto encode = [&](auto f) {
+                        constexpr int FMT = decltype(f)::value;
+                        const LbScale sc = lb_scale<FMT>(m);
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            uint2 w;
+                            w.x = lb_encode4<FMT>(v[t][0] * sc.inv, v[t][1] * sc.inv, v[t][2] * sc.inv, v[t][3] * sc.inv);
+                            w.y = lb_encode4<FMT>(v[t][4] * sc.inv, v[t][5] * sc.inv, v[t][6] * sc.inv, v[t][7] * sc.inv);
+                            if (live) *reinterpret_cast<uint2*>(code + 16 * t) = w;
+                        }
+                        if (live && h == 0) a.keep.scales[(size_t)row * (a.keep.kp / 64) + g] = sc.s;
+                    };
+                    if (a.fmt == GS4D_FMT_INT8) encode(Int<GS4D_FMT_INT8>());
+                    else if (a.fmt == GS4D_FMT_UINT8) encode(Int<GS4D_FMT_UINT8>());
+                    else if (a.fmt == GS4D_FMT_E4M3) encode(Int<GS4D_FMT_E4M3>());
+                    else encode(Int<GS4D_FMT_E5M2>());
+                }
+            }
+            auto multiply = [&](auto safe) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    uint4 xs[TERMS];
+                    if constexpr (sizeof(T) == 4) split8<TERMS, decltype(safe)::value != 0>(v[t], xs);
+                    else xs[0] = cur.w[t];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        uint4 ws[TERMS];
+#pragma unroll
+                        for (int u = 0; u < TERMS; u++) ws[u] = wl[((t * NT + nt) * TERMS + u) * 64];
+#pragma unroll
+                        for (int u = TERMS - 1; u >= 0; u--)                  // the smallest products first
+#pragma unroll
+                            for (int z = 0; z <= u; z++) acc[nt] = mfma<T>(ws[z], xs[u - z], acc[nt]);
+                    }
+                }
+            };
+            if (sizeof(T) == 4 && rare) multiply(Int<1>());
+            else multiply(Int<0>());
+            cur = nxt;
+        }
+        // ---- a quad of features per (tile, register quad)
+        if (live) {
+            T* __restrict__ y = (T*)a.y + row * F + f0;
+            const bool quads = (F & 3) == 0 && ((uintptr_t)a.y & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                unsigned mask = 0xffffffffu;
+                if (DX && a.keep.bits && f0 + nt * 32 < F)
+                    mask = *reinterpret_cast<const unsigned*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + (f0 >> 3) + 4 * nt);
+#pragma unroll
+                for (int mq = 0; mq < 4; mq++) {
+                    const int f = nt * 32 + 8 * mq + 4 * h;
+                    T o[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) o[q] = lb_store<T>(!DX || (mask >> (8 * mq + 4 * h + q) & 1u) ? acc[nt][4 * mq + q] : 0.f);
+                    if (quads) {
+                        if (f0 + f < F) {
+                            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y + f) = make_float4(o[0], o[1], o[2], o[3]);
+                            else *reinterpret_cast<uint2*>(y + f) = *reinterpret_cast<const uint2*>(o);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            if (f0 + f + q < F) y[f + q] = o[q];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// dW[m][k] = sum over rows r of dy[r][m] s[r] c[r][k] with the kept codes c and their group's scale s.  The contraction runs over
+// the ROWS, and any 8 rows may be the 8 elements a lane supplies as long as both operands agree: a lane loads column pairs
+// (2 i, 2 i + 1) of dy and of the codes straight from memory, row after row, coalesced, and no transposition through LDS is needed.
+// Tile t of the result then holds the columns 2 i + t.  The codes are exact in bfloat16 (8 significant bits), so the rounding
+// lies in dy s alone, which is split into TERMS bfloat16 numbers: three are its 24 bits.
+// A workgroup: 64 columns m, GW groups of 64 columns k (a wave each) and 8 / GW row slices per group, summed through LDS;
+// one slab of partial sums per workgroup.
+struct DwArgs {
+    long long N; int K, M;
+    const void* dy; Keep keep;
+    long long per;                        // rows per chunk
+    int gw, groups, mtiles, chunks;
+    float* slabs;                         // [chunk][m tile][group][64 registers][64 lanes], then [chunk][m tile][64] of db
+};
+
+template <typename T, int FMT, int TERMS, bool VEC>
+__global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
+{
+    __shared__ float s_red[4][64 * 64];
+    __shared__ float s_db[8][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
+    const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks, mt = rest % a.mtiles, z = rest / a.mtiles;
+    const int g = z * a.gw + wave % a.gw, slice = wave / a.gw, slices = 8 / a.gw;
+    const long long n0 = chunk * a.per, n1 = n0 + a.per < a.N ? n0 + a.per : a.N;
+    const bool mine = g < a.groups;
+    const int gc = min(g, a.groups - 1), m = mt * 64 + 2 * i, kp = a.keep.kp, ng = kp / 64;
+    const T* __restrict__ dy = (const T*)a.dy + (VEC ? min(m, a.M - 2) : min(m, a.M - 1));
+    const int second = m + 1 < a.M ? 1 : 0;
+    const unsigned char* __restrict__ codes = a.keep.codes + gc * 64 + 2 * i;
+    const float* __restrict__ scales = a.keep.scales + gc;
+    struct Rows { unsigned d[8][sizeof(T) / 2]; unsigned short c[8]; float s[8]; };
+    auto load = [&](Rows& r, long long r0) {
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const long long n = r0 + 8 * h + q, row = n < a.N ? n : a.N - 1;
+            const T* p = dy + row * a.M;
+            if constexpr (sizeof(T) == 4) {
+                if constexpr (VEC) { const uint2 w = *reinterpret_cast<const uint2*>(p); r.d[q][0] = w.x; r.d[q][1] = w.y; }
+                else { r.d[q][0] = __float_as_uint(p[0]); r.d[q][1] = __float_as_uint(p[second]); }
+            } else {
+                if constexpr (VEC) r.d[q][0] = *reinterpret_cast<const unsigned*>(p);
+                else { const unsigned short* u = reinterpret_cast<const unsigned short*>(p); r.d[q][0] = u[0] | (unsigned)u[second] << 16; }
+            }
+            r.c[q] = *reinterpret_cast<const unsigned short*>(codes + (size_t)row * kp);
+            r.s[q] = scales[(size_t)row * ng];
+        }
+    };
+    f32x16 acc[2][2] = {};
+    float db0 = 0.f, db1 = 0.f;
+    Rows cur, nxt;
+    const long long first = n0 + 16 * slice, stride = 16ll * slices;
+    if (mine && first < n1) load(cur, first);
+    if (mine)
+        for (long long r0 = first; r0 < n1; r0 += stride) {
+            load(nxt, r0 + stride);
+            float d0[8], d1[8], c0[8], c1[8];
+            const bool whole = r0 + 16 <= n1;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                if constexpr (sizeof(T) == 4) { d0[q] = __uint_as_float(cur.d[q][0]); d1[q] = __uint_as_float(cur.d[q][1]); }
+                else { d0[q] = low16<T>(cur.d[q][0]); d1[q] = high16<T>(cur.d[q][0]); }
+                const bool in = whole || r0 + 8 * h + q < n1;
+                if (!in) { d0[q] = 0.f; d1[q] = 0.f; cur.s[q] = 0.f; }
+                db0 += d0[q]; db1 += d1[q];
+                d0[q] *= cur.s[q]; d1[q] *= cur.s[q];
+                if constexpr (FMT == GS4D_FMT_E4M3 || FMT == GS4D_FMT_E5M2) {
+                    const float4 f = lb_decode4<FMT>(cur.c[q]);
+                    c0[q] = f.x; c1[q] = f.y;
+                } else if constexpr (FMT == GS4D_FMT_UINT8) { c0[q] = (float)(cur.c[q] & 255u); c1[q] = (float)(cur.c[q] >> 8); }
+                else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
+            }
+            uint4 da[2][TERMS], cc[2][1];
+            split8<TERMS, false>(d0, da[0]);
+            split8<TERMS, false>(d1, da[1]);
+            split8<1, false>(c0, cc[0]);
+            split8<1, false>(c1, cc[1]);
+#pragma unroll
+            for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) acc[t][y] = mfma<LbBf16>(da[t][u], cc[y][0], acc[t][y]);
+            cur = nxt;
+        }
+    // ---- the slices of a group, in a fixed order: the upper half adds to the lower half until one is left
+    for (int n = slices; n > 1; n >>= 1) {
+        const int half = n >> 1;
+        __syncthreads();
+        if (slice >= half && slice < n) {
+            float* p = s_red[(slice - half) * a.gw + wave % a.gw];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) p[((t * 2 + y) * 16 + r) * 64 + lane] = acc[t][y][r];
+        }
+        __syncthreads();
+        if (slice < half) {
+            const float* p = s_red[slice * a.gw + wave % a.gw];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[t][y][r] += p[((t * 2 + y) * 16 + r) * 64 + lane];
+        }
+    }
+    const size_t cell = (size_t)chunk * a.mtiles + mt;
+    if (slice == 0 && mine) {
+        float* p = a.slabs + (cell * a.groups + g) * 4096;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int y = 0; y < 2; y++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) p[((t * 2 + y) * 16 + r) * 64 + lane] = acc[t][y][r];
+    }
+    if (z == 0) {                                         // db: the waves of group 0 have the column sums of their slices
+        db0 += __shfl_xor(db0, 32, 64);
+        db1 += __shfl_xor(db1, 32, 64);
+        if (h == 0) { s_db[wave][2 * i] = db0; s_db[wave][2 * i + 1] = db1; }
+        __syncthreads();
+        if (tid < 64) {
+            float s = 0.f;
+            for (int q = 0; q < slices; q++) s += s_db[q * a.gw][tid];
+            a.slabs[(size_t)a.chunks * a.mtiles * a.groups * 4096 + cell * 64 + tid] = s;
+        }
+    }
+}
+
+// db alone (a frozen weight): the same sums in the same order as linear8_dw_kernel's, so that freezing changes no bit of them
+template <typename T>
+__global__ __launch_bounds__(512) void linear8_db_kernel(DwArgs a)
+{
+    __shared__ float s_db[8][64];
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, i = lane & 31, h = lane >> 5, slices = 8 / a.gw;
+    const int chunk = blockIdx.x % a.chunks, mt = blockIdx.x / a.chunks;
+    const long long n0 = chunk * a.per, n1 = n0 + a.per < a.N ? n0 + a.per : a.N;
+    const int m0 = min(mt * 64 + 2 * i, a.M - 1), m1 = min(mt * 64 + 2 * i + 1, a.M - 1);
+    const T* __restrict__ dy = (const T*)a.dy;
+    float d0 = 0.f, d1 = 0.f;
+    if (slice < slices)
+        for (long long r0 = n0 + 16 * slice; r0 < n1; r0 += 16ll * slices) {
+            float v0[8], v1[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const long long n = r0 + 8 * h + q, row = n < a.N ? n : a.N - 1;
+                v0[q] = lb_load(dy[row * a.M + m0]);
+                v1[q] = lb_load(dy[row * a.M + m1]);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const bool in = r0 + 8 * h + q < n1;
+                d0 += in ? v0[q] : 0.f;
+                d1 += in ? v1[q] : 0.f;
+            }
+        }
+    d0 += __shfl_xor(d0, 32, 64);
+    d1 += __shfl_xor(d1, 32, 64);
+    if (h == 0) { s_db[slice][2 * i] = d0; s_db[slice][2 * i + 1] = d1; }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        float s = 0.f;
+        for (int q = 0; q < slices; q++) s += s_db[q][threadIdx.x];
+        a.slabs[((size_t)chunk * a.mtiles + mt) * 64 + threadIdx.x] = s;
+    }
+}
+
+// The slabs' sum, chunks in a fixed order (8 runs of them side by side), to the caller's arrays.
+template <typename T>
+__global__ __launch_bounds__(256) void linear8_dw_sum_kernel(DwArgs a, T* __restrict__ dw, T* __restrict__ db)
+{
+    __shared__ float part[8][32];
+    const int o = threadIdx.x & 31, q = threadIdx.x >> 5;
+    const long long cells = (long long)a.mtiles * a.groups * 4096, total = cells + a.mtiles * 64, e = (long long)blockIdx.x * 32 + o;
+    const bool bias = e >= cells;
+    const float* __restrict__ p = bias ? a.slabs + a.chunks * cells + (min(e, total - 1) - cells) : a.slabs + e;
+    const long long step = bias ? a.mtiles * 64 : cells;
+    const int per = (a.chunks + 7) / 8, c0 = q * per, c1 = min(a.chunks, c0 + per);
     float s = 0.f;
-    for (int c = 0; c < chunks; c++) s += partial[(size_t)c * total + e];
-    const int m = (int)(e / (K + 1)), k = (int)(e % (K + 1));
-    if (k < K) { if (dw) dw[(size_t)m * K + k] = lb_store<T>(s); }
-    else if (db) db[m] = lb_store<T>(s);
+    for (int c = c0; c < c1; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = p[min(c + u, c1 - 1) * step];
+#pragma unroll
+        for (int u = 0; u < 8; u++) s += c + u < c1 ? v[u] : 0.f;
+    }
+    part[q][o] = s;
+    __syncthreads();
+    if (q != 0 || e >= total) return;
+    s = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; u++) s += part[u][o];
+    if (bias) {
+        const int m = (int)(e - cells);
+        if (db && m < a.M) db[m] = lb_store<T>(s);
+    } else if (dw) {
+        const int lane = (int)(e & 63), r = (int)(e >> 6) & 15, y = (int)(e >> 10) & 1, t = (int)(e >> 11) & 1;
+        const int g = (int)((e >> 12) % a.groups), mt = (int)((e >> 12) / a.groups);
+        const int m = mt * 64 + 2 * ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + t, k = g * 64 + 2 * (lane & 31) + y;
+        if (m < a.M && k < a.K) dw[(size_t)m * a.K + k] = lb_store<T>(s);
+    }
 }
 
-static long long dw_chunks(long long N) { return N <= 0 ? 1 : (N + 2047) / 2048 < 256 ? (N + 2047) / 2048 : 256; }
+#define LB_CUS 256
+
+// how the weight gradient is cut: about one workgroup per CU, but at least 128 rows per chunk
+static DwArgs dw_plan(long long N, int K, int M)
+{
+    DwArgs a = {};
+    a.N = N; a.K = K; a.M = M;
+    a.mtiles = (M + 63) / 64;
+    a.groups = (K + 63) / 64;
+    a.gw = a.groups >= 8 ? 8 : a.groups >= 4 ? 4 : a.groups >= 2 ? 2 : 1;
+    const long long blocks = (long long)a.mtiles * ((a.groups + a.gw - 1) / a.gw);
+    long long chunks = blocks >= LB_CUS ? 1 : LB_CUS / blocks;
+    if (chunks > (N + 127) / 128) chunks = (N + 127) / 128;
+    if (chunks < 1) chunks = 1;
+    a.per = ((N + chunks - 1) / chunks + 127) / 128 * 128;
+    if (a.per < 128) a.per = 128;
+    a.chunks = (int)((N + a.per - 1) / a.per);
+    if (a.chunks < 1) a.chunks = 1;
+    return a;
+}
 
 static int check_cache(const gs4d_rows8* c, const char* who)
 {
@@ -257,17 +735,6 @@ static int check_rows(const gs4d_rows8* c, const void* rows, int dtype, long lon
         return GS4D_EINVAL;
     }
     return GS4D_OK;
-}
-
-template <typename F> static int by_type(int dtype, F f)
-{
-    return dtype == GS4D_F32 ? f(float()) : dtype == GS4D_BF16 ? f(LbBf16()) : f(LbF16());
-}
-template <int V> struct Int { static constexpr int value = V; };
-template <typename F> static int by_fmt(int fmt, F f)
-{
-    return fmt == GS4D_FMT_INT8 ? f(Int<GS4D_FMT_INT8>()) : fmt == GS4D_FMT_E4M3 ? f(Int<GS4D_FMT_E4M3>()) :
-           fmt == GS4D_FMT_E5M2 ? f(Int<GS4D_FMT_E5M2>()) : f(Int<GS4D_FMT_UINT8>());
 }
 
 }  // namespace
@@ -351,8 +818,69 @@ size_t gs4d_linear8_keep_bytes(long long N, int K, int what)
 size_t gs4d_linear8_scratch_bytes(long long N, int K, int M)
 {
     if (N < 0 || K < 1 || M < 1) return 0;
-    return (size_t)dw_chunks(N) * M * ((size_t)K + 1) * sizeof(float) + 256;
+    const DwArgs a = dw_plan(N, K, M);
+    return (size_t)a.chunks * a.mtiles * ((size_t)a.groups * 4096 + 64) * sizeof(float) + 256;
 }
+
+}  // extern "C"
+
+namespace {
+
+// the products over the rows: NT tiles of 32 features per wave and as many groups of the weight in LDS as fit
+template <typename T, bool DX>
+static int launch_rows(RowsArgs& a, hipStream_t s)
+{
+    constexpr int LDS = 144 * 1024;
+    const bool vec = a.C % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.ldx * sizeof(T)) % 16 == 0;
+    const int most = sizeof(T) == 4 ? 2 : 4, nt = a.F <= 32 ? 1 : a.F <= 64 || most == 2 ? 2 : 4;
+    a.groups = (a.C + 63) / 64;
+    const int per = 4 * nt * kTerms<T> * 1024;
+    a.chunk = LDS / per < a.groups ? LDS / per : a.groups;
+    const size_t lds = (size_t)a.chunk * per;
+    a.ncb = (a.F + nt * 32 - 1) / (nt * 32);
+    const long long ntile = (a.N + 31) / 32;
+    long long nwg = LB_CUS * (lds <= 72 * 1024 ? 2 : 1) / a.ncb;
+    if (nwg > ntile) nwg = ntile;
+    if (nwg < 1) nwg = 1;
+    if (nwg >= 8) nwg = nwg / 8 * 8;
+    a.nwg = (int)nwg;
+    auto launch = [&](auto n, auto v) {
+        auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX>;
+        if (lds > 64 * 1024) GS4D_HIP_CHECK(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        hipLaunchKernelGGL(k, dim3((unsigned)(a.nwg * a.ncb)), dim3(512), lds, s, a);
+        return GS4D_OK;
+    };
+    auto with_nt = [&](auto n) { return vec ? launch(n, Int<1>()) : launch(n, Int<0>()); };
+    if constexpr (sizeof(T) == 2) { if (nt == 4) return with_nt(Int<4>()); }
+    return nt == 1 ? with_nt(Int<1>()) : with_nt(Int<2>());
+}
+
+template <typename T>
+static int launch_dw(DwArgs& a, int fmt, void* dw, void* db, hipStream_t s)
+{
+    if (dw) {
+        const bool vec = a.M % 2 == 0 && ((uintptr_t)a.dy & (2 * sizeof(T) - 1)) == 0;
+        const unsigned grid = (unsigned)(a.chunks * a.mtiles * ((a.groups + a.gw - 1) / a.gw));
+        by_fmt(fmt, [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3(grid), dim3(512), 0, s, a); };
+            // 16-bit results: two terms of dy s (2^-16 of a product) where the float32 sum over the rows is itself no better
+            if (sizeof(T) == 2 && a.N >= 1024) { if (vec) go(linear8_dw_kernel<T, F, 2, true>); else go(linear8_dw_kernel<T, F, 2, false>); }
+            else { if (vec) go(linear8_dw_kernel<T, F, 3, true>); else go(linear8_dw_kernel<T, F, 3, false>); }
+            return 0;
+        });
+    } else {
+        hipLaunchKernelGGL(linear8_db_kernel<T>, dim3((unsigned)(a.chunks * a.mtiles)), dim3(512), 0, s, a);
+        a.groups = 0;                                     // the slabs hold db alone
+    }
+    const long long total = (long long)a.mtiles * a.groups * 4096 + a.mtiles * 64;
+    hipLaunchKernelGGL(linear8_dw_sum_kernel<T>, dim3((unsigned)((total + 31) / 32)), dim3(256), 0, s, a, (T*)dw, (T*)db);
+    return GS4D_OK;
+}
+
+}  // namespace
+
+extern "C" {
 
 int gs4d_linear8_forward(int dtype, long long N, int K, int M, const void* x, long long ldx, const void* w, const void* b, int relu,
                          int fmt, void* y, char* keep, int what, void* stream)
@@ -365,22 +893,14 @@ int gs4d_linear8_forward(int dtype, long long N, int K, int M, const void* x, lo
         gs4d_set_error("gs4d_linear8_forward: null or misaligned pointer, or a row pitch below K");
         return GS4D_EINVAL;
     }
-    const Keep kp = what ? carve_keep(keep, N, K, what, nullptr) : Keep{};
-    const int kf = relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt;
-    by_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (what)
-            by_fmt(kf, [&](auto f) {
-                constexpr int F = decltype(f)::value;
-                const unsigned grid = (unsigned)(((size_t)N * (kp.kp / 8) + 255) / 256);
-                auto k = relu ? linear8_keep_kernel<F, true, T> : linear8_keep_kernel<F, false, T>;
-                hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, s, kp, (const T*)x, ldx, N, K);
-                return 0;
-            });
-        auto k = relu ? linear8_forward_kernel<true, T> : linear8_forward_kernel<false, T>;
-        hipLaunchKernelGGL(k, dim3((unsigned)((N + 63) / 64), (M + 63) / 64), dim3(256), 0, s, N, K, M, (const T*)x, ldx, (const T*)w, (const T*)b, (T*)y);
-        return 0;
-    });
+    RowsArgs a = {};
+    a.N = N; a.C = K; a.F = M;
+    a.x = x; a.ldx = ldx; a.w = w; a.wf = K; a.wc = 1; a.bias = b; a.y = y;
+    a.lowest = relu ? 0 : (int)0x80000000;
+    if (what) a.keep = carve_keep(keep, N, K, what, nullptr);
+    a.fmt = relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt;
+    const int rc = by_type(dtype, [&](auto t) { return launch_rows<decltype(t), false>(a, s); });
+    if (rc) return rc;
     GS4D_LAUNCH_CHECK("linear8_forward", 0, s);
     return GS4D_OK;
 }
@@ -397,25 +917,22 @@ int gs4d_linear8_backward(int dtype, long long N, int K, int M, const void* dy, 
         return GS4D_EINVAL;
     }
     const Keep kp = what && keep ? carve_keep(keep, N, K, what, nullptr) : Keep{};
-    Keep masked = kp;
-    if (!relu) masked.bits = nullptr;
-    const int kf = relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt;
-    by_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (dx && N > 0)
-            hipLaunchKernelGGL(linear8_dx_kernel<T>, dim3((unsigned)((N + 63) / 64), (K + 63) / 64), dim3(256), 0, s, N, K, M, (const T*)dy, (const T*)w, masked, (T*)dx);
-        if (dw || db) {
-            const int chunks = (int)dw_chunks(N), Kw = dw ? K : 0;       // without dw: the bias column alone
-            const long long per = (N + chunks - 1) / chunks;
-            by_fmt(kf, [&](auto f) {
-                constexpr int F = decltype(f)::value;
-                hipLaunchKernelGGL((linear8_dw_kernel<F, T>), dim3(chunks, (M + 63) / 64, (Kw + 64) / 64), dim3(256), 0, s, N, Kw, M, (const T*)dy, kp, per, (float*)scratch);
-                return 0;
-            });
-            hipLaunchKernelGGL(linear8_dw_sum_kernel<T>, dim3((unsigned)(((size_t)M * (Kw + 1) + 255) / 256)), dim3(256), 0, s, Kw, M, chunks, (const float*)scratch, (T*)dw, (T*)db);
-        }
-        return 0;
-    });
+    int rc = GS4D_OK;
+    if (dx && N > 0) {
+        RowsArgs a = {};
+        a.N = N; a.C = M; a.F = K;
+        a.x = dy; a.ldx = M; a.w = w; a.wf = 1; a.wc = K; a.y = dx;
+        a.lowest = (int)0x80000000;
+        if (relu) a.keep = kp;
+        rc = by_type(dtype, [&](auto t) { return launch_rows<decltype(t), true>(a, s); });
+        if (rc) return rc;
+    }
+    if (dw || db) {
+        DwArgs a = dw_plan(N, K, M);
+        a.dy = dy; a.keep = kp; a.slabs = (float*)scratch;
+        rc = by_type(dtype, [&](auto t) { return launch_dw<decltype(t)>(a, relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt, dw, db, s); });
+        if (rc) return rc;
+    }
     GS4D_LAUNCH_CHECK("linear8_backward", 0, s);
     return GS4D_OK;
 }
