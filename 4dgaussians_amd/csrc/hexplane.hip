@@ -8,6 +8,7 @@
 //   scene/deformation.py:128-141                    t' = force_time_embed([t, f])
 #include <stdlib.h>
 #include <string.h>
+#include <type_traits>
 
 #include "deform_hexplane.h"
 #include "lowbit.h"
@@ -206,6 +207,83 @@ __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L
             acc.w *= f00.w * n.w00 + f01.w * n.w01 + f10.w * n.w10 + f11.w * n.w11;
         }
         reinterpret_cast<float4*>(out + p * ld + l * C)[sub] = acc;
+    }
+}
+
+// The same with ONE t for all points: a plane over (axis, t) is then a line over the axis, the two rows around t blended.  A
+// workgroup blends the lines of its `slice` channels into LDS once and walks the points with half the corner rows, all of them in
+// LDS: what is left to memory is the cache row, the point and the result.  slice / 4 lanes per point, 4 channels of every level
+// each; workgroups that share points (other slices) differ by 8 in their number, i.e. sit behind one L2.
+#define FRAME_LINES_MIN 65536         // points * channels from which the lines pay
+struct FrameArgs {
+    gs4d_rows8 c; int L, C, slice, nslices, nwg, gshift;
+    FramePlanes T; int row0[GS4D_MAX_LEVELS * 3];        // first LDS row of a line
+    const float* aabb; const float* xyz; const float* t; long long P; float* out; long long ld;
+};
+
+template <int FMT, int L>
+__global__ __launch_bounds__(512) void frame_lines_kernel(FrameArgs a)
+{
+    extern __shared__ float4 s_line[];                    // [row][slice / 4]
+    const int lanes = a.slice >> 2, shift = __builtin_ctz(lanes);
+    const int rest = blockIdx.x >> 3, sl = (a.nwg & 7) ? blockIdx.x % a.nslices : rest % a.nslices;
+    const int wg = (a.nwg & 7) ? blockIdx.x / a.nslices : (rest / a.nslices) * 8 + (blockIdx.x & 7);
+    const int ch0 = sl * a.slice;
+    const float tt = a.t[0];
+    for (int i = 0; i < 3 * L; i++) {
+        const int H = a.T.h[i], W = a.T.w[i];
+        const float y = fminf(fmaxf((tt + 1.f) * 0.5f * (float)(H - 1), 0.f), (float)(H - 1)), y0 = floorf(y), wy = y - y0;
+        const int j0 = (int)y0, j1 = min(j0 + 1, H - 1);
+        for (int e = threadIdx.x; e < W << shift; e += 512) {
+            const int x = e >> shift, q = e & (lanes - 1);
+            const float4 lo = *reinterpret_cast<const float4*>(a.T.p[i] + ((size_t)j0 * W + x) * a.C + ch0 + 4 * q);
+            const float4 hi = *reinterpret_cast<const float4*>(a.T.p[i] + ((size_t)j1 * W + x) * a.C + ch0 + 4 * q);
+            s_line[((a.row0[i] + x) << shift) + q] = make_float4(lo.x * (1.f - wy) + hi.x * wy, lo.y * (1.f - wy) + hi.y * wy,
+                                                                 lo.z * (1.f - wy) + hi.z * wy, lo.w * (1.f - wy) + hi.w * wy);
+        }
+    }
+    float lo3[3], sc3[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) { lo3[k] = a.aabb[k]; sc3[k] = 2.0f / (a.aabb[3 + k] - lo3[k]); }
+    __syncthreads();
+    const int sub = threadIdx.x & (lanes - 1), ppw = 512 >> shift, ng = (a.c.width + a.c.group - 1) >> a.gshift;
+    struct Point { float x[3], s[L]; unsigned k[L]; } cur, nxt;
+    auto load = [&](Point& o, long long p) {
+        p = p < a.P ? p : a.P - 1;
+#pragma unroll
+        for (int k = 0; k < 3; k++) o.x[k] = a.xyz[3 * p + k];
+#pragma unroll
+        for (int l = 0; l < L; l++) {
+            const int col = l * a.C + ch0 + 4 * sub;
+            o.k[l] = *reinterpret_cast<const unsigned*>(a.c.codes + (size_t)p * a.c.pitch + col);
+            o.s[l] = a.c.scales[p * ng + (col >> a.gshift)];
+        }
+    };
+    long long p = (long long)wg * ppw + (threadIdx.x >> shift);
+    load(cur, p);
+    for (; p < a.P; p += (long long)a.nwg * ppw) {
+        load(nxt, p + (long long)a.nwg * ppw);
+        float u[3];
+#pragma unroll
+        for (int k = 0; k < 3; k++) u[k] = (cur.x[k] - lo3[k]) * sc3[k] - 1.0f;
+#pragma unroll
+        for (int l = 0; l < L; l++) {
+            const float4 k4 = lb_decode4<FMT>(cur.k[l]);
+            float4 acc = make_float4(cur.s[l] * k4.x, cur.s[l] * k4.y, cur.s[l] * k4.z, cur.s[l] * k4.w);
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const int W = a.T.w[3 * l + k];
+                const float x = fminf(fmaxf((u[k] + 1.f) * 0.5f * (float)(W - 1), 0.f), (float)(W - 1)), x0 = floorf(x), wx = x - x0;
+                const int i0 = (int)x0, i1 = min(i0 + 1, W - 1);
+                const float4 f0 = s_line[((a.row0[3 * l + k] + i0) << shift) + sub], f1 = s_line[((a.row0[3 * l + k] + i1) << shift) + sub];
+                acc.x *= f0.x * (1.f - wx) + f1.x * wx;
+                acc.y *= f0.y * (1.f - wx) + f1.y * wx;
+                acc.z *= f0.z * (1.f - wx) + f1.z * wx;
+                acc.w *= f0.w * (1.f - wx) + f1.w * wx;
+            }
+            *reinterpret_cast<float4*>(a.out + p * a.ld + l * a.C + ch0 + 4 * sub) = acc;
+        }
+        cur = nxt;
     }
 }
 
@@ -978,6 +1056,36 @@ extern "C" int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const floa
     for (int i = 0; i < L * 3; i++) {
         if (!planes[i] || ((uintptr_t)planes[i] & 15) || plane_w[i] < 1 || plane_h[i] < 1) { gs4d_set_error("gs4d_frame_features: plane %d null, empty or not 16-byte aligned", i); return GS4D_EINVAL; }
         T.p[i] = planes[i]; T.w[i] = plane_w[i]; T.h[i] = plane_h[i];
+    }
+    // one t and enough points to pay for the lines: about 10 us of blending per workgroup against 60 ns a point and CU
+    int rows = 0;
+    FrameArgs f = {};
+    for (int i = 0; i < L * 3; i++) { f.row0[i] = rows; rows += plane_w[i]; }
+    f.slice = C < 64 ? C : 64;
+    while (f.slice > 4 && (size_t)rows * f.slice * sizeof(float) > 78 * 1024) f.slice >>= 1;
+    const size_t lds = (size_t)rows * f.slice * sizeof(float);
+    if (t_stride == 0 && lds <= 78 * 1024 && (long long)P * C >= FRAME_LINES_MIN) {
+        f.c = *c; f.L = L; f.C = C; f.nslices = C / f.slice; f.T = T; f.aabb = aabb; f.xyz = points; f.t = t; f.P = P; f.out = out; f.ld = ld;
+        f.gshift = c->group == 32 ? 5 : c->group == 64 ? 6 : 7;
+        const long long ppw = 512 / (f.slice / 4), need = (P + ppw - 1) / ppw;
+        long long nwg = 512 / f.nslices;
+        if (nwg > need) nwg = need;
+        if (nwg >= 8) nwg = nwg / 8 * 8;
+        f.nwg = (int)(nwg < 1 ? 1 : nwg);
+        auto go = [&](auto kern) -> int {
+            if (lds > 64 * 1024) GS4D_HIP_CHECK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            hipLaunchKernelGGL(kern, dim3((unsigned)(f.nwg * f.nslices)), dim3(512), lds, s, f);
+            return GS4D_OK;
+        };
+        auto with_fmt = [&](auto lv) -> int {
+            constexpr int LV = decltype(lv)::value;
+            return c->fmt == GS4D_FMT_INT8 ? go(frame_lines_kernel<GS4D_FMT_INT8, LV>) : c->fmt == GS4D_FMT_E4M3 ? go(frame_lines_kernel<GS4D_FMT_E4M3, LV>) : go(frame_lines_kernel<GS4D_FMT_E5M2, LV>);
+        };
+        const int rc = L == 1 ? with_fmt(std::integral_constant<int, 1>()) : L == 2 ? with_fmt(std::integral_constant<int, 2>()) :
+                       L == 3 ? with_fmt(std::integral_constant<int, 3>()) : with_fmt(std::integral_constant<int, 4>());
+        if (rc) return rc;
+        GS4D_LAUNCH_CHECK("frame_lines", 0, s);
+        return GS4D_OK;
     }
     int lpp_shift = 0;
     while ((1 << lpp_shift) < C / 4) lpp_shift++;

@@ -4,44 +4,115 @@
 
 namespace {
 
-// ------------------------------------------------------------------ row cache
-// A thread owns 8 consecutive columns, so a group is 4, 8 or 16 neighbouring lanes and its maximum a few lane exchanges.  A
-// workgroup owns rpb rows; a row of more than 256 chunks is walked in steps of 256.
-template <int FMT, int LANES, typename T, typename S>
-__global__ __launch_bounds__(256) void rows8_write_kernel(gs4d_rows8 c, const T* __restrict__ rows, long long ld, long long n,
-                                                          const S* __restrict__ slots, long long start, int cpr, int rpb, int dup)
+// the two halves of a word as numbers of a 16-bit type
+template <typename T> __device__ __forceinline__ float low16(unsigned w)
 {
-    const int r = cpr >= 256 ? 0 : (int)threadIdx.x / cpr, ch0 = cpr >= 256 ? (int)threadIdx.x : (int)threadIdx.x % cpr;
-    const long long i = (long long)blockIdx.x * rpb + r;
-    if (r >= rpb || i >= n) return;
-    const long long slot = slots ? (long long)slots[i] : start + i;
-    if (slot < 0 || slot >= c.capacity) return;
-    if (dup == 1) {                                      // few rows: is this the last one of its slot?
-        for (long long j = i + 1; j < n; j++)
-            if ((long long)slots[j] == slot) return;
-    } else if (dup == 2) {
-        if (c.owner[slot] != (int)(i + 1)) return;
-    }
-    const T* __restrict__ x = rows + i * ld;
-    const int ng = (c.width + c.group - 1) / c.group;
-    for (int ch = ch0; ch < cpr; ch += 256) {
-        const int col = ch * 8;
-        float v[8];
-        unsigned m = 0;
+    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)w);
+    else return __uint_as_float(w << 16);
+}
+template <typename T> __device__ __forceinline__ float high16(unsigned w)
+{
+    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+    else return __uint_as_float(w & 0xffff0000u);
+}
+
+// ------------------------------------------------------------------ row cache
+// Both directions move 16 bytes of the caller's rows per lane and step (COLS = 4 float32 or 8 16-bit numbers, neighbouring lanes
+// neighbouring addresses; VEC: rows are 16-byte aligned) and their codes as one word or two.  A workgroup owns rpb rows, i.e.
+// about ROWS8_ITEMS (row, columns) items; item e of it is row e / cpr by a multiply-high (exact: e * cpr < 2^32).
+#define ROWS8_ITEMS 2048
+#define ROWS8_ROWS 256
+
+// the maximum over the LANES neighbouring lanes of a group: four steps within 16 lanes, then across
+template <int LANES> __device__ __forceinline__ unsigned group_max(unsigned m)
+{
+    if constexpr (LANES > 1) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));    // lane ^ 1
+    if constexpr (LANES > 2) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));    // lane ^ 2
+    if constexpr (LANES > 4) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true));   // mirrored in 8
+    if constexpr (LANES > 8) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, true));   // mirrored in 16
+    if constexpr (LANES > 16) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
+    return m;
+}
+
+// COLS consecutive numbers of a row from column col on; columns past width are zero
+template <typename T, int COLS, bool VEC>
+__device__ __forceinline__ void load_cols(float (&v)[COLS], const T* __restrict__ x, int col, int width)
+{
+    if (VEC) {                                            // width is a multiple of COLS
+        const uint4 w = *reinterpret_cast<const uint4*>(x + min(col, width - COLS));
+        const unsigned e[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int q = 0; q < 8; q++) {
-            v[q] = col + q < c.width ? lb_load(x[col + q]) : 0.f;
-            m = max(m, lb_abs_bits(v[q]));
+        for (int q = 0; q < COLS; q++) {
+            if constexpr (sizeof(T) == 4) v[q] = __uint_as_float(e[q]);
+            else v[q] = (q & 1) ? high16<T>(e[q >> 1]) : low16<T>(e[q >> 1]);
         }
 #pragma unroll
-        for (int s = 1; s < LANES; s <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, s, 64));
-        const LbScale sc = lb_scale<FMT>(m);
-        if (col < c.width) {
-            uint2 w;
-            w.x = lb_encode4<FMT>(v[0] * sc.inv, v[1] * sc.inv, v[2] * sc.inv, v[3] * sc.inv);
-            w.y = lb_encode4<FMT>(v[4] * sc.inv, v[5] * sc.inv, v[6] * sc.inv, v[7] * sc.inv);
-            *reinterpret_cast<uint2*>(c.codes + (size_t)slot * c.pitch + col) = w;
-            if ((ch & (LANES - 1)) == 0) c.scales[(size_t)slot * ng + ch / LANES] = sc.s;
+        for (int q = 0; q < COLS; q++) v[q] = col < width ? v[q] : 0.f;
+    } else {
+#pragma unroll
+        for (int q = 0; q < COLS; q++) v[q] = lb_load(x[min(col + q, width - 1)]);
+#pragma unroll
+        for (int q = 0; q < COLS; q++) v[q] = col + q < width ? v[q] : 0.f;
+    }
+}
+
+template <int FMT, int LANES, typename T, typename S, bool VEC>
+__global__ __launch_bounds__(256) void rows8_write_kernel(gs4d_rows8 c, const T* __restrict__ rows, long long ld, long long n,
+                                                          const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int dup)
+{
+    constexpr int COLS = 16 / (int)sizeof(T);
+    __shared__ long long s_slot[ROWS8_ROWS], s_all[GS4D_ROWS8_SCAN];
+    const long long i0 = (long long)blockIdx.x * rpb;
+    const int nrow = (int)min((long long)rpb, n - i0);
+    // where each row of this workgroup goes (-1: nowhere): one lane per row
+    if (dup == 1 && (int)threadIdx.x < n) s_all[threadIdx.x] = slots[threadIdx.x];
+    __syncthreads();
+    if ((int)threadIdx.x < nrow) {
+        const long long i = i0 + threadIdx.x;
+        long long slot = slots ? (long long)slots[i] : start + i;
+        if (slot < 0 || slot >= c.capacity) slot = -1;
+        if (dup == 1) {                                   // few rows: does a later one have the same slot?
+            bool last = true;
+            for (int j = 0; j < (int)n; j++) last = last && (j <= (int)i || s_all[j] != slot);
+            if (!last) slot = -1;
+        } else if (dup == 2 && slot >= 0) {
+            // rows8_owner_kernel left the last row's number.  It leaves the word zero again: a row that reads it later is not
+            // the last one either way
+            if (c.owner[slot] == (int)(i + 1)) c.owner[slot] = 0;
+            else slot = -1;
+        }
+        s_slot[threadIdx.x] = slot;
+    }
+    __syncthreads();
+    const int items = nrow * cpr, ng = (c.width + c.group - 1) / c.group;
+    constexpr int U = 4;
+    for (int e0 = threadIdx.x; e0 < items; e0 += 256 * U) {
+        float v[U][COLS];
+        int ch[U];
+        long long slot[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int e = min(e0 + 256 * u, items - 1);
+            const int r = cpr == 1 ? e : (int)__umulhi((unsigned)e, rcp);
+            ch[u] = e - r * cpr;
+            slot[u] = e0 + 256 * u < items ? s_slot[r] : -1;
+            load_cols<T, COLS, VEC>(v[u], rows + (i0 + r) * ld, ch[u] * COLS, c.width);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            unsigned m = 0;
+#pragma unroll
+            for (int q = 0; q < COLS; q++) m = max(m, lb_abs_bits(v[u][q]));
+            const LbScale sc = lb_scale<FMT>(group_max<LANES>(m));
+            const int col = ch[u] * COLS;
+            if (slot[u] < 0 || col >= c.width) continue;
+            unsigned* out = reinterpret_cast<unsigned*>(c.codes + (size_t)slot[u] * c.pitch + col);
+            const unsigned w0 = lb_encode4<FMT>(v[u][0] * sc.inv, v[u][1] * sc.inv, v[u][2] * sc.inv, v[u][3] * sc.inv);
+            if constexpr (COLS == 8)
+                *reinterpret_cast<uint2*>(out) = make_uint2(w0, lb_encode4<FMT>(v[u][4] * sc.inv, v[u][5] * sc.inv, v[u][6] * sc.inv, v[u][7] * sc.inv));
+            else
+                *out = w0;
+            if ((ch[u] & (LANES - 1)) == 0) c.scales[(size_t)slot[u] * ng + ch[u] / LANES] = sc.s;
         }
     }
 }
@@ -56,39 +127,59 @@ __global__ __launch_bounds__(256) void rows8_owner_kernel(gs4d_rows8 c, const S*
     if (slot >= 0 && slot < c.capacity) atomicMax(c.owner + slot, (int)(i + 1));
 }
 
-template <typename S>
-__global__ __launch_bounds__(256) void rows8_owner_clear_kernel(gs4d_rows8 c, const S* __restrict__ slots, long long n)
-{
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const long long slot = slots[i];
-    if (slot >= 0 && slot < c.capacity) c.owner[slot] = 0;
-}
-
-template <int FMT, typename T, typename S>
+// VEC: the output's rows are 16-byte aligned and width a multiple of COLS; else one number per item, so that neighbouring lanes
+// still write neighbouring addresses
+template <int FMT, typename T, typename S, bool VEC>
 __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __restrict__ out, long long ld, long long n,
-                                                         const S* __restrict__ slots, long long start, int cpr, int rpb)
+                                                         const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int gshift)
 {
-    const int r = cpr >= 256 ? 0 : (int)threadIdx.x / cpr, ch0 = cpr >= 256 ? (int)threadIdx.x : (int)threadIdx.x % cpr;
-    const long long i = (long long)blockIdx.x * rpb + r;
-    if (r >= rpb || i >= n) return;
-    const long long slot = slots ? (long long)slots[i] : start + i;
-    const bool inside = slot >= 0 && slot < c.capacity;
-    const int ng = (c.width + c.group - 1) / c.group;
-    for (int ch = ch0; ch < cpr; ch += 256) {
-        const int col = ch * 8;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        float s = 0.f;
-        if (inside) {
-            const uint2 w = *reinterpret_cast<const uint2*>(c.codes + (size_t)slot * c.pitch + col);
-            s = c.scales[(size_t)slot * ng + col / c.group];
-            a = lb_decode4<FMT>(w.x);
-            b = lb_decode4<FMT>(w.y);
-        }
-        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    constexpr int COLS = VEC ? 16 / (int)sizeof(T) : 1;
+    __shared__ long long s_slot[ROWS8_ROWS];
+    const long long i0 = (long long)blockIdx.x * rpb;
+    const int nrow = (int)min((long long)rpb, n - i0);
+    if ((int)threadIdx.x < nrow) {
+        const long long slot = slots ? (long long)slots[i0 + threadIdx.x] : start + i0 + threadIdx.x;
+        s_slot[threadIdx.x] = slot >= 0 && slot < c.capacity ? slot : -1;
+    }
+    __syncthreads();
+    const int items = nrow * cpr, ng = (c.width + c.group - 1) / c.group;
+    constexpr int U = VEC ? 4 : 8;
+    for (int e0 = threadIdx.x; e0 < items; e0 += 256 * U) {
+        unsigned w[U][2];
+        float s[U];
+        int row[U], col[U];
 #pragma unroll
-        for (int q = 0; q < 8; q++)
-            if (col + q < c.width) out[i * ld + col + q] = lb_store<T>(s * v[q]);
+        for (int u = 0; u < U; u++) {
+            const int e = min(e0 + 256 * u, items - 1);
+            row[u] = cpr == 1 ? e : (int)__umulhi((unsigned)e, rcp);
+            col[u] = (e - row[u] * cpr) * COLS;
+            const long long slot = s_slot[row[u]];
+            const size_t at = slot < 0 ? 0 : (size_t)slot;
+            const unsigned char* p = c.codes + at * c.pitch + col[u];
+            if constexpr (COLS == 8) { const uint2 t = *reinterpret_cast<const uint2*>(p); w[u][0] = t.x; w[u][1] = t.y; }
+            else if constexpr (COLS == 4) w[u][0] = *reinterpret_cast<const unsigned*>(p);
+            else w[u][0] = *p;
+            s[u] = c.scales[at * ng + (col[u] >> gshift)];
+            if (slot < 0) { w[u][0] = 0; w[u][1] = 0; s[u] = 0.f; }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (e0 + 256 * u >= items) break;
+            T* y = out + (i0 + row[u]) * ld + col[u];
+            const float4 a = lb_decode4<FMT>(w[u][0]);
+            if constexpr (COLS == 8) {
+                const float4 b = lb_decode4<FMT>(w[u][1]);
+                T o[8] = {lb_store<T>(s[u] * a.x), lb_store<T>(s[u] * a.y), lb_store<T>(s[u] * a.z), lb_store<T>(s[u] * a.w),
+                          lb_store<T>(s[u] * b.x), lb_store<T>(s[u] * b.y), lb_store<T>(s[u] * b.z), lb_store<T>(s[u] * b.w)};
+                uint4 q;
+                __builtin_memcpy(&q, o, 16);
+                *reinterpret_cast<uint4*>(y) = q;
+            } else if constexpr (COLS == 4) {
+                *reinterpret_cast<float4*>(y) = make_float4(s[u] * a.x, s[u] * a.y, s[u] * a.z, s[u] * a.w);
+            } else {
+                *y = lb_store<T>(s[u] * a.x);
+            }
+        }
     }
 }
 
@@ -183,17 +274,6 @@ __device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b)
 {
     return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
-template <typename T> __device__ __forceinline__ float low16(unsigned w)
-{
-    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)w);
-    else return __uint_as_float(w << 16);
-}
-template <typename T> __device__ __forceinline__ float high16(unsigned w)
-{
-    if constexpr (__is_same(T, LbF16)) return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
-    else return __uint_as_float(w & 0xffff0000u);
-}
-
 // A lane's share of a row's group of 64 columns: 4 steps of 8 elements, at columns 16 t + 8 h.
 template <typename T> struct Group { uint4 w[4]; };
 template <> struct Group<float> { uint4 w[8]; };
@@ -716,10 +796,10 @@ static DwArgs dw_plan(long long N, int K, int M)
 
 static int check_cache(const gs4d_rows8* c, const char* who)
 {
-    if (!c || !c->codes || !c->scales || c->capacity < 1 || c->width < 1 || c->pitch < c->width || (c->pitch & 15) ||
+    if (!c || !c->codes || !c->scales || c->capacity < 1 || c->width < 1 || c->width > 65536 || c->pitch < c->width || (c->pitch & 15) ||
         ((uintptr_t)c->codes & 15) || ((uintptr_t)c->scales & 3) ||
         (c->group != 32 && c->group != 64 && c->group != 128) || c->fmt < GS4D_FMT_INT8 || c->fmt > GS4D_FMT_E5M2) {
-        gs4d_set_error("%s: bad cache (pitch and codes must be multiples of 16 bytes, group 32, 64 or 128)", who);
+        gs4d_set_error("%s: bad cache (1 to 65536 columns, pitch and codes multiples of 16 bytes, group 32, 64 or 128)", who);
         return GS4D_EINVAL;
     }
     return GS4D_OK;
@@ -737,6 +817,19 @@ static int check_rows(const gs4d_rows8* c, const void* rows, int dtype, long lon
     return GS4D_OK;
 }
 
+// items per row -> rows per workgroup, workgroups and the multiplier of the division by cpr
+struct RowItems { int cpr, rpb; unsigned rcp, grid; };
+static RowItems row_items(int cpr, long long n)
+{
+    RowItems r;
+    r.cpr = cpr;
+    r.rpb = cpr >= ROWS8_ITEMS ? 1 : ROWS8_ITEMS / cpr < ROWS8_ROWS ? ROWS8_ITEMS / cpr : ROWS8_ROWS;
+    while (r.rpb > 1 && (n + r.rpb - 1) / r.rpb < 512) r.rpb = (r.rpb + 1) / 2;      // few rows: two workgroups per CU before long ones
+    r.rcp = cpr > 1 ? (unsigned)((0x100000000ull + cpr - 1) / cpr) : 0;
+    r.grid = (unsigned)((n + r.rpb - 1) / r.rpb);
+    return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -750,22 +843,27 @@ int gs4d_rows8_write(const gs4d_rows8* c, const void* rows, int dtype, long long
     if (n == 0) return GS4D_OK;
     const int dup = !slots || n == 1 ? 0 : n <= GS4D_ROWS8_SCAN ? 1 : 2;
     if (dup == 2 && !c->owner) { gs4d_set_error("gs4d_rows8_write: %lld rows at given slots need the cache's owner array", n); return GS4D_EINVAL; }
-    const int cpr = lb_groups(c->width, c->group) * (c->group / 8), rpb = cpr >= 256 ? 1 : 256 / cpr;
-    const unsigned grid = (unsigned)((n + rpb - 1) / rpb), ogrid = (unsigned)((n + 255) / 256);
+    const unsigned ogrid = (unsigned)((n + 255) / 256);
     auto with_slots = [&](auto tag) {
         using S = decltype(tag);
         const S* sl = (const S*)slots;
         if (dup == 2) hipLaunchKernelGGL(rows8_owner_kernel<S>, dim3(ogrid), dim3(256), 0, s, *c, sl, n);
         by_type(dtype, [&](auto t) {
             using T = decltype(t);
+            constexpr int COLS = 16 / (int)sizeof(T);
+            const RowItems it = row_items(lb_groups(c->width, c->group) * (c->group / COLS), n);
+            const bool vec = c->width % COLS == 0 && ((uintptr_t)rows & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
             return by_fmt(c->fmt, [&](auto f) {
                 constexpr int F = decltype(f)::value;
-                auto k = c->group == 32 ? rows8_write_kernel<F, 4, T, S> : c->group == 64 ? rows8_write_kernel<F, 8, T, S> : rows8_write_kernel<F, 16, T, S>;
-                hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, s, *c, (const T*)rows, ld, n, sl, start, cpr, rpb, dup);
+                auto go = [&](auto v) {
+                    constexpr bool V = decltype(v)::value != 0;
+                    auto k = c->group == 32 ? rows8_write_kernel<F, 32 / COLS, T, S, V> : c->group == 64 ? rows8_write_kernel<F, 64 / COLS, T, S, V> : rows8_write_kernel<F, 128 / COLS, T, S, V>;
+                    hipLaunchKernelGGL(k, dim3(it.grid), dim3(256), 0, s, *c, (const T*)rows, ld, n, sl, start, it.cpr, it.rpb, it.rcp, dup);
+                };
+                if (vec) go(Int<1>()); else go(Int<0>());
                 return 0;
             });
         });
-        if (dup == 2) hipLaunchKernelGGL(rows8_owner_clear_kernel<S>, dim3(ogrid), dim3(256), 0, s, *c, sl, n);
     };
     if (slots && slot_bytes == 4) with_slots(int());
     else with_slots((long long)0);
@@ -780,16 +878,21 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
     hipStream_t s = (hipStream_t)stream;
     if (check_rows(c, out, dtype, ld, n, slots, slot_bytes, start, "gs4d_rows8_read")) return GS4D_EINVAL;
     if (n == 0) return GS4D_OK;
-    const int cpr = (c->width + 7) / 8, rpb = cpr >= 256 ? 1 : 256 / cpr;
-    const unsigned grid = (unsigned)((n + rpb - 1) / rpb);
+    const int gshift = c->group == 32 ? 5 : c->group == 64 ? 6 : 7;
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
+        constexpr int COLS = 16 / (int)sizeof(T);
+        const bool vec = c->width % COLS == 0 && ((uintptr_t)out & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+        const RowItems it = row_items(vec ? c->width / COLS : c->width, n);
         return by_fmt(c->fmt, [&](auto f) {
             constexpr int F = decltype(f)::value;
-            if (slots && slot_bytes == 4)
-                hipLaunchKernelGGL((rows8_read_kernel<F, T, int>), dim3(grid), dim3(256), 0, s, *c, (T*)out, ld, n, (const int*)slots, start, cpr, rpb);
-            else
-                hipLaunchKernelGGL((rows8_read_kernel<F, T, long long>), dim3(grid), dim3(256), 0, s, *c, (T*)out, ld, n, (const long long*)slots, start, cpr, rpb);
+            auto go = [&](auto tag, auto v) {
+                using S = decltype(tag);
+                hipLaunchKernelGGL((rows8_read_kernel<F, T, S, decltype(v)::value != 0>), dim3(it.grid), dim3(256), 0, s, *c, (T*)out, ld, n, (const S*)slots, start, it.cpr, it.rpb, it.rcp, gshift);
+            };
+            const bool narrow = slots && slot_bytes == 4;
+            if (vec) { if (narrow) go(int(), Int<1>()); else go((long long)0, Int<1>()); }
+            else { if (narrow) go(int(), Int<0>()); else go((long long)0, Int<0>()); }
             return 0;
         });
     });

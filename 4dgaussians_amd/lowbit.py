@@ -67,8 +67,8 @@ class RowCache:
     Calls run on the current stream of the cache's device; calls on one cache from several streams are ordered by the caller."""
 
     def __init__(self, capacity, width, fmt="int8", group=64, device="cuda"):
-        if int(capacity) < 1 or int(width) < 1:
-            raise RuntimeError(f"RowCache: capacity and width must be at least 1, got {capacity} and {width}")
+        if int(capacity) < 1 or not 1 <= int(width) <= 65536:
+            raise RuntimeError(f"RowCache: at least one row of 1 to 65536 columns, got {capacity} and {width}")
         if group not in GROUPS:
             raise RuntimeError(f"RowCache: group must be 32, 64 or 128, got {group}")
         _format(fmt)
@@ -89,7 +89,7 @@ class RowCache:
         f = _format(fmt)
         _on_device("codes", codes)
         _on_device("scales", scales, codes.device)
-        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous() or codes.shape[0] < 1 or width < 1 \
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous() or codes.shape[0] < 1 or not 1 <= width <= 65536 \
                 or codes.shape[1] < width or codes.shape[1] % 16 or codes.data_ptr() % 16:
             raise RuntimeError("RowCache: codes must be a contiguous uint8 tensor [capacity, pitch], 16-byte aligned, pitch a "
                                "multiple of 16 and at least width")

@@ -632,7 +632,7 @@ typedef struct gs4d_rows8 {
     float* scales;
     int* owner;
     long long capacity;
-    int width, pitch, group, fmt;      /* group: 32, 64 or 128 columns */
+    int width, pitch, group, fmt;      /* width: at most 65536; group: 32, 64 or 128 columns */
 } gs4d_rows8;
 
 /* rows [n] of `dtype` with a pitch of ld elements -> the cache.  slots: device [n] ints of slot_bytes (4 or 8) bytes each, or

@@ -213,6 +213,29 @@ def test_frame_features(levels, ch, res, res_t, n, fmt):
         assert torch.equal(got, again)                                # planes of another memory format
 
 
+@pytest.mark.parametrize("levels,ch,res,res_t,n", [(2, 32, 20, 7, 4099), (2, 128, 64, 5, 1031), (1, 256, 9, 3, 700), (3, 4, 5, 4, 20_000),
+                                                   (4, 16, 30, 9, 5000), (1, 64, 900, 3, 2000), (1, 8, 4000, 2, 9000), (1, 4, 1, 1, 17_000)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_frame_features_of_many_points(levels, ch, res, res_t, n, fmt):
+    """One t for enough points that the planes are blended to lines first; long axes among them."""
+    g = torch.Generator().manual_seed(n)
+    static = 0.1 + torch.rand(n, levels * ch, generator=g) * 2
+    c = lb().RowCache(n, levels * ch, fmt, 128)
+    c.write(static.cuda())
+    held = R.quantise(np64(static), fmt, 128)[0]
+    planes = [(0.5 + torch.rand(1, res_t, res << (lv % 2), ch, generator=g)).permute(0, 3, 1, 2) for lv in range(levels) for _ in range(3)]
+    aabb = torch.tensor([[1.3, 1.2, 1.1], [-1.3, -1.2, -1.0]])
+    pts = (torch.rand(n, 3, generator=g) * 2 - 1) * 1.6
+    args = [p.cuda() for p in planes], aabb.cuda(), pts.cuda()
+    for t in (torch.tensor([0.3721]), torch.tensor([1.0]), torch.tensor([-2.0])):
+        got = lb().frame_features(c, *args, t.cuda())
+        want = R.frame_features(held, [p[0].numpy() for p in planes], aabb.numpy(), pts.numpy(), t.expand(n).numpy())
+        tol = (12 * 8 * 4 * max(2 * res, res_t) + 20) * 2.0 ** -24    # as above
+        assert np.abs(np64(got) / want - 1).max() <= tol
+        each = lb().frame_features(c, *args, t.expand(n).contiguous().cuda())
+        assert np.abs(np64(each) / want - 1).max() <= tol             # a value per point: the other kernel
+
+
 def test_frame_features_refuses():
     c = lb().RowCache(10, 16)
     z = lambda *s: torch.zeros(*s, device="cuda")
