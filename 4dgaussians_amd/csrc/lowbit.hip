@@ -184,8 +184,9 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
 }
 
 // ------------------------------------------------------------------ linear
-// What the backward keeps of the input, in one block: codes [N][kp] | scales [N][kp / 64] | sign bits [N][kp / 8] (bit k & 7 of
-// byte k >> 3: x > 0), kp = K rounded up to 64.
+// What the backward keeps of the input, in one block: codes [N][kp] | scales [N][kp / 64] | sign bits [N][kp / 64][2 words]
+// (x > 0), kp = K rounded up to 64.  Column c of a group is bit c & 31 of word c >> 5 for float32 and bit c >> 1 of word c & 1
+// for the 16-bit types: a word is the lane mask of one tile of linear8_rows_kernel's result.
 struct Keep { unsigned char* codes; float* scales; unsigned char* bits; int kp; };
 
 static Keep carve_keep(char* base, long long N, int K, int what, size_t* bytes)
@@ -239,27 +240,31 @@ template <typename T> __device__ __forceinline__ f32x16 mfma(const uint4& a, con
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ float top8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// two numbers -> their TERMS bfloat16 parts, packed.  SAFE: also for infinities (whose remainder would be a NaN)
-template <int TERMS, bool SAFE>
+// two numbers -> their TERMS bfloat16 parts, packed.  The remainder of an infinity is a NaN, which the clamp (no remainder of a
+// finite number is larger) turns into a number: the infinity stays one.
+template <int TERMS>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
     for (int t = 0; t < TERMS; t++) {
         o[t] = hi16(__float_as_uint(a), __float_as_uint(b));
         if (t + 1 < TERMS) {
-            const float ra = a - top8(a), rb = b - top8(b);
-            a = SAFE && lb_abs_bits(a) == 0x7f800000u ? 0.f : ra;
-            b = SAFE && lb_abs_bits(b) == 0x7f800000u ? 0.f : rb;
+            a -= top8(a);
+            b -= top8(b);
+            if (t == 0) {
+                a = __builtin_amdgcn_fmed3f(a, -0x1p120f, 0x1p120f);
+                b = __builtin_amdgcn_fmed3f(b, -0x1p120f, 0x1p120f);
+            }
         }
     }
 }
 
-template <int TERMS, bool SAFE>
+template <int TERMS>
 __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 {
     unsigned w[4][TERMS];
 #pragma unroll
-    for (int q = 0; q < 4; q++) split2<TERMS, SAFE>(v[2 * q], v[2 * q + 1], w[q]);
+    for (int q = 0; q < 4; q++) split2<TERMS>(v[2 * q], v[2 * q + 1], w[q]);
 #pragma unroll
     for (int t = 0; t < TERMS; t++) o[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
 }
@@ -340,6 +345,8 @@ __device__ __forceinline__ void positive_nans(Group<T>& g)
     }
 }
 
+template <typename T, int NT, bool VEC> constexpr int kRowsThreads = VEC && NT <= 2 ? 1024 : 512;
+
 struct RowsArgs {
     long long N; int C, F;                // rows, contraction length, features of the result
     const void* x; long long ldx;
@@ -351,17 +358,18 @@ struct RowsArgs {
     int ncb, nwg, groups, chunk;          // column blocks, workgroups per column block, groups of 64 of the contraction, groups in LDS at once
 };
 
-// Both products over the rows, y^T[feature][row] = W x^T (+ bias) and dx^T = W^T dy^T: a wave owns 32 rows, which are the columns
-// of v_mfma_f32_32x32x16, and NT tiles of 32 features; a lane streams its row from memory in groups of 64 columns (the next group
-// is in flight while this one is multiplied) and ends up with quads of neighbouring features of that row.  The weight lies in LDS
-// as MFMA operands, split once per workgroup, for as many groups as fit; a workgroup of 8 waves walks the rows in steps of
-// 8 * nwg tiles.  What the backward needs of x is quantised on the way, from the registers that feed the product: x is read once.
+// Both products over the rows, y = x W^T (+ bias) and dx = dy W: a wave owns 32 rows and NT tiles of 32 features of
+// v_mfma_f32_32x32x16; a lane streams its row from memory in groups of 64 columns and ends up with one feature of 16 rows, so
+// that a row's results leave as whole lines.  (With features and rows exchanged a lane holds quads of one row, whose stores
+// touch 32 lines each: the address units were busy 80 % of the time and the 1.2 M x 256 -> 64 product took 576 us.)  Tile nt
+// holds the features 32 nt + lane, for 16-bit types the features 2 lane + (nt & 1) of 64, which leave as one word.
+// The weight lies in LDS as MFMA operands, split once per workgroup, for as many groups as fit; the waves of a workgroup walk the
+// rows.  What the backward needs of x is quantised on the way, from the registers that feed the product: x is read once.
 template <typename T, int NT, bool VEC, bool DX>
-__global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
+__global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kernel(RowsArgs a)
 {
-    constexpr int TERMS = kTerms<T>;
+    constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC>, WAVES = THREADS / 64;
     extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane]
-    __shared__ float s_bias[NT * 32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
     // workgroups that share rows differ by 8 in their number, i.e. run on one XCD behind one L2
     int cb, wg;
@@ -376,11 +384,11 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
     const int f0 = cb * NT * 32, C = a.C, F = a.F;
     const T* __restrict__ X = (const T*)a.x;
     const T* __restrict__ W = (const T*)a.w;
-    if (tid < NT * 32) s_bias[tid] = !DX && a.bias && f0 + tid < F ? lb_load(((const T*)a.bias)[f0 + tid]) : 0.f;
+    auto feature = [&](int nt, int l) { return f0 + (sizeof(T) == 4 ? nt * 32 + l : (nt >> 1) * 64 + 2 * l + (nt & 1)); };
     auto stage = [&](int g0, int n) {                     // groups g0 .. g0 + n - 1 of the weight
-        for (int e = tid; e < n * 4 * NT * 64; e += 512) {
+        for (int e = tid; e < n * 4 * NT * 64; e += THREADS) {
             const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
-            const int f = f0 + nt * 32 + (l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
+            const int f = feature(nt, l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
             const T* p = W + (long long)min(f, F - 1) * a.wf;
             if constexpr (sizeof(T) == 4) {
                 float v[8];
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
                     v[q] = f < F && c + q < C ? u : 0.f;
                 }
                 uint4 o[TERMS];
-                split8<TERMS, true>(v, o);
+                split8<TERMS>(v, o);
 #pragma unroll
                 for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
             } else {
@@ -405,32 +413,45 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
             }
         }
     };
-    if (a.chunk >= a.groups) stage(0, a.groups);
-    __syncthreads();
-
     const int ntile = (int)((a.N + 31) >> 5);
     const bool keeping = !DX && cb == 0 && (a.keep.codes || a.keep.bits);
     auto row_of = [&](long long tile) { const long long r = tile * 32 + j; return X + (r < a.N ? r : a.N - 1) * a.ldx; };
-    Group<T> cur, nxt;
+    float bias[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) bias[nt] = !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt, j), F - 1)]) : 0.f;
     long long tile = (long long)wave * a.nwg + wg;
-    load_group<T, VEC>(cur, row_of(tile), 8 * h, C);
-    for (long long base = 0; base * a.nwg < ntile; base += 8, tile += 8ll * a.nwg) {      // uniform: every wave takes part in the barriers
+    Group<T> cur;
+    // the waves start at different groups: a row of several 256-byte groups, read by all waves in step, would keep to a fraction of
+    // the memory channels at a time
+    const int turn = a.chunk >= a.groups ? wave % a.groups : 0;
+    auto group_at = [&](int gi) { const int g = gi + turn; return g < a.groups ? g : g - a.groups; };
+    load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C);      // in flight while the weight is staged
+    if (a.chunk >= a.groups) stage(0, a.groups);
+    __syncthreads();
+    for (long long base = 0; base * a.nwg < ntile; base += WAVES, tile += (long long)WAVES * a.nwg) {      // uniform: every wave takes part in the barriers
         const long long row = tile * 32 + j;
         const bool live = row < a.N;
         f32x16 acc[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[nt][r] = s_bias[nt * 32 + (r & 3) + 8 * (r >> 2) + 4 * h];
-        for (int g = 0; g < a.groups; g++) {
-            if (a.chunk < a.groups && g % a.chunk == 0) {
+            for (int r = 0; r < 16; r++) acc[nt][r] = bias[nt];
+        // dx: the sign bits of the lane's row for the tiles' features
+        unsigned sign[NT];
+        if (DX && a.keep.bits) {
+            const unsigned* p = reinterpret_cast<const unsigned*>(a.keep.bits) + (live ? row : a.N - 1) * (a.keep.kp / 32) + (f0 >> 5);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) sign[nt] = p[min(nt, a.keep.kp / 32 - 1 - (f0 >> 5))];
+        }
+        for (int gi = 0; gi < a.groups; gi++) {
+            const int g = group_at(gi);
+            if (a.chunk < a.groups && gi % a.chunk == 0) {
                 __syncthreads();
-                stage(g, min(a.chunk, a.groups - g));
+                stage(gi, min(a.chunk, a.groups - gi));
                 __syncthreads();
             }
-            load_group<T, VEC>(nxt, g + 1 < a.groups ? row_of(tile) : row_of(tile + 8ll * a.nwg), g + 1 < a.groups ? (g + 1) * 64 + 8 * h : 8 * h, C);
             if (g * 64 + 64 > C) clear_past(cur, g * 64 + 8 * h, C);
-            const uint4* __restrict__ wl = s_w + (size_t)(g % a.chunk) * 4 * NT * TERMS * 64 + lane;
+            const uint4* __restrict__ wl = s_w + (size_t)(a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
             float v[4][8];
@@ -444,8 +465,7 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
                 for (int t = 0; t < 4; t++) o2 = max_u16x2(max_u16x2(o2, max_u16x2(cur.w[t].x & 0x7fff7fffu, cur.w[t].y & 0x7fff7fffu)), max_u16x2(cur.w[t].z & 0x7fff7fffu, cur.w[t].w & 0x7fff7fffu));
                 odd = max(o2 & 0xffffu, o2 >> 16) >= (__is_same(T, LbF16) ? 0x7c00u : 0x7f80u);
             }
-            const bool rare = __builtin_amdgcn_ballot_w64(odd) != 0;
-            if (rare && !DX) positive_nans(cur);
+            if (!DX && __builtin_amdgcn_ballot_w64(odd)) positive_nans(cur);
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -472,7 +492,6 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
                 m = __float_as_uint(low16<T>(max(m2 & 0xffffu, m2 >> 16)));
             }
             if (keeping) {
-                unsigned bits = 0;
                 if constexpr (sizeof(T) == 2) {
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
@@ -482,30 +501,39 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
                     }
                 }
                 if (a.keep.bits) {                        // relu: every number is at least 0 here
+                    unsigned w[2] = {0, 0};
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
-                        for (int q = 0; q < 8; q++) bits |= min(__float_as_uint(v[t][q]), 1u) << (8 * t + q);
-                    // byte 2 t + h of the group's 8 holds step t: the halves' bytes alternate
-                    const unsigned other = (unsigned)__shfl_xor((int)bits, 32, 64);
-                    const unsigned ev = h ? other : bits, od = h ? bits : other;
-                    uint2 w;
-                    w.x = (ev & 255u) | (od & 255u) << 8 | (ev >> 8 & 255u) << 16 | (od >> 8 & 255u) << 24;
-                    w.y = (ev >> 16 & 255u) | (od >> 16 & 255u) << 8 | (ev >> 24) << 16 | (od >> 24) << 24;
-                    if (live && h == 0) *reinterpret_cast<uint2*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + g * 8) = w;
+                        for (int q = 0; q < 8; q++) {
+                            const unsigned positive = min(__float_as_uint(v[t][q]), 1u);
+                            if (sizeof(T) == 4) w[t >> 1] |= positive << (16 * (t & 1) + q);
+                            else w[q & 1] |= positive << (8 * t + (q >> 1));
+                        }
+                    const int at = sizeof(T) == 4 ? 8 * h : 4 * h;
+                    w[0] <<= at;
+                    w[1] <<= at;
+                    w[0] |= (unsigned)__shfl_xor((int)w[0], 32, 64);
+                    w[1] |= (unsigned)__shfl_xor((int)w[1], 32, 64);
+                    if (live && h == 0) *reinterpret_cast<uint2*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + g * 8) = make_uint2(w[0], w[1]);
                 }
                 if (a.keep.codes) {
                     m = max(m, (unsigned)__shfl_xor((int)m, 32, 64));
-                    unsigned char* code = a.keep.codes + (size_t)row * a.keep.kp + g * 64 + 8 * h;
+                    unsigned char* code = a.keep.codes + (size_t)row * a.keep.kp + g * 64 + 16 * h;
                     auto encode = [&](auto f) {
                         constexpr int FMT = decltype(f)::value;
                         const LbScale sc = lb_scale<FMT>(m);
 #pragma unroll
-                        for (int t = 0; t < 4; t++) {
-                            uint2 w;
-                            w.x = lb_encode4<FMT>(v[t][0] * sc.inv, v[t][1] * sc.inv, v[t][2] * sc.inv, v[t][3] * sc.inv);
-                            w.y = lb_encode4<FMT>(v[t][4] * sc.inv, v[t][5] * sc.inv, v[t][6] * sc.inv, v[t][7] * sc.inv);
-                            if (live) *reinterpret_cast<uint2*>(code + 16 * t) = w;
+                        for (int t = 0; t < 4; t += 2) {
+                            unsigned w[4];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const float* p = &v[t + (q >> 1)][4 * (q & 1)];
+                                w[q] = lb_encode4<FMT>(p[0] * sc.inv, p[1] * sc.inv, p[2] * sc.inv, p[3] * sc.inv);
+                            }
+                            // the halves swap, so that a lane has 16 codes in a row: step t for h = 0, step t + 1 for h = 1
+                            const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                            if (live) *reinterpret_cast<uint4*>(code + 16 * t) = make_uint4(x[0], y[0], x[1], y[1]);
                         }
                         if (live && h == 0) a.keep.scales[(size_t)row * (a.keep.kp / 64) + g] = sc.s;
                     };
@@ -515,54 +543,58 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(RowsArgs a)
                     else encode(Int<GS4D_FMT_E5M2>());
                 }
             }
-            auto multiply = [&](auto safe) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    uint4 xs[TERMS];
-                    if constexpr (sizeof(T) == 4) split8<TERMS, decltype(safe)::value != 0>(v[t], xs);
-                    else xs[0] = cur.w[t];
+            for (int t = 0; t < 4; t++) {
+                __builtin_amdgcn_sched_barrier(0);        // a step at a time: hoisted splits and weights would spill
+                uint4 xs[TERMS];
+                if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs);
+                else xs[0] = cur.w[t];
+                uint4 ws[NT][TERMS];
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        uint4 ws[TERMS];
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int u = 0; u < TERMS; u++) ws[u] = wl[((t * NT + nt) * TERMS + u) * 64];
+                    for (int u = 0; u < TERMS; u++) ws[nt][u] = wl[((t * NT + nt) * TERMS + u) * 64];
 #pragma unroll
-                        for (int u = TERMS - 1; u >= 0; u--)                  // the smallest products first
+                for (int u = TERMS - 1; u >= 0; u--)      // the smallest products first
 #pragma unroll
-                            for (int z = 0; z <= u; z++) acc[nt] = mfma<T>(ws[z], xs[u - z], acc[nt]);
-                    }
-                }
-            };
-            if (sizeof(T) == 4 && rare) multiply(Int<1>());
-            else multiply(Int<0>());
-            cur = nxt;
+                    for (int z = 0; z <= u; z++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool more = gi + 1 < a.groups;
+            load_group<T, VEC>(cur, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, C);
         }
-        // ---- a quad of features per (tile, register quad)
-        if (live) {
-            T* __restrict__ y = (T*)a.y + row * F + f0;
-            const bool quads = (F & 3) == 0 && ((uintptr_t)a.y & (4 * sizeof(T) - 1)) == 0;
+        // ---- register r is the row (r & 3) + 8 (r >> 2) + 4 h of the tile
+        const bool whole = tile * 32 + 32 <= a.N;
+        T* __restrict__ y = (T*)a.y + (tile * 32 + 4 * h) * F;
+        const bool pairs = sizeof(T) == 2 && (F & 1) == 0 && ((uintptr_t)a.y & 3) == 0;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int rr = (r & 3) + 8 * (r >> 2);
+            if (!whole && tile * 32 + rr + 4 * h >= a.N) continue;
+            float o[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                unsigned mask = 0xffffffffu;
-                if (DX && a.keep.bits && f0 + nt * 32 < F)
-                    mask = *reinterpret_cast<const unsigned*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + (f0 >> 3) + 4 * nt);
-#pragma unroll
-                for (int mq = 0; mq < 4; mq++) {
-                    const int f = nt * 32 + 8 * mq + 4 * h;
-                    T o[4];
-#pragma unroll
-                    for (int q = 0; q < 4; q++) o[q] = lb_store<T>(!DX || (mask >> (8 * mq + 4 * h + q) & 1u) ? acc[nt][4 * mq + q] : 0.f);
-                    if (quads) {
-                        if (f0 + f < F) {
-                            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y + f) = make_float4(o[0], o[1], o[2], o[3]);
-                            else *reinterpret_cast<uint2*>(y + f) = *reinterpret_cast<const uint2*>(o);
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            if (f0 + f + q < F) y[f + q] = o[q];
-                    }
+                o[nt] = acc[nt][r];
+                if (DX && a.keep.bits) {
+                    const unsigned long long lanes = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(sign[nt], rr + 4) << 32 | (unsigned)__builtin_amdgcn_readlane(sign[nt], rr);
+                    o[nt] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? o[nt] : 0.f;
                 }
+            }
+            T* __restrict__ yr = y + (long long)rr * F;
+            if (pairs) {
+#pragma unroll
+                for (int nt = 0; nt + 1 < NT; nt += 2) {
+                    const T two[2] = {lb_store<T>(o[nt]), lb_store<T>(o[nt + 1])};
+                    unsigned w;
+                    __builtin_memcpy(&w, two, 4);
+                    if (feature(nt, j) < F) *reinterpret_cast<unsigned*>(yr + feature(nt, j)) = w;
+                }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    if (feature(nt, j) < F) yr[feature(nt, j)] = lb_store<T>(o[nt]);
             }
         }
     }
@@ -640,10 +672,10 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
                 else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
             }
             uint4 da[2][TERMS], cc[2][1];
-            split8<TERMS, false>(d0, da[0]);
-            split8<TERMS, false>(d1, da[1]);
-            split8<1, false>(c0, cc[0]);
-            split8<1, false>(c1, cc[1]);
+            split8<TERMS>(d0, da[0]);
+            split8<TERMS>(d1, da[1]);
+            split8<1>(c0, cc[0]);
+            split8<1>(c1, cc[1]);
 #pragma unroll
             for (int u = TERMS - 1; u >= 0; u--)
 #pragma unroll
@@ -935,27 +967,30 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
 {
     constexpr int LDS = 144 * 1024;
     const bool vec = a.C % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.ldx * sizeof(T)) % 16 == 0;
-    const int most = sizeof(T) == 4 ? 2 : 4, nt = a.F <= 32 ? 1 : a.F <= 64 || most == 2 ? 2 : 4;
+    const int nt = sizeof(T) == 4 ? (a.F <= 32 ? 1 : 2) : a.F <= 64 ? 2 : 4;
     a.groups = (a.C + 63) / 64;
     const int per = 4 * nt * kTerms<T> * 1024;
     a.chunk = LDS / per < a.groups ? LDS / per : a.groups;
     const size_t lds = (size_t)a.chunk * per;
     a.ncb = (a.F + nt * 32 - 1) / (nt * 32);
     const long long ntile = (a.N + 31) / 32;
-    long long nwg = LB_CUS * (lds <= 72 * 1024 ? 2 : 1) / a.ncb;
-    if (nwg > ntile) nwg = ntile;
-    if (nwg < 1) nwg = 1;
-    if (nwg >= 8) nwg = nwg / 8 * 8;
-    a.nwg = (int)nwg;
     auto launch = [&](auto n, auto v) {
+        constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0>;
         auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX>;
+        // 16 waves per CU if registers and LDS allow, never more workgroups than row tiles
+        long long nwg = LB_CUS * (THREADS == 512 && lds <= 78 * 1024 ? 2 : 1) / a.ncb;
+        if (nwg > ntile) nwg = ntile;
+        if (nwg < 1) nwg = 1;
+        if (nwg >= 8) nwg = nwg / 8 * 8;
+        a.nwg = (int)nwg;
         if (lds > 64 * 1024) GS4D_HIP_CHECK(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        hipLaunchKernelGGL(k, dim3((unsigned)(a.nwg * a.ncb)), dim3(512), lds, s, a);
+        hipLaunchKernelGGL(k, dim3((unsigned)(a.nwg * a.ncb)), dim3(THREADS), lds, s, a);
         return GS4D_OK;
     };
     auto with_nt = [&](auto n) { return vec ? launch(n, Int<1>()) : launch(n, Int<0>()); };
-    if constexpr (sizeof(T) == 2) { if (nt == 4) return with_nt(Int<4>()); }
-    return nt == 1 ? with_nt(Int<1>()) : with_nt(Int<2>());
+    if (nt == 2) return with_nt(Int<2>());
+    if constexpr (sizeof(T) == 2) return with_nt(Int<4>());
+    else return with_nt(Int<1>());
 }
 
 template <typename T>
