@@ -242,7 +242,7 @@ __device__ __forceinline__ float top8(float x) { return __uint_as_float(__float_
 
 // two numbers -> their TERMS bfloat16 parts, packed.  The remainder of an infinity is a NaN, which the clamp (no remainder of a
 // finite number is larger) turns into a number: the infinity stays one.
-template <int TERMS>
+template <int TERMS, bool CLAMP>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
@@ -251,7 +251,7 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
         if (t + 1 < TERMS) {
             a -= top8(a);
             b -= top8(b);
-            if (t == 0) {
+            if (CLAMP && t == 0) {
                 a = __builtin_amdgcn_fmed3f(a, -0x1p120f, 0x1p120f);
                 b = __builtin_amdgcn_fmed3f(b, -0x1p120f, 0x1p120f);
             }
@@ -259,12 +259,12 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
     }
 }
 
-template <int TERMS>
+template <int TERMS, bool CLAMP = true>
 __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 {
     unsigned w[4][TERMS];
 #pragma unroll
-    for (int q = 0; q < 4; q++) split2<TERMS>(v[2 * q], v[2 * q + 1], w[q]);
+    for (int q = 0; q < 4; q++) split2<TERMS, CLAMP>(v[2 * q], v[2 * q + 1], w[q]);
 #pragma unroll
     for (int t = 0; t < TERMS; t++) o[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
 }
@@ -345,7 +345,8 @@ __device__ __forceinline__ void positive_nans(Group<T>& g)
     }
 }
 
-template <typename T, int NT, bool VEC> constexpr int kRowsThreads = VEC && NT <= 2 ? 1024 : 512;
+// 16 waves where 128 registers do
+template <typename T, int NT, bool VEC, bool ONE> constexpr int kRowsThreads = VEC && NT <= 2 && !ONE ? 1024 : 512;
 
 struct RowsArgs {
     long long N; int C, F;                // rows, contraction length, features of the result
@@ -355,7 +356,8 @@ struct RowsArgs {
     void* y;                              // [N][F]
     int lowest;                           // relu_bits()
     Keep keep; int fmt;                   // forward: what to keep; dx: keep.bits masks the result
-    int ncb, nwg, groups, chunk;          // column blocks, workgroups per column block, groups of 64 of the contraction, groups in LDS at once
+    int ncb, nwg, groups, chunk;          // sets of column blocks, workgroups per set, groups of 64 of the contraction, groups in LDS at once
+    int blocks;                           // column blocks of NT * 32 features per set: 1, or more where the contraction is one group (ONE)
 };
 
 // Both products over the rows, y = x W^T (+ bias) and dx = dy W: a wave owns 32 rows and NT tiles of 32 features of
@@ -365,10 +367,10 @@ struct RowsArgs {
 // holds the features 32 nt + lane, for 16-bit types the features 2 lane + (nt & 1) of 64, which leave as one word.
 // The weight lies in LDS as MFMA operands, split once per workgroup, for as many groups as fit; the waves of a workgroup walk the
 // rows.  What the backward needs of x is quantised on the way, from the registers that feed the product: x is read once.
-template <typename T, int NT, bool VEC, bool DX>
-__global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kernel(RowsArgs a)
+template <typename T, int NT, bool VEC, bool DX, bool ONE>
+__global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_kernel(RowsArgs a)
 {
-    constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC>, WAVES = THREADS / 64;
+    constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC, ONE>, WAVES = THREADS / 64, BLOCK = 4 * NT * TERMS * 64;
     extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
     // workgroups that share rows differ by 8 in their number, i.e. run on one XCD behind one L2
@@ -381,11 +383,12 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kerne
         cb = blockIdx.x % a.ncb;
         wg = blockIdx.x / a.ncb;
     }
-    const int f0 = cb * NT * 32, C = a.C, F = a.F;
+    const int C = a.C, F = a.F;
+    int f0 = cb * a.blocks * NT * 32;
     const T* __restrict__ X = (const T*)a.x;
     const T* __restrict__ W = (const T*)a.w;
     auto feature = [&](int nt, int l) { return f0 + (sizeof(T) == 4 ? nt * 32 + l : (nt >> 1) * 64 + 2 * l + (nt & 1)); };
-    auto stage = [&](int g0, int n) {                     // groups g0 .. g0 + n - 1 of the weight
+    auto stage = [&](int g0, int n, uint4* s_w) {         // groups g0 .. g0 + n - 1 of the weight, for the features from f0 on
         for (int e = tid; e < n * 4 * NT * 64; e += THREADS) {
             const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
             const int f = feature(nt, l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
@@ -416,9 +419,6 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kerne
     const int ntile = (int)((a.N + 31) >> 5);
     const bool keeping = !DX && cb == 0 && (a.keep.codes || a.keep.bits);
     auto row_of = [&](long long tile) { const long long r = tile * 32 + j; return X + (r < a.N ? r : a.N - 1) * a.ldx; };
-    float bias[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) bias[nt] = !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt, j), F - 1)]) : 0.f;
     long long tile = (long long)wave * a.nwg + wg;
     Group<T> cur;
     // the waves start at different groups: a row of several 256-byte groups, read by all waves in step, would keep to a fraction of
@@ -426,31 +426,89 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kerne
     const int turn = a.chunk >= a.groups ? wave % a.groups : 0;
     auto group_at = [&](int gi) { const int g = gi + turn; return g < a.groups ? g : g - a.groups; };
     load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C);      // in flight while the weight is staged
-    if (a.chunk >= a.groups) stage(0, a.groups);
+    if constexpr (ONE) {
+        for (int k = 0; k < a.blocks; k++) { stage(0, 1, s_w + k * BLOCK); f0 += NT * 32; }
+        f0 -= a.blocks * NT * 32;
+    } else if (a.chunk >= a.groups) {
+        stage(0, a.groups, s_w);
+    }
     __syncthreads();
     for (long long base = 0; base * a.nwg < ntile; base += WAVES, tile += (long long)WAVES * a.nwg) {      // uniform: every wave takes part in the barriers
         const long long row = tile * 32 + j;
         const bool live = row < a.N;
         f32x16 acc[NT];
+        unsigned sign[NT];                                // dx: the sign bits of the lane's row for the tiles' features
+        auto begin = [&]() {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
+                const float b = !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt, j), F - 1)]) : 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[nt][r] = bias[nt];
-        // dx: the sign bits of the lane's row for the tiles' features
-        unsigned sign[NT];
-        if (DX && a.keep.bits) {
-            const unsigned* p = reinterpret_cast<const unsigned*>(a.keep.bits) + (live ? row : a.N - 1) * (a.keep.kp / 32) + (f0 >> 5);
+                for (int r = 0; r < 16; r++) acc[nt][r] = b;
+            }
+            if (DX && a.keep.bits) {
+                const unsigned* p = reinterpret_cast<const unsigned*>(a.keep.bits) + (live ? row : a.N - 1) * (a.keep.kp / 32);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) sign[nt] = p[min(nt, a.keep.kp / 32 - 1 - (f0 >> 5))];
-        }
+                for (int nt = 0; nt < NT; nt++) sign[nt] = p[min((f0 >> 5) + nt, a.keep.kp / 32 - 1)];
+            }
+        };
+        auto step = [&](const uint4 (&xs)[TERMS], const uint4* __restrict__ wl) {
+            uint4 ws[NT][TERMS];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int u = 0; u < TERMS; u++) ws[nt][u] = wl[(nt * TERMS + u) * 64];
+#pragma unroll
+            for (int u = TERMS - 1; u >= 0; u--)          // the smallest products first
+#pragma unroll
+                for (int z = 0; z <= u; z++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
+        };
+        // register r is the row (r & 3) + 8 (r >> 2) + 4 h of the tile
+        auto finish = [&]() {
+            const bool whole = tile * 32 + 32 <= a.N;
+            T* __restrict__ y = (T*)a.y + (tile * 32 + 4 * h) * F;
+            const bool pairs = sizeof(T) == 2 && (F & 1) == 0 && ((uintptr_t)a.y & 3) == 0;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int rr = (r & 3) + 8 * (r >> 2);
+                if (!whole && tile * 32 + rr + 4 * h >= a.N) continue;
+                float o[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    o[nt] = acc[nt][r];
+                    if (DX && a.keep.bits) {
+                        const unsigned long long lanes = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(sign[nt], rr + 4) << 32 | (unsigned)__builtin_amdgcn_readlane(sign[nt], rr);
+                        o[nt] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? o[nt] : 0.f;
+                    }
+                }
+                T* __restrict__ yr = y + (long long)rr * F;
+                if (pairs) {
+#pragma unroll
+                    for (int nt = 0; nt + 1 < NT; nt += 2) {
+                        const T two[2] = {lb_store<T>(o[nt]), lb_store<T>(o[nt + 1])};
+                        unsigned w;
+                        __builtin_memcpy(&w, two, 4);
+                        if (feature(nt, j) < F) *reinterpret_cast<unsigned*>(yr + feature(nt, j)) = w;
+                    }
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        if (feature(nt, j) < F) yr[feature(nt, j)] = lb_store<T>(o[nt]);
+                }
+            }
+        };
+        if (!ONE) begin();
         for (int gi = 0; gi < a.groups; gi++) {
             const int g = group_at(gi);
+            int Cn = a.C;
+            asm("" : "+s"(Cn));                           // column limits are recomputed: kept over the loop they would spill
             if (a.chunk < a.groups && gi % a.chunk == 0) {
                 __syncthreads();
-                stage(gi, min(a.chunk, a.groups - gi));
+                stage(gi, min(a.chunk, a.groups - gi), s_w);
                 __syncthreads();
             }
-            if (g * 64 + 64 > C) clear_past(cur, g * 64 + 8 * h, C);
+            if (g * 64 + 64 > Cn) clear_past(cur, g * 64 + 8 * h, Cn);
             const uint4* __restrict__ wl = s_w + (size_t)(a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
@@ -543,60 +601,42 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC>)) void linear8_rows_kerne
                     else encode(Int<GS4D_FMT_E5M2>());
                 }
             }
+            if constexpr (ONE) {
+                // one group: its operands stay in registers for all of the workgroup's features
+                uint4 xs[4][TERMS];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                __builtin_amdgcn_sched_barrier(0);        // a step at a time: hoisted splits and weights would spill
-                uint4 xs[TERMS];
-                if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs);
-                else xs[0] = cur.w[t];
-                uint4 ws[NT][TERMS];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int u = 0; u < TERMS; u++) ws[nt][u] = wl[((t * NT + nt) * TERMS + u) * 64];
-#pragma unroll
-                for (int u = TERMS - 1; u >= 0; u--)      // the smallest products first
-#pragma unroll
-                    for (int z = 0; z <= u; z++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            const bool more = gi + 1 < a.groups;
-            load_group<T, VEC>(cur, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, C);
-        }
-        // ---- register r is the row (r & 3) + 8 (r >> 2) + 4 h of the tile
-        const bool whole = tile * 32 + 32 <= a.N;
-        T* __restrict__ y = (T*)a.y + (tile * 32 + 4 * h) * F;
-        const bool pairs = sizeof(T) == 2 && (F & 1) == 0 && ((uintptr_t)a.y & 3) == 0;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int rr = (r & 3) + 8 * (r >> 2);
-            if (!whole && tile * 32 + rr + 4 * h >= a.N) continue;
-            float o[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                o[nt] = acc[nt][r];
-                if (DX && a.keep.bits) {
-                    const unsigned long long lanes = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(sign[nt], rr + 4) << 32 | (unsigned)__builtin_amdgcn_readlane(sign[nt], rr);
-                    o[nt] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? o[nt] : 0.f;
+                for (int t = 0; t < 4; t++) {
+                    if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs[t]);
+                    else xs[t][0] = cur.w[t];
                 }
-            }
-            T* __restrict__ yr = y + (long long)rr * F;
-            if (pairs) {
+                for (int k = 0; k < a.blocks; k++) {
+                    begin();
 #pragma unroll
-                for (int nt = 0; nt + 1 < NT; nt += 2) {
-                    const T two[2] = {lb_store<T>(o[nt]), lb_store<T>(o[nt + 1])};
-                    unsigned w;
-                    __builtin_memcpy(&w, two, 4);
-                    if (feature(nt, j) < F) *reinterpret_cast<unsigned*>(yr + feature(nt, j)) = w;
+                    for (int t = 0; t < 4; t++) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        step(xs[t], s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
+                    }
+                    finish();
+                    f0 += NT * 32;
                 }
+                f0 -= a.blocks * NT * 32;
+                __builtin_amdgcn_sched_barrier(0);
+                load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn);
             } else {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    if (feature(nt, j) < F) yr[feature(nt, j)] = lb_store<T>(o[nt]);
+                for (int t = 0; t < 4; t++) {
+                    __builtin_amdgcn_sched_barrier(0);    // a step at a time: hoisted splits and weights would spill
+                    uint4 xs[TERMS];
+                    if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs);
+                    else xs[0] = cur.w[t];
+                    step(xs, wl + t * NT * TERMS * 64);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                const bool more = gi + 1 < a.groups;
+                load_group<T, VEC>(cur, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn);
             }
         }
+        if (!ONE) finish();
     }
 }
 
@@ -625,17 +665,26 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
     const int g = z * a.gw + wave % a.gw, slice = wave / a.gw, slices = 8 / a.gw;
     const long long n0 = chunk * a.per, n1 = n0 + a.per < a.N ? n0 + a.per : a.N;
     const bool mine = g < a.groups;
-    const int gc = min(g, a.groups - 1), m = mt * 64 + 2 * i, kp = a.keep.kp, ng = kp / 64;
-    const T* __restrict__ dy = (const T*)a.dy + (VEC ? min(m, a.M - 2) : min(m, a.M - 1));
-    const int second = m + 1 < a.M ? 1 : 0;
-    const unsigned char* __restrict__ codes = a.keep.codes + gc * 64 + 2 * i;
+    const int gc = min(g, a.groups - 1), m = mt * 64 + 2 * i, kp = a.keep.kp, ng = kp / 64, M = a.M;
+    const T* __restrict__ dy = (const T*)a.dy;
+    const int mc = VEC ? min(m, M - 2) : min(m, M - 1), second = m + 1 < M ? 1 : 0;
+    const unsigned char* __restrict__ codes = a.keep.codes + gc * 64;
     const float* __restrict__ scales = a.keep.scales + gc;
-    struct Rows { unsigned d[8][sizeof(T) / 2]; unsigned short c[8]; float s[8]; };
-    auto load = [&](Rows& r, long long r0) {
+    // a load's address is the wave's row plus the lane's share, which does not change
+    const unsigned dlane = (unsigned)((8 * h * M + mc) * (int)sizeof(T)), clane = (unsigned)(8 * h * kp + 2 * i);
+    struct Rows { unsigned d[8][sizeof(T) / 2]; unsigned short c[8]; float lo[8], hi[8]; };
+    // rows r0 + 8 h + q; LAST: some of them may lie past the end
+    auto load = [&](Rows& r, long long r0, auto last) {
+        constexpr bool LAST = decltype(last)::value != 0;
 #pragma unroll
         for (int q = 0; q < 8; q++) {
-            const long long n = r0 + 8 * h + q, row = n < a.N ? n : a.N - 1;
-            const T* p = dy + row * a.M;
+            const char* pd = reinterpret_cast<const char*>(dy + (r0 + q) * M) + dlane;
+            const char* pc = reinterpret_cast<const char*>(codes + (r0 + q) * kp) + clane;
+            if (LAST && r0 + 8 * h + q >= a.N) {          // the last row instead
+                pd = reinterpret_cast<const char*>(dy + (a.N - 1) * M + mc);
+                pc = reinterpret_cast<const char*>(codes + (a.N - 1) * kp + 2 * i);
+            }
+            const T* p = reinterpret_cast<const T*>(pd);
             if constexpr (sizeof(T) == 4) {
                 if constexpr (VEC) { const uint2 w = *reinterpret_cast<const uint2*>(p); r.d[q][0] = w.x; r.d[q][1] = w.y; }
                 else { r.d[q][0] = __float_as_uint(p[0]); r.d[q][1] = __float_as_uint(p[second]); }
@@ -643,47 +692,72 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
                 if constexpr (VEC) r.d[q][0] = *reinterpret_cast<const unsigned*>(p);
                 else { const unsigned short* u = reinterpret_cast<const unsigned short*>(p); r.d[q][0] = u[0] | (unsigned)u[second] << 16; }
             }
-            r.c[q] = *reinterpret_cast<const unsigned short*>(codes + (size_t)row * kp);
-            r.s[q] = scales[(size_t)row * ng];
+            r.c[q] = *reinterpret_cast<const unsigned short*>(pc);
+        }
+        // the scales are the same for 32 lanes: scalar loads, one of two per lane
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const long long u = r0 + q < a.N ? r0 + q : a.N - 1, v = r0 + 8 + q < a.N ? r0 + 8 + q : a.N - 1;
+            r.lo[q] = scales[(LAST ? u : r0 + q) * ng];
+            r.hi[q] = scales[(LAST ? v : r0 + 8 + q) * ng];
         }
     };
     f32x16 acc[2][2] = {};
     float db0 = 0.f, db1 = 0.f;
-    Rows cur, nxt;
-    const long long first = n0 + 16 * slice, stride = 16ll * slices;
-    if (mine && first < n1) load(cur, first);
-    if (mine)
-        for (long long r0 = first; r0 < n1; r0 += stride) {
-            load(nxt, r0 + stride);
-            float d0[8], d1[8], c0[8], c1[8];
-            const bool whole = r0 + 16 <= n1;
+    auto add = [&](const Rows& cur, long long r0, auto last) {
+        constexpr bool LAST = decltype(last)::value != 0;
+        float d0[8], d1[8], c0[8], c1[8];
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                if constexpr (sizeof(T) == 4) { d0[q] = __uint_as_float(cur.d[q][0]); d1[q] = __uint_as_float(cur.d[q][1]); }
-                else { d0[q] = low16<T>(cur.d[q][0]); d1[q] = high16<T>(cur.d[q][0]); }
-                const bool in = whole || r0 + 8 * h + q < n1;
-                if (!in) { d0[q] = 0.f; d1[q] = 0.f; cur.s[q] = 0.f; }
-                db0 += d0[q]; db1 += d1[q];
-                d0[q] *= cur.s[q]; d1[q] *= cur.s[q];
-                if constexpr (FMT == GS4D_FMT_E4M3 || FMT == GS4D_FMT_E5M2) {
-                    const float4 f = lb_decode4<FMT>(cur.c[q]);
-                    c0[q] = f.x; c1[q] = f.y;
-                } else if constexpr (FMT == GS4D_FMT_UINT8) { c0[q] = (float)(cur.c[q] & 255u); c1[q] = (float)(cur.c[q] >> 8); }
-                else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
-            }
-            uint4 da[2][TERMS], cc[2][1];
-            split8<TERMS>(d0, da[0]);
-            split8<TERMS>(d1, da[1]);
-            split8<1>(c0, cc[0]);
-            split8<1>(c1, cc[1]);
-#pragma unroll
-            for (int u = TERMS - 1; u >= 0; u--)
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int y = 0; y < 2; y++) acc[t][y] = mfma<LbBf16>(da[t][u], cc[y][0], acc[t][y]);
-            cur = nxt;
+        for (int q = 0; q < 8; q++) {
+            float s = h ? cur.hi[q] : cur.lo[q];
+            if constexpr (sizeof(T) == 4) { d0[q] = __uint_as_float(cur.d[q][0]); d1[q] = __uint_as_float(cur.d[q][1]); }
+            else { d0[q] = low16<T>(cur.d[q][0]); d1[q] = high16<T>(cur.d[q][0]); }
+            if (LAST && r0 + 8 * h + q >= n1) { d0[q] = 0.f; d1[q] = 0.f; s = 0.f; }
+            if (g == 0) { db0 += d0[q]; db1 += d1[q]; }
+            d0[q] *= s; d1[q] *= s;
+            if constexpr (FMT == GS4D_FMT_E4M3 || FMT == GS4D_FMT_E5M2) {
+                const float4 f = lb_decode4<FMT>(cur.c[q]);
+                c0[q] = f.x; c1[q] = f.y;
+            } else if constexpr (FMT == GS4D_FMT_UINT8) { c0[q] = (float)(cur.c[q] & 255u); c1[q] = (float)(cur.c[q] >> 8); }
+            else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
         }
+        uint4 da[2][TERMS], cc[2][1];
+        split8<1, false>(c0, cc[0]);
+        split8<1, false>(c1, cc[1]);
+        split8<TERMS, false>(d0, da[0]);
+        split8<TERMS, false>(d1, da[1]);
+#pragma unroll
+        for (int u = TERMS - 1; u >= 0; u--)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) acc[t][y] = mfma<LbBf16>(da[t][u], cc[y][0], acc[t][y]);
+    };
+    if (mine) {
+        // whole steps of 16 rows, the next one in flight; the chunk's last, shorter step follows
+        const long long stride = 16ll * slices, end = n1 - 15;
+        long long r0 = n0 + 16 * slice;
+        if (r0 < end) {
+            // three steps in flight: with one, a step took as long as its loads (4900 cycles for 2900 of work)
+            Rows ring[3];
+            load(ring[0], r0, Int<0>());
+            load(ring[1], r0 + stride < end ? r0 + stride : r0, Int<0>());
+            for (bool more = true; more;) {
+#pragma unroll
+                for (int u = 0; u < 3; u++) {
+                    load(ring[(u + 2) % 3], r0 + 2 * stride < end ? r0 + 2 * stride : r0, Int<0>());
+                    add(ring[u], r0, Int<0>());
+                    r0 += stride;
+                    if (r0 >= end) { more = false; break; }
+                }
+            }
+        }
+        if (r0 < n1) {
+            Rows cur;
+            load(cur, r0, Int<1>());
+            add(cur, r0, Int<1>());
+        }
+    }
     // ---- the slices of a group, in a fixed order: the upper half adds to the lower half until one is left
     for (int n = slices; n > 1; n >>= 1) {
         const int half = n >> 1;
@@ -971,12 +1045,16 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
     a.groups = (a.C + 63) / 64;
     const int per = 4 * nt * kTerms<T> * 1024;
     a.chunk = LDS / per < a.groups ? LDS / per : a.groups;
-    const size_t lds = (size_t)a.chunk * per;
-    a.ncb = (a.F + nt * 32 - 1) / (nt * 32);
+    // a contraction of one group: a workgroup takes as many of the column blocks as its LDS holds (a row's result in one go)
+    const int all = (a.F + nt * 32 - 1) / (nt * 32);
+    const bool one = a.groups == 1 && all > 1;
+    a.blocks = one ? (LDS / per < all ? LDS / per : all) : 1;
+    a.ncb = (all + a.blocks - 1) / a.blocks;
+    const size_t lds = (size_t)a.chunk * a.blocks * per;
     const long long ntile = (a.N + 31) / 32;
-    auto launch = [&](auto n, auto v) {
-        constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0>;
-        auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX>;
+    auto launch = [&](auto n, auto v, auto o) {
+        constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0, decltype(o)::value != 0>;
+        auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX, decltype(o)::value != 0>;
         // 16 waves per CU if registers and LDS allow, never more workgroups than row tiles
         long long nwg = LB_CUS * (THREADS == 512 && lds <= 78 * 1024 ? 2 : 1) / a.ncb;
         if (nwg > ntile) nwg = ntile;
@@ -987,7 +1065,10 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
         hipLaunchKernelGGL(k, dim3((unsigned)(a.nwg * a.ncb)), dim3(THREADS), lds, s, a);
         return GS4D_OK;
     };
-    auto with_nt = [&](auto n) { return vec ? launch(n, Int<1>()) : launch(n, Int<0>()); };
+    auto with_nt = [&](auto n) {
+        if (one) return vec ? launch(n, Int<1>(), Int<1>()) : launch(n, Int<0>(), Int<1>());
+        return vec ? launch(n, Int<1>(), Int<0>()) : launch(n, Int<0>(), Int<0>());
+    };
     if (nt == 2) return with_nt(Int<2>());
     if constexpr (sizeof(T) == 2) return with_nt(Int<4>());
     else return with_nt(Int<1>());
