@@ -345,8 +345,14 @@ __device__ __forceinline__ void positive_nans(Group<T>& g)
     }
 }
 
-// 16 waves where 128 registers do
-template <typename T, int NT, bool VEC, bool ONE> constexpr int kRowsThreads = VEC && NT <= 2 && !ONE ? 1024 : 512;
+// How the groups of the contraction and the column blocks are walked:
+//   ROWS_ONE   one group, one column block (64 x 64 layers): nothing to prefetch within a tile, 16 waves of 128 registers
+//              (100 k rows: 23 us; as ROWS_MANY 26)
+//   ROWS_WIDE  one group, several column blocks: the group's operands stay in registers for all of them
+//   ROWS_MANY  several groups: the next one is in flight while this one is multiplied, 8 waves (1.2 M x 256: 463 us; 16 waves
+//              without the prefetch 503)
+enum { ROWS_ONE, ROWS_WIDE, ROWS_MANY };
+template <typename T, int NT, bool VEC, int MODE> constexpr int kRowsThreads = VEC && NT <= 2 && MODE == ROWS_ONE ? 1024 : 512;
 
 struct RowsArgs {
     long long N; int C, F;                // rows, contraction length, features of the result
@@ -357,7 +363,7 @@ struct RowsArgs {
     int lowest;                           // relu_bits()
     Keep keep; int fmt;                   // forward: what to keep; dx: keep.bits masks the result
     int ncb, nwg, groups, chunk;          // sets of column blocks, workgroups per set, groups of 64 of the contraction, groups in LDS at once
-    int blocks;                           // column blocks of NT * 32 features per set: 1, or more where the contraction is one group (ONE)
+    int blocks;                           // column blocks of NT * 32 features per set: 1, or more where the contraction is one group (ROWS_WIDE)
 };
 
 // Both products over the rows, y = x W^T (+ bias) and dx = dy W: a wave owns 32 rows and NT tiles of 32 features of
@@ -367,10 +373,10 @@ struct RowsArgs {
 // holds the features 32 nt + lane, for 16-bit types the features 2 lane + (nt & 1) of 64, which leave as one word.
 // The weight lies in LDS as MFMA operands, split once per workgroup, for as many groups as fit; the waves of a workgroup walk the
 // rows.  What the backward needs of x is quantised on the way, from the registers that feed the product: x is read once.
-template <typename T, int NT, bool VEC, bool DX, bool ONE>
-__global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_kernel(RowsArgs a)
+template <typename T, int NT, bool VEC, bool DX, int MODE>
+__global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows_kernel(RowsArgs a)
 {
-    constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC, ONE>, WAVES = THREADS / 64, BLOCK = 4 * NT * TERMS * 64;
+    constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC, MODE>, WAVES = THREADS / 64, BLOCK = 4 * NT * TERMS * 64;
     extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
     // workgroups that share rows differ by 8 in their number, i.e. run on one XCD behind one L2
@@ -426,7 +432,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
     const int turn = a.chunk >= a.groups ? wave % a.groups : 0;
     auto group_at = [&](int gi) { const int g = gi + turn; return g < a.groups ? g : g - a.groups; };
     load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C);      // in flight while the weight is staged
-    if constexpr (ONE) {
+    if constexpr (MODE == ROWS_WIDE) {
         for (int k = 0; k < a.blocks; k++) { stage(0, 1, s_w + k * BLOCK); f0 += NT * 32; }
         f0 -= a.blocks * NT * 32;
     } else if (a.chunk >= a.groups) {
@@ -498,7 +504,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
                 }
             }
         };
-        if (!ONE) begin();
+        if (MODE != ROWS_WIDE) begin();
         for (int gi = 0; gi < a.groups; gi++) {
             const int g = group_at(gi);
             int Cn = a.C;
@@ -510,6 +516,9 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
             }
             if (g * 64 + 64 > Cn) clear_past(cur, g * 64 + 8 * h, Cn);
             const uint4* __restrict__ wl = s_w + (size_t)(a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
+            const bool more = gi + 1 < a.groups;
+            Group<T> nxt;
+            if (MODE == ROWS_MANY) load_group<T, VEC>(nxt, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn);
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
             float v[4][8];
@@ -601,7 +610,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
                     else encode(Int<GS4D_FMT_E5M2>());
                 }
             }
-            if constexpr (ONE) {
+            if constexpr (MODE == ROWS_WIDE) {
                 // one group: its operands stay in registers for all of the workgroup's features
                 uint4 xs[4][TERMS];
 #pragma unroll
@@ -613,7 +622,6 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
                     begin();
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                        __builtin_amdgcn_sched_barrier(0);
                         step(xs[t], s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
                     }
                     finish();
@@ -625,18 +633,21 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, ONE>)) void linear8_rows_
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    __builtin_amdgcn_sched_barrier(0);    // a step at a time: hoisted splits and weights would spill
+                    if (MODE == ROWS_ONE) __builtin_amdgcn_sched_barrier(0);      // a step at a time: hoisted splits and weights would spill
                     uint4 xs[TERMS];
                     if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs);
                     else xs[0] = cur.w[t];
                     step(xs, wl + t * NT * TERMS * 64);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                const bool more = gi + 1 < a.groups;
-                load_group<T, VEC>(cur, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn);
+                if (MODE == ROWS_MANY) {
+                    cur = nxt;
+                } else {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn);
+                }
             }
         }
-        if (!ONE) finish();
+        if (MODE != ROWS_WIDE) finish();
     }
 }
 
@@ -1047,14 +1058,14 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
     a.chunk = LDS / per < a.groups ? LDS / per : a.groups;
     // a contraction of one group: a workgroup takes as many of the column blocks as its LDS holds (a row's result in one go)
     const int all = (a.F + nt * 32 - 1) / (nt * 32);
-    const bool one = a.groups == 1 && all > 1;
-    a.blocks = one ? (LDS / per < all ? LDS / per : all) : 1;
+    const int mode = a.groups > 1 ? ROWS_MANY : all > 1 ? ROWS_WIDE : ROWS_ONE;
+    a.blocks = mode == ROWS_WIDE ? (LDS / per < all ? LDS / per : all) : 1;
     a.ncb = (all + a.blocks - 1) / a.blocks;
     const size_t lds = (size_t)a.chunk * a.blocks * per;
     const long long ntile = (a.N + 31) / 32;
     auto launch = [&](auto n, auto v, auto o) {
-        constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0, decltype(o)::value != 0>;
-        auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX, decltype(o)::value != 0>;
+        constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0, decltype(o)::value>;
+        auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX, decltype(o)::value>;
         // 16 waves per CU if registers and LDS allow, never more workgroups than row tiles
         long long nwg = LB_CUS * (THREADS == 512 && lds <= 78 * 1024 ? 2 : 1) / a.ncb;
         if (nwg > ntile) nwg = ntile;
@@ -1066,8 +1077,8 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
         return GS4D_OK;
     };
     auto with_nt = [&](auto n) {
-        if (one) return vec ? launch(n, Int<1>(), Int<1>()) : launch(n, Int<0>(), Int<1>());
-        return vec ? launch(n, Int<1>(), Int<0>()) : launch(n, Int<0>(), Int<0>());
+        auto with_mode = [&](auto v) { return mode == ROWS_MANY ? launch(n, v, Int<ROWS_MANY>()) : mode == ROWS_WIDE ? launch(n, v, Int<ROWS_WIDE>()) : launch(n, v, Int<ROWS_ONE>()); };
+        return vec ? with_mode(Int<1>()) : with_mode(Int<0>());
     };
     if (nt == 2) return with_nt(Int<2>());
     if constexpr (sizeof(T) == 2) return with_nt(Int<4>());
