@@ -33,6 +33,7 @@
 
 #include "gs4d_internal.h"
 #include "deform_hexplane.h"
+#include "lowbit.h"
 
 #define WIDTH 64            // net_width of every supported config
 #define NHEAD 4             // pos, scales, rotations, shs
@@ -1268,6 +1269,56 @@ static GemmJob simple_job(const float* A, int lda, int acol0, int K, int relu_a,
     return j;
 }
 
+static int launch_pe_forward(const gs4d_deform_desc* d, const Layout& l, int P, const float* points, const float* scales,
+                             const float* rotations, const float* time, const float* force, float* Z, hipStream_t s)
+{
+    const PeArgs pa = {P, l.ldz, l.oX, l.oS, l.oR, l.oT, l.oF, l.Kz, d->pos_pe, d->sr_pe, d->time_pe, d->force_pe,
+                       d->use_time, d->use_force};
+    const size_t lds = sizeof(float) * PE_PTS * (size_t)(l.ldz - l.oX);     // 14 KB at the mutant shape
+    if (lds > 48 * 1024 || l.ldz - l.oX > PE_MAX_SLOTS) { gs4d_set_error("deform forward: %d positional-encoding columns exceed the LDS tile", l.ldz - l.oX); return GS4D_EINVAL; }
+    hipLaunchKernelGGL(pe_forward_kernel, dim3((unsigned)(((size_t)P + PE_PTS - 1) / PE_PTS)), dim3(256), lds, s, pa,
+                       points, scales, rotations, time, force, Z);
+    GS4D_LAUNCH_CHECK("pe_forward", 0, s);
+    return GS4D_OK;
+}
+
+// ---- the 8-bit checkpoint: the inputs of every Linear but the encodings, which are computed again
+__global__ __launch_bounds__(256) void checkpoint_copy_kernel(int P, float* __restrict__ tprime, float* __restrict__ O, float* __restrict__ kept_t,
+                                                              float4* __restrict__ kept_rot, int write)
+{
+    const int p = blockIdx.x * 256 + threadIdx.x;
+    if (p >= P) return;
+    float4* rot = reinterpret_cast<float4*>(O + (size_t)p * OUT_LD + OC_R);
+    if (write) { kept_t[p] = tprime[p]; kept_rot[p] = *rot; }
+    else { tprime[p] = kept_t[p]; *rot = kept_rot[p]; }
+}
+
+struct Checkpoint { float* tprime; float4* rot; Gs4dKeepJobs jobs; };
+
+static Checkpoint carve_checkpoint(char* base, const gs4d_deform_desc* d, const Layout& l, const Workspace& w, size_t P, size_t* bytes)
+{
+    Checkpoint c = {};
+    char* p = base;
+    gs4d_obtain(p, c.rot, P);
+    gs4d_obtain(p, c.tprime, P);
+    auto add = [&](float* x, int ld, int width, int relu, unsigned* hmask, int hword) {
+        Gs4dKeepJob& j = c.jobs.j[c.jobs.n];
+        const int groups = (width + 63) / 64;
+        j = {x, ld, width, relu, nullptr, nullptr, nullptr, hmask, 10, hword};
+        gs4d_obtain(p, j.codes, P * groups * 64);
+        gs4d_obtain(p, j.scales, P * groups);
+        if (relu) gs4d_obtain(p, j.bits, P * groups * 2);
+        c.jobs.group0[c.jobs.n + 1] = c.jobs.group0[c.jobs.n] + groups;
+        c.jobs.n++;
+    };
+    add(w.feat, l.F, l.F, 0, nullptr, 0);
+    for (int i = 0; i + 1 < d->trunk_layers; i++) add(w.trunk[i], WIDTH, WIDTH, 1, nullptr, 0);
+    add(w.Z, l.ldz, WIDTH, 1, w.hmask, 8);                // the hidden columns; hmask words 8, 9
+    add(w.H1, NHEAD * WIDTH, NHEAD * WIDTH, 1, w.hmask, 0);
+    if (bytes) *bytes = (size_t)(p - base) + 256;
+    return c;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1342,19 +1393,13 @@ int gs4d_deform_forward(const gs4d_deform_desc* d, int P, const float* points, c
 
     {
         GS4D_PROF("hexplane_forward", s);
-        rc = gs4d_hex_launch_forward(d, P, points, time, force, w.tprime, w.feat, l.F, s);
+        rc = d->no_grad && d->static_codes ? gs4d_hex_launch_frozen(d, P, points, time, force, w.feat, l.F, s)
+                                           : gs4d_hex_launch_forward(d, P, points, time, force, w.tprime, w.feat, l.F, s);
         if (rc) return rc;
     }
     GS4D_PROF("mlp_forward", s);
-    PeArgs pa = {P, l.ldz, l.oX, l.oS, l.oR, l.oT, l.oF, l.Kz, d->pos_pe, d->sr_pe, d->time_pe, d->force_pe,
-                 d->use_time, d->use_force};
-    {
-        const size_t lds = sizeof(float) * PE_PTS * (size_t)(l.ldz - l.oX);     // 14 KB at the mutant shape
-        if (lds > 48 * 1024 || l.ldz - l.oX > PE_MAX_SLOTS) { gs4d_set_error("deform forward: %d positional-encoding columns exceed the LDS tile", l.ldz - l.oX); return GS4D_EINVAL; }
-        hipLaunchKernelGGL(pe_forward_kernel, dim3((unsigned)(((size_t)P + PE_PTS - 1) / PE_PTS)), dim3(256), lds, s, pa,
-                           points, scales, rotations, time, force, w.Z);
-        GS4D_LAUNCH_CHECK("pe_forward", 0, s);
-    }
+    rc = launch_pe_forward(d, l, P, points, scales, rotations, time, force, w.Z, s);
+    if (rc) return rc;
     // trunk
     for (int i = 0; i < d->trunk_layers; i++) {
         GemmJobs jobs = {};
@@ -1402,6 +1447,59 @@ int gs4d_deform_forward(const gs4d_deform_desc* d, int P, const float* points, c
         GS4D_LAUNCH_CHECK("deform_outputs_forward", 0, s);
     }
     return GS4D_OK;
+}
+
+size_t gs4d_deform_checkpoint_bytes(const gs4d_deform_desc* d, int P)
+{
+    if (validate(d, P)) return 0;
+    const Layout l = make_layout(d);
+    const Workspace w = carve_workspace(nullptr, d, l, (size_t)P, nullptr);
+    size_t bytes = 0;
+    carve_checkpoint(nullptr, d, l, w, (size_t)P, &bytes);
+    return bytes;
+}
+
+static int checkpoint_move(const gs4d_deform_desc* d, int P, char* checkpoint, char* workspace, bool write, hipStream_t s)
+{
+    const Layout l = make_layout(d);
+    const Workspace w = carve_workspace(workspace, d, l, (size_t)P, nullptr);
+    const Checkpoint c = carve_checkpoint(checkpoint, d, l, w, (size_t)P, nullptr);
+    const int rc = gs4d_launch_keep(c.jobs, P, write, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL(checkpoint_copy_kernel, dim3((P + 255) / 256), dim3(256), 0, s, P, w.tprime, w.O, c.tprime, c.rot, write ? 1 : 0);
+    GS4D_LAUNCH_CHECK("deform_checkpoint", 0, s);
+    return GS4D_OK;
+}
+
+int gs4d_deform_checkpoint_pack(const gs4d_deform_desc* d, int P, char* workspace, char* checkpoint, void* stream)
+{
+    GS4D_TRACE_SCOPE("gs4d_deform_checkpoint_pack");
+    const int rc = validate(d, P);
+    if (rc) return rc;
+    if (P == 0) return GS4D_OK;
+    if (!workspace || !checkpoint || ((uintptr_t)workspace & 255) || ((uintptr_t)checkpoint & 255) || d->no_grad) {
+        gs4d_set_error("gs4d_deform_checkpoint_pack: null or misaligned pointer, or a forward without a backward (no_grad)");
+        return GS4D_EINVAL;
+    }
+    return checkpoint_move(d, P, checkpoint, workspace, true, (hipStream_t)stream);
+}
+
+int gs4d_deform_checkpoint_unpack(const gs4d_deform_desc* d, int P, const float* points, const float* scales, const float* rotations,
+                                  const float* time, const float* force, char* checkpoint, char* workspace, void* stream)
+{
+    GS4D_TRACE_SCOPE("gs4d_deform_checkpoint_unpack");
+    const int rc = validate(d, P);
+    if (rc) return rc;
+    if (P == 0) return GS4D_OK;
+    if (!points || !scales || !rotations || !time || !force || !workspace || !checkpoint || ((uintptr_t)workspace & 255) || ((uintptr_t)checkpoint & 255)) {
+        gs4d_set_error("gs4d_deform_checkpoint_unpack: null or misaligned pointer");
+        return GS4D_EINVAL;
+    }
+    const Layout l = make_layout(d);
+    const Workspace w = carve_workspace(workspace, d, l, (size_t)P, nullptr);
+    const int rc2 = launch_pe_forward(d, l, P, points, scales, rotations, time, force, w.Z, (hipStream_t)stream);
+    if (rc2) return rc2;
+    return checkpoint_move(d, P, checkpoint, workspace, false, (hipStream_t)stream);
 }
 
 int gs4d_deform_backward_phases(const gs4d_deform_desc* d, const gs4d_deform_grads* g, int P, const float* points,

@@ -24,6 +24,9 @@ size_t gs4d_hex_batch_points(const gs4d_deform_desc* d, size_t P);
 // feat[p][l * C + c] = product over the six planes of level l of their bilinear samples; tprime[p] = t'
 int gs4d_hex_launch_forward(const gs4d_deform_desc* d, int P, const float* points, const float* time, const float* force,
                             float* tprime, float* feat, int ldf, hipStream_t s);
+// the same features with the spatial planes' product from the descriptor's cache (gs4d_deform_desc::static_codes)
+int gs4d_hex_launch_frozen(const gs4d_deform_desc* d, int P, const float* points, const float* time, const float* force,
+                           float* feat, int ldf, hipStream_t s);
 // plane gradients (accumulated into g->planes), dL_dpoints += the path through the planes, per-workgroup partial sums of
 // the t' gradient in dtprime (3 floats per 256 points; summed by the caller).  hist arrives zeroed.
 int gs4d_hex_launch_backward(const gs4d_deform_desc* d, const gs4d_deform_grads* g, int P, const float* points,

@@ -170,13 +170,25 @@ __global__ __launch_bounds__(256) void hexplane_forward_shared_kernel(
 
 // The features of a frame from a cache of the spatial planes' product (gs4d_frame_features): three bilinear samples per level
 // over (axis, t) and one 8-bit row, instead of six samples.  C / 4 lanes per point, 4 channels each.
+struct FrameTime {                       // t' of row p: t[p * stride], or with ft_w the field's embedding of (time, force)
+    const float* t; const float* force; const float* ft_w; const float* ft_b; int use_time, use_force, stride;
+};
+__device__ __forceinline__ float frame_time(const FrameTime& a, long long p)
+{
+    const float v = a.t[p * a.stride];
+    if (!a.ft_w) return v;
+    const float f = a.force[p * a.stride];
+    return (a.use_time ? v : v * 0.0f) * a.ft_w[0] + (a.use_force ? f : f * 0.0f) * a.ft_w[1] + a.ft_b[0];
+}
+// the cache row of row p: the rows of a call may be several copies of the cache's points
+__device__ __forceinline__ long long cache_row(long long p, long long P, unsigned rows) { return P > rows ? (long long)((unsigned)p % rows) : p; }
+
 struct FramePlanes { const float* p[GS4D_MAX_LEVELS * 3]; int w[GS4D_MAX_LEVELS * 3]; int h[GS4D_MAX_LEVELS * 3]; };
 
 template <int FMT>
 __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L, int C, int lpp_shift, FramePlanes T,
                                                              const float* __restrict__ aabb, const float* __restrict__ xyz,
-                                                             const float* __restrict__ t, int t_stride, long long P,
-                                                             float* __restrict__ out, long long ld)
+                                                             FrameTime ft, long long P, float* __restrict__ out, long long ld)
 {
     const long long gtid = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long p = gtid >> lpp_shift;
@@ -188,12 +200,13 @@ __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L
         const float lo = aabb[a], hi = aabb[3 + a];
         u[a] = (xyz[3 * p + a] - lo) * (2.0f / (hi - lo)) - 1.0f;
     }
-    const float tt = t[p * t_stride];
+    const float tt = frame_time(ft, p);
+    const long long row = cache_row(p, P, (unsigned)c.capacity);
     const int ng = (c.width + c.group - 1) / c.group, q = C >> 2;
     for (int l = 0; l < L; l++) {
         const int col = l * C + 4 * sub;
-        const float s = c.scales[p * ng + col / c.group];
-        const float4 k = lb_decode4<FMT>(*reinterpret_cast<const unsigned*>(c.codes + (size_t)p * c.pitch + col));
+        const float s = c.scales[row * ng + col / c.group];
+        const float4 k = lb_decode4<FMT>(*reinterpret_cast<const unsigned*>(c.codes + (size_t)row * c.pitch + col));
         float4 acc = make_float4(s * k.x, s * k.y, s * k.z, s * k.w);
 #pragma unroll
         for (int a = 0; a < 3; a++) {
@@ -210,6 +223,37 @@ __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L
     }
 }
 
+// What the cache holds: the product of a level's (x, y), (x, z) and (y, z) planes (no frame needs it again).
+__global__ __launch_bounds__(256) void static_features_kernel(int P, int C, int L, int lpp_shift, PlaneTable T, const float* __restrict__ aabb,
+                                                              const float* __restrict__ xyz, float* __restrict__ out)
+{
+    const long long gtid = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int p = (int)(gtid >> lpp_shift), sub = (int)(gtid & ((1 << lpp_shift) - 1)), q = C >> 2;
+    if (p >= P) return;
+    float u[3];
+#pragma unroll
+    for (int a = 0; a < 3; a++) {
+        const float lo = aabb[a], hi = aabb[3 + a];
+        u[a] = (xyz[3 * (size_t)p + a] - lo) * (2.0f / (hi - lo)) - 1.0f;
+    }
+    for (int l = 0; l < L; l++) {
+        float4 acc = make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const int pl = l * 6 + (i == 2 ? 3 : i), a = i == 2 ? 1 : 0, b = i == 0 ? 1 : 2;
+            const Corner n = corner_of(u[a], u[b], T.w[pl], T.h[pl]);
+            const float4* __restrict__ base = reinterpret_cast<const float4*>(T.p[pl]) + sub;
+            const float4 f00 = base[(size_t)n.i00 * q], f01 = base[(size_t)n.i01 * q];
+            const float4 f10 = base[(size_t)n.i10 * q], f11 = base[(size_t)n.i11 * q];
+            acc.x *= f00.x * n.w00 + f01.x * n.w01 + f10.x * n.w10 + f11.x * n.w11;
+            acc.y *= f00.y * n.w00 + f01.y * n.w01 + f10.y * n.w10 + f11.y * n.w11;
+            acc.z *= f00.z * n.w00 + f01.z * n.w01 + f10.z * n.w10 + f11.z * n.w11;
+            acc.w *= f00.w * n.w00 + f01.w * n.w01 + f10.w * n.w10 + f11.w * n.w11;
+        }
+        reinterpret_cast<float4*>(out + (size_t)p * L * C + l * C)[sub] = acc;
+    }
+}
+
 // The same with ONE t for all points: a plane over (axis, t) is then a line over the axis, the two rows around t blended.  A
 // workgroup blends the lines of its `slice` channels into LDS once and walks the points with half the corner rows, all of them in
 // LDS: what is left to memory is the cache row, the point and the result.  slice / 4 lanes per point, 4 channels of every level
@@ -218,7 +262,7 @@ __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L
 struct FrameArgs {
     gs4d_rows8 c; int L, C, slice, nslices, nwg, gshift;
     FramePlanes T; int row0[GS4D_MAX_LEVELS * 3];        // first LDS row of a line
-    const float* aabb; const float* xyz; const float* t; long long P; float* out; long long ld;
+    const float* aabb; const float* xyz; FrameTime ft; long long P; float* out; long long ld;
 };
 
 template <int FMT, int L>
@@ -229,7 +273,7 @@ __global__ __launch_bounds__(512) void frame_lines_kernel(FrameArgs a)
     const int rest = blockIdx.x >> 3, sl = (a.nwg & 7) ? blockIdx.x % a.nslices : rest % a.nslices;
     const int wg = (a.nwg & 7) ? blockIdx.x / a.nslices : (rest / a.nslices) * 8 + (blockIdx.x & 7);
     const int ch0 = sl * a.slice;
-    const float tt = a.t[0];
+    const float tt = frame_time(a.ft, 0);
     for (int i = 0; i < 3 * L; i++) {
         const int H = a.T.h[i], W = a.T.w[i];
         const float y = fminf(fmaxf((tt + 1.f) * 0.5f * (float)(H - 1), 0.f), (float)(H - 1)), y0 = floorf(y), wy = y - y0;
@@ -250,13 +294,14 @@ __global__ __launch_bounds__(512) void frame_lines_kernel(FrameArgs a)
     struct Point { float x[3], s[L]; unsigned k[L]; } cur, nxt;
     auto load = [&](Point& o, long long p) {
         p = p < a.P ? p : a.P - 1;
+        const long long row = cache_row(p, a.P, (unsigned)a.c.capacity);
 #pragma unroll
         for (int k = 0; k < 3; k++) o.x[k] = a.xyz[3 * p + k];
 #pragma unroll
         for (int l = 0; l < L; l++) {
             const int col = l * a.C + ch0 + 4 * sub;
-            o.k[l] = *reinterpret_cast<const unsigned*>(a.c.codes + (size_t)p * a.c.pitch + col);
-            o.s[l] = a.c.scales[p * ng + (col >> a.gshift)];
+            o.k[l] = *reinterpret_cast<const unsigned*>(a.c.codes + (size_t)row * a.c.pitch + col);
+            o.s[l] = a.c.scales[row * ng + (col >> a.gshift)];
         }
     };
     long long p = (long long)wg * ppw + (threadIdx.x >> shift);
@@ -1034,38 +1079,19 @@ int gs4d_hex_launch_backward(const gs4d_deform_desc* d, const gs4d_deform_grads*
     return GS4D_OK;
 }
 
-extern "C" int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const float* const* planes, const int* plane_w,
-                                   const int* plane_h, const float* aabb, const float* points, const float* t, int t_stride,
-                                   long long P, float* out, long long ld, void* stream)
+// c->capacity >= 1 rows; P rows that are the cache's first ones, or several copies of all of them
+static int launch_frame(const gs4d_rows8* c, int L, int C, const FramePlanes& T, const float* aabb, const float* points, const FrameTime& ft,
+                        long long P, float* out, long long ld, hipStream_t s)
 {
-    GS4D_TRACE_SCOPE("gs4d_frame_features");
-    hipStream_t s = (hipStream_t)stream;
-    if (!c || L < 1 || L > GS4D_MAX_LEVELS || C < 4 || C > 256 || (C & (C - 1)) || c->width != L * C || P < 0 || P > c->capacity ||
-        !c->codes || !c->scales || c->pitch < c->width || (c->pitch & 15) || ((uintptr_t)c->codes & 15) ||
-        (c->group != 32 && c->group != 64 && c->group != 128) || c->fmt < GS4D_FMT_INT8 || c->fmt > GS4D_FMT_E5M2) {
-        gs4d_set_error("gs4d_frame_features: bad cache, levels or channels (rows of L * C values, C a power of two in [4, 256], at least P rows)");
-        return GS4D_EINVAL;
-    }
-    if (P == 0) return GS4D_OK;
-    if (!planes || !plane_w || !plane_h || !aabb || !points || !t || !out || ((uintptr_t)out & 15) || (ld & 3) || ld < c->width ||
-        (t_stride != 0 && t_stride != 1)) {
-        gs4d_set_error("gs4d_frame_features: null or misaligned pointer, or a row pitch that is too small or no multiple of 4");
-        return GS4D_EINVAL;
-    }
-    FramePlanes T = {};
-    for (int i = 0; i < L * 3; i++) {
-        if (!planes[i] || ((uintptr_t)planes[i] & 15) || plane_w[i] < 1 || plane_h[i] < 1) { gs4d_set_error("gs4d_frame_features: plane %d null, empty or not 16-byte aligned", i); return GS4D_EINVAL; }
-        T.p[i] = planes[i]; T.w[i] = plane_w[i]; T.h[i] = plane_h[i];
-    }
     // one t and enough points to pay for the lines: about 10 us of blending per workgroup against 60 ns a point and CU
     int rows = 0;
     FrameArgs f = {};
-    for (int i = 0; i < L * 3; i++) { f.row0[i] = rows; rows += plane_w[i]; }
+    for (int i = 0; i < L * 3; i++) { f.row0[i] = rows; rows += T.w[i]; }
     f.slice = C < 64 ? C : 64;
     while (f.slice > 4 && (size_t)rows * f.slice * sizeof(float) > 78 * 1024) f.slice >>= 1;
     const size_t lds = (size_t)rows * f.slice * sizeof(float);
-    if (t_stride == 0 && lds <= 78 * 1024 && (long long)P * C >= FRAME_LINES_MIN) {
-        f.c = *c; f.L = L; f.C = C; f.nslices = C / f.slice; f.T = T; f.aabb = aabb; f.xyz = points; f.t = t; f.P = P; f.out = out; f.ld = ld;
+    if (ft.stride == 0 && lds <= 78 * 1024 && (long long)P * C >= FRAME_LINES_MIN) {
+        f.c = *c; f.L = L; f.C = C; f.nslices = C / f.slice; f.T = T; f.aabb = aabb; f.xyz = points; f.ft = ft; f.P = P; f.out = out; f.ld = ld;
         f.gshift = c->group == 32 ? 5 : c->group == 64 ? 6 : 7;
         const long long ppw = 512 / (f.slice / 4), need = (P + ppw - 1) / ppw;
         long long nwg = 512 / f.nslices;
@@ -1090,9 +1116,78 @@ extern "C" int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const floa
     int lpp_shift = 0;
     while ((1 << lpp_shift) < C / 4) lpp_shift++;
     const size_t threads = (size_t)P << lpp_shift;
-    if (threads > 0xffffff00ull) { gs4d_set_error("gs4d_frame_features: %lld points are too many for one call", P); return GS4D_EINVAL; }
+    if (threads > 0xffffff00ull) { gs4d_set_error("plane features: %lld points are too many for one call", P); return GS4D_EINVAL; }
     auto k = c->fmt == GS4D_FMT_INT8 ? frame_features_kernel<GS4D_FMT_INT8> : c->fmt == GS4D_FMT_E4M3 ? frame_features_kernel<GS4D_FMT_E4M3> : frame_features_kernel<GS4D_FMT_E5M2>;
-    hipLaunchKernelGGL(k, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, *c, L, C, lpp_shift, T, aabb, points, t, t_stride, P, out, ld);
+    hipLaunchKernelGGL(k, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, *c, L, C, lpp_shift, T, aabb, points, ft, P, out, ld);
     GS4D_LAUNCH_CHECK("frame_features", 0, s);
+    return GS4D_OK;
+}
+
+extern "C" int gs4d_frame_features(const gs4d_rows8* c, int L, int C, const float* const* planes, const int* plane_w,
+                                   const int* plane_h, const float* aabb, const float* points, const float* t, int t_stride,
+                                   long long P, float* out, long long ld, void* stream)
+{
+    GS4D_TRACE_SCOPE("gs4d_frame_features");
+    hipStream_t s = (hipStream_t)stream;
+    if (!c || L < 1 || L > GS4D_MAX_LEVELS || C < 4 || C > 256 || (C & (C - 1)) || c->width != L * C || P < 0 || P > c->capacity ||
+        !c->codes || !c->scales || c->pitch < c->width || (c->pitch & 15) || ((uintptr_t)c->codes & 15) ||
+        (c->group != 32 && c->group != 64 && c->group != 128) || c->fmt < GS4D_FMT_INT8 || c->fmt > GS4D_FMT_E5M2) {
+        gs4d_set_error("gs4d_frame_features: bad cache, levels or channels (rows of L * C values, C a power of two in [4, 256], at least P rows)");
+        return GS4D_EINVAL;
+    }
+    if (P == 0) return GS4D_OK;
+    if (!planes || !plane_w || !plane_h || !aabb || !points || !t || !out || ((uintptr_t)out & 15) || (ld & 3) || ld < c->width ||
+        (t_stride != 0 && t_stride != 1)) {
+        gs4d_set_error("gs4d_frame_features: null or misaligned pointer, or a row pitch that is too small or no multiple of 4");
+        return GS4D_EINVAL;
+    }
+    FramePlanes T = {};
+    for (int i = 0; i < L * 3; i++) {
+        if (!planes[i] || ((uintptr_t)planes[i] & 15) || plane_w[i] < 1 || plane_h[i] < 1) { gs4d_set_error("gs4d_frame_features: plane %d null, empty or not 16-byte aligned", i); return GS4D_EINVAL; }
+        T.p[i] = planes[i]; T.w[i] = plane_w[i]; T.h[i] = plane_h[i];
+    }
+    const FrameTime ft = {t, nullptr, nullptr, nullptr, 1, 1, t_stride};
+    return launch_frame(c, L, C, T, aabb, points, ft, P, out, ld, s);
+}
+
+int gs4d_hex_launch_frozen(const gs4d_deform_desc* d, int P, const float* points, const float* time, const float* force,
+                           float* feat, int ldf, hipStream_t s)
+{
+    const gs4d_rows8 c = {const_cast<unsigned char*>(d->static_codes), const_cast<float*>(d->static_scales), nullptr, d->static_rows,
+                          d->L * d->C, d->static_pitch, d->static_group, d->static_fmt};
+    if (!c.scales || c.capacity < 1 || P % d->static_rows || c.pitch < c.width || (c.pitch & 15) || ((uintptr_t)c.codes & 15) ||
+        (c.group != 32 && c.group != 64 && c.group != 128) || c.fmt < GS4D_FMT_INT8 || c.fmt > GS4D_FMT_E5M2) {
+        gs4d_set_error("deform: %d rows do not fit the frozen planes' cache of %d rows, or the cache is malformed", P, d->static_rows);
+        return GS4D_EINVAL;
+    }
+    static const int kTimePlane[3] = {2, 4, 5};           // (x, t), (y, t), (z, t) among a level's six
+    FramePlanes T = {};
+    for (int i = 0; i < d->L * 3; i++) {
+        const int pl = i / 3 * 6 + kTimePlane[i % 3];
+        if (!d->planes[pl] || ((uintptr_t)d->planes[pl] & 15)) { gs4d_set_error("deform: plane %d null or not 16-byte aligned", pl); return GS4D_EINVAL; }
+        T.p[i] = d->planes[pl]; T.w[i] = d->plane_w[pl]; T.h[i] = d->plane_h[pl];
+    }
+    const FrameTime ft = {time, force, d->ft_w, d->ft_b, d->use_time, d->use_force, d->uniform_time ? 0 : 1};
+    return launch_frame(&c, d->L, d->C, T, d->aabb, points, ft, P, feat, ldf, s);
+}
+
+extern "C" int gs4d_static_features(const gs4d_deform_desc* d, int P, const float* points, float* out, void* stream)
+{
+    GS4D_TRACE_SCOPE("gs4d_static_features");
+    hipStream_t s = (hipStream_t)stream;
+    if (!d || P < 0 || d->L < 1 || d->L > GS4D_MAX_LEVELS || d->C < 4 || d->C > 256 || (d->C & (d->C - 1))) { gs4d_set_error("gs4d_static_features: bad descriptor or negative P"); return GS4D_EINVAL; }
+    if (P == 0) return GS4D_OK;
+    if (!points || !out || ((uintptr_t)out & 15) || !d->aabb) { gs4d_set_error("gs4d_static_features: null or misaligned pointer"); return GS4D_EINVAL; }
+    PlaneTable T = {};
+    for (int i = 0; i < d->L * 6; i++) {
+        if (!d->planes[i] || ((uintptr_t)d->planes[i] & 15)) { gs4d_set_error("gs4d_static_features: plane %d null or not 16-byte aligned", i); return GS4D_EINVAL; }
+        T.p[i] = d->planes[i]; T.w[i] = d->plane_w[i]; T.h[i] = d->plane_h[i];
+    }
+    int lpp_shift = 0;
+    while ((1 << lpp_shift) < d->C / 4) lpp_shift++;
+    const size_t threads = (size_t)P << lpp_shift;
+    if (threads > 0xffffff00ull) { gs4d_set_error("gs4d_static_features: %d points are too many for one call", P); return GS4D_EINVAL; }
+    hipLaunchKernelGGL(static_features_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, P, d->C, d->L, lpp_shift, T, d->aabb, points, out);
+    GS4D_LAUNCH_CHECK("static_features", 0, s);
     return GS4D_OK;
 }

@@ -90,3 +90,13 @@ template <> __device__ __forceinline__ LbBf16 lb_store<LbBf16>(float x)
 }
 
 static inline int lb_groups(int width, int group) { return (width + group - 1) / group; }
+
+// One matrix of float32 rows kept as 8-bit rows (groups of 64 columns) and back: lowbit.hip, for the deformation field's checkpoint.
+// x [rows][ld] (16-byte aligned, ld and width multiples of 4) <-> codes [rows][groups * 64], scales [rows][groups] and, rectified
+// (relu: the values kept are max(x, 0)), bits [rows][groups][2] (bit c of a group: x > 0).  Read back, a rectified number whose bit
+// is set is positive, whatever its code.  hmask (read only): the bits again, as rows of hld words at word hword + 2 * group, bit
+// 4 m + q of word h standing for column 8 m + 4 h + q.
+struct Gs4dKeepJob { float* x; int ld, width, relu; unsigned char* codes; float* scales; unsigned* bits; unsigned* hmask; int hld, hword; };
+#define GS4D_KEEP_JOBS 12
+struct Gs4dKeepJobs { Gs4dKeepJob j[GS4D_KEEP_JOBS]; int n, group0[GS4D_KEEP_JOBS + 1]; };
+int gs4d_launch_keep(const Gs4dKeepJobs& jobs, long long rows, bool write, hipStream_t s);

@@ -183,6 +183,94 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
     }
 }
 
+// ------------------------------------------------------------------ several matrices of rows at once (Gs4dKeepJobs)
+// blockIdx.y: a group of 64 columns of one of the matrices; 16 lanes of 4 columns each, 64 rows per workgroup
+template <bool WRITE>
+__global__ __launch_bounds__(256) void keep_jobs_kernel(Gs4dKeepJobs jobs, long long rows)
+{
+    int job_v = 0;
+    while (job_v + 1 < jobs.n && (int)blockIdx.y >= jobs.group0[job_v + 1]) job_v++;
+    const int job = __builtin_amdgcn_readfirstlane(job_v);
+    const Gs4dKeepJob& J = jobs.j[job];
+    const int g = blockIdx.y - jobs.group0[job], ng = jobs.group0[job + 1] - jobs.group0[job], sub = threadIdx.x & 15, col = g * 64 + 4 * sub;
+    const bool inside = col < J.width;
+    constexpr int U = 4;
+    const long long r0 = (long long)blockIdx.x * (16 * U) + (threadIdx.x >> 4);
+    if (WRITE) {
+        float4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = min(r0 + 16 * u, rows - 1);
+            v[u] = *reinterpret_cast<const float4*>(J.x + r * J.ld + (inside ? col : 0));
+            if (!inside) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = r0 + 16 * u;
+            float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            unsigned bits = 0, m = 0;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (J.relu) {
+                    bits |= (e[q] > 0.f ? 1u : 0u) << (4 * (sub & 7) + q);
+                    e[q] = e[q] < 0.f ? 0.f : e[q];
+                }
+                m = max(m, lb_abs_bits(e[q]));
+            }
+            m = group_max<16>(m);
+            unsigned w;
+            float s;
+            if (J.relu) {
+                const LbScale sc = lb_scale<GS4D_FMT_UINT8>(m);
+                w = lb_encode4<GS4D_FMT_UINT8>(e[0] * sc.inv, e[1] * sc.inv, e[2] * sc.inv, e[3] * sc.inv);
+                s = sc.s;
+#pragma unroll
+                for (int k = 1; k < 8; k <<= 1) bits |= (unsigned)__shfl_xor((int)bits, k, 64);
+            } else {
+                const LbScale sc = lb_scale<GS4D_FMT_INT8>(m);
+                w = lb_encode4<GS4D_FMT_INT8>(e[0] * sc.inv, e[1] * sc.inv, e[2] * sc.inv, e[3] * sc.inv);
+                s = sc.s;
+            }
+            if (r >= rows) continue;
+            *reinterpret_cast<unsigned*>(J.codes + (r * ng + g) * 64 + 4 * sub) = w;
+            if (sub == 0) J.scales[r * ng + g] = s;
+            if (J.relu && (sub & 7) == 0) J.bits[(r * ng + g) * 2 + (sub >> 3)] = bits;
+        }
+    } else {
+        unsigned w[U], bits[U];
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = min(r0 + 16 * u, rows - 1);
+            w[u] = *reinterpret_cast<const unsigned*>(J.codes + (r * ng + g) * 64 + 4 * sub);
+            s[u] = J.scales[r * ng + g];
+            bits[u] = J.relu ? J.bits[(r * ng + g) * 2 + (sub >> 3)] : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = r0 + 16 * u;
+            float4 v = J.relu ? lb_decode4<GS4D_FMT_UINT8>(w[u]) : lb_decode4<GS4D_FMT_INT8>(w[u]);
+            v = make_float4(s[u] * v.x, s[u] * v.y, s[u] * v.z, s[u] * v.w);
+            if (J.relu) {                                 // a positive number whose code is 0 stays positive: the sign is the mask
+                const unsigned b = bits[u] >> (4 * (sub & 7));
+                auto positive = [](unsigned bit, float x) { return !bit ? 0.f : x < 1.17549435e-38f ? 1.17549435e-38f : x; };
+                v = make_float4(positive(b & 1u, v.x), positive(b & 2u, v.y), positive(b & 4u, v.z), positive(b & 8u, v.w));
+            }
+            unsigned word = 0;
+            if (J.hmask) {                                // columns 8 m + 4 h + q: the nibbles of word h are the even or odd ones
+                const unsigned lo = (unsigned)__shfl((int)bits[u], (int)(threadIdx.x & 48), 64), hi = (unsigned)__shfl((int)bits[u], (int)(threadIdx.x & 48) + 8, 64);
+                const int h = sub & 1;
+#pragma unroll
+                for (int m = 0; m < 4; m++)
+                    word |= ((lo >> (8 * m + 4 * h)) & 15u) << (4 * m) | ((hi >> (8 * m + 4 * h)) & 15u) << (16 + 4 * m);
+            }
+            if (r >= rows) continue;
+            if (inside) *reinterpret_cast<float4*>(J.x + r * J.ld + col) = v;
+            if (J.hmask && sub < 2) J.hmask[r * J.hld + J.hword + 2 * g + sub] = word;
+        }
+    }
+}
+
 // ------------------------------------------------------------------ linear
 // What the backward keeps of the input, in one block: codes [N][kp] | scales [N][kp / 64] | sign bits [N][kp / 64][2 words]
 // (x > 0), kp = K rounded up to 64.  Column c of a group is bit c & 31 of word c >> 5 for float32 and bit c >> 1 of word c & 1
@@ -1168,3 +1256,12 @@ int gs4d_linear8_backward(int dtype, long long N, int K, int M, const void* dy, 
 }
 
 }  // extern "C"
+
+int gs4d_launch_keep(const Gs4dKeepJobs& jobs, long long rows, bool write, hipStream_t s)
+{
+    const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)jobs.group0[jobs.n]);
+    if (write) hipLaunchKernelGGL(keep_jobs_kernel<true>, grid, dim3(256), 0, s, jobs, rows);
+    else hipLaunchKernelGGL(keep_jobs_kernel<false>, grid, dim3(256), 0, s, jobs, rows);
+    GS4D_LAUNCH_CHECK("keep_jobs", 0, s);
+    return GS4D_OK;
+}

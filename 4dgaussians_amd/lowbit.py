@@ -205,7 +205,7 @@ def frame_features(cache, planes, aabb, points, t):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, relu, fmt):
+    def forward(ctx, x, weight, bias, relu, fmt, grad):
         L = _cabi.lib()
         dev, dt = x.device, DTYPES[x.dtype]
         M, K = weight.shape
@@ -214,7 +214,8 @@ class _Linear(torch.autograd.Function):
         if N and ((K > 1 and rows.stride(1) != 1) or (N > 1 and rows.stride(0) < K)):
             rows = rows.contiguous()
         w, b = weight.detach().contiguous(), None if bias is None else bias.detach().contiguous()
-        what = (KEEP_CODES if ctx.needs_input_grad[1] else 0) | (KEEP_SIGNS if relu and ctx.needs_input_grad[0] else 0)
+        # needs_input_grad says what requires a gradient, grad whether one is recorded at all
+        what = (KEEP_CODES if ctx.needs_input_grad[1] else 0) | (KEEP_SIGNS if relu and ctx.needs_input_grad[0] else 0) if grad else 0
         y = torch.empty(N, M, dtype=x.dtype, device=dev)
         keep = torch.empty(int(L.gs4d_linear8_keep_bytes(C.c_longlong(N), C.c_int(K), C.c_int(what))) if what else 0,
                            dtype=torch.uint8, device=dev)
@@ -246,7 +247,7 @@ class _Linear(torch.autograd.Function):
                                          C.c_int(relu), C.c_int(fmt), _cabi.ptr(keep), C.c_int(what), _cabi.ptr(dx), _cabi.ptr(dw),
                                          _cabi.ptr(db), _cabi.ptr(scratch), _cabi.current_stream(dev))
         _cabi.check(rc, "gs4d_linear8_backward")
-        return None if dx is None else dx.view(x_shape), dw, None if db is None else db.view(b_shape), None, None
+        return None if dx is None else dx.view(x_shape), dw, None if db is None else db.view(b_shape), None, None, None
 
 
 def linear(x, weight, bias=None, relu=False, fmt="int8"):
@@ -266,4 +267,4 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
         _on_device("bias", bias, x.device)
         if bias.dtype != x.dtype or tuple(bias.shape) != (weight.shape[0],):
             raise RuntimeError(f"linear: bias must be {x.dtype} [{weight.shape[0]}], got {bias.dtype} {tuple(bias.shape)}")
-    return _Linear.apply(x, weight, bias, bool(relu), f)
+    return _Linear.apply(x, weight, bias, bool(relu), f, torch.is_grad_enabled())

@@ -55,9 +55,11 @@ class RenderCall:
     """Everything of one render() call that is not a differentiable tensor: the camera, the per-point time / force
     columns, the optional L1 target and the data-parallel hooks."""
     __slots__ = ("H", "W", "tanfovx", "tanfovy", "bg", "view", "proj", "campos", "scale_modifier", "sh_degree", "debug",
-                 "time", "force", "target", "deform_net", "shs_grad_hook", "params", "cfg")
+                 "time", "force", "target", "deform_net", "shs_grad_hook", "params", "cfg", "uniform_time", "grad")
 
     def __init__(self, cam, bg, scale_modifier, sh_degree, debug, deform_net, time, force, target, shs_grad_hook):
+        self.grad = torch.is_grad_enabled()          # the autograd function's forward cannot see it
+        self.uniform_time = bool(getattr(type(cam), "uniform_columns", False))       # one time and force for all rows
         self.H, self.W = int(cam.image_height), int(cam.image_width)
         self.tanfovx, self.tanfovy = math.tan(cam.FoVx * 0.5), math.tan(cam.FoVy * 0.5)
         self.bg, self.view, self.proj, self.campos = bg, cam.world_view_transform, cam.full_proj_transform, cam.camera_center
@@ -74,6 +76,8 @@ class RenderCall:
             return False
         if self.deform_net is not None:
             plan = self.cfg["plan"]
+            if self.cfg["activation_bits"] == 8 and torch.is_grad_enabled():
+                return False                       # the staged path keeps the field's activations in 8 bits
             if not plan.in_place or not (_usable(self.time) and _usable(self.force)):
                 return False
         return True
@@ -108,6 +112,7 @@ def _issue_forward(call: RenderCall, xyz, scaling, rotation, opacity, features, 
     d = RenderDesc()
     if call.deform_net is not None:
         call.cfg["plan"].desc.no_grad = 0 if needs_grad else 1
+        call.cfg["plan"].desc.uniform_time = int(call.uniform_time)
     _fill_desc(d, call, P, M, xyz, scaling, rotation, opacity, features, flags)
     d.l1_grad_scale = l1_grad_scale.data_ptr() if (l1_grad_scale is not None and call.target is not None) else None
     d.visible = visible.data_ptr() if visible is not None else None      # bool [P]: radii > 0, written by the preprocess launch
@@ -142,6 +147,7 @@ class _BackwardBuffers:
         g.d_opacity_logit, g.d_shs = self.d_op.data_ptr(), self.d_shs.data_ptr()
         self.dg, self.views, self.order_key = None, (), None
         if call.deform_net is not None:
+            call.deform_net.thaw_planes()      # a training step: planes frozen for rendering would be stale after it
             plan, cfg = call.cfg["plan"], call.cfg
             self.dg, self.views = plan.new_grads(dev)
             oc = cfg.get("hex_order_cache")
@@ -197,7 +203,7 @@ class _RenderFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, call, xyz, scaling, rotation, opacity, features, means2D, *params):
-        needs_grad = any(ctx.needs_input_grad)
+        needs_grad = call.grad and any(ctx.needs_input_grad)
         color, radii, depth, loss, d, state, arena = _issue_forward(call, xyz, scaling, rotation, opacity, features, needs_grad)
         ctx.num_rendered = state.num_rendered
         if needs_grad:

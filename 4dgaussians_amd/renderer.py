@@ -37,6 +37,8 @@ class GaussianParams(nn.Module):
 
 
 class Camera:
+    uniform_columns = True                       # time_force_columns() holds one time and one force in all rows
+
     def __init__(self, cam, device, time: float = 0.0, force: float = 0.0):
         self.image_width, self.image_height = cam.image_width, cam.image_height
         self.FoVx, self.FoVy = cam.FoVx, cam.FoVy

@@ -19,6 +19,7 @@ import torch.nn as nn
 import torch.nn.init as init
 
 from .. import _cabi
+from ..lowbit import FORMATS, RowCache
 from .hexplane import HexPlaneField
 
 MAX_LEVELS, MAX_TRUNK = 4, 8
@@ -33,7 +34,9 @@ class DeformDesc(C.Structure):
                 ("planes", FP * (MAX_LEVELS * 6)), ("plane_w", C.c_int * (MAX_LEVELS * 6)),
                 ("plane_h", C.c_int * (MAX_LEVELS * 6)), ("aabb", FP), ("ft_w", FP), ("ft_b", FP),
                 ("trunk_w", FP * MAX_TRUNK), ("trunk_b", FP * MAX_TRUNK), ("head_w1", FP * 4), ("head_b1", FP * 4),
-                ("head_w2", FP * 4), ("head_b2", FP * 4), ("no_grad", C.c_int)]
+                ("head_w2", FP * 4), ("head_b2", FP * 4), ("no_grad", C.c_int), ("static_codes", FP), ("static_scales", FP),
+                ("static_rows", C.c_int), ("static_pitch", C.c_int), ("static_group", C.c_int), ("static_fmt", C.c_int),
+                ("uniform_time", C.c_int), ("reserved_", C.c_int)]
 
 
 class DeformGrads(C.Structure):
@@ -94,7 +97,17 @@ def _lib():
     L = _cabi.lib()
     L.gs4d_deform_workspace_bytes.restype = C.c_size_t
     L.gs4d_deform_backward_scratch_bytes.restype = C.c_size_t
+    L.gs4d_deform_checkpoint_bytes.restype = C.c_size_t
     return L
+
+
+# activation_bits = 8: rows per forward / backward call of the library, i.e. how many rows ever have float32 activations
+CHECKPOINT_ROWS = 1 << 18
+
+
+def _one_value(t):
+    """A column whose rows are one number by construction (a broadcast view)."""
+    return t.shape[0] <= 1 or t.stride(0) == 0
 
 
 def init_zero_(model):
@@ -192,6 +205,17 @@ class _DeformFunction(torch.autograd.Function):
         return planes, aabb, ft_w, ft_b, trunk, heads
 
     @staticmethod
+    def _checkpoint_bytes(L, d, n):
+        return (int(L.gs4d_deform_checkpoint_bytes(C.byref(d), C.c_int(n))) + 255) // 256 * 256
+
+    @staticmethod
+    def _chunks(L, d, P):
+        """[(first row, rows, offset of their checkpoint)] with at most CHECKPOINT_ROWS rows each."""
+        n = min(P, CHECKPOINT_ROWS)
+        step = _DeformFunction._checkpoint_bytes(L, d, n)
+        return [(r0, min(n, P - r0), i * step) for i, r0 in enumerate(range(0, max(P, 1), max(n, 1)))]
+
+    @staticmethod
     def forward(ctx, points, scales, rotations, shs, time, force, cfg, *params):
         L = _lib()
         dev = points.device
@@ -212,17 +236,31 @@ class _DeformFunction(torch.autograd.Function):
             plan = None
             planes, aabb, ft_w, ft_b, trunk, heads = _DeformFunction._split(cfg, [p.detach() for p in params])
             d = _DeformFunction._desc(cfg, planes, aabb, ft_w, ft_b, trunk, heads)
-        d.no_grad = 0 if any(ctx.needs_input_grad) else 1      # under torch.no_grad() nothing will read the activations
+        # under torch.no_grad() nothing will read the activations (needs_input_grad says only what requires a gradient)
+        d.no_grad = 0 if cfg["grad"] and any(ctx.needs_input_grad) else 1
+        d.uniform_time = int(_one_value(time) and _one_value(force))
+        kept8 = cfg.get("activation_bits") == 8 and not d.no_grad
         o_xyz, o_sc, o_rot, o_shs = (torch.empty_like(t) for t in (points_, scales_, rot_, shs_))
-        ws = torch.empty(max(int(L.gs4d_deform_workspace_bytes(C.byref(d), C.c_int(P))), 256), dtype=torch.uint8, device=dev)
+        chunks = _DeformFunction._chunks(L, d, P) if kept8 else [(0, P, 0)]
+        ws = torch.empty(max(int(L.gs4d_deform_workspace_bytes(C.byref(d), C.c_int(chunks[0][1]))), 256), dtype=torch.uint8, device=dev)
+        kept = torch.empty(chunks[-1][2] + _DeformFunction._checkpoint_bytes(L, d, chunks[-1][1]), dtype=torch.uint8, device=dev) if kept8 else None
+        row = lambda t, r0: C.c_void_p(t.data_ptr() + 4 * t[0:1].numel() * r0) if P else C.c_void_p(0)
         with torch.cuda.device(dev):
-            rc = L.gs4d_deform_forward(C.byref(d), C.c_int(P), _cabi.ptr(points_), _cabi.ptr(scales_), _cabi.ptr(rot_),
-                                       _cabi.ptr(shs_), _cabi.ptr(time_), _cabi.ptr(force_), _cabi.ptr(o_xyz),
-                                       _cabi.ptr(o_sc), _cabi.ptr(o_rot), _cabi.ptr(o_shs), _cabi.ptr(ws),
-                                       _cabi.current_stream(dev))
-        _cabi.check(rc, "gs4d_deform_forward")
+            for r0, n, off in chunks:
+                rc = L.gs4d_deform_forward(C.byref(d), C.c_int(n), row(points_, r0), row(scales_, r0), row(rot_, r0),
+                                           row(shs_, r0), row(time_, r0), row(force_, r0), row(o_xyz, r0),
+                                           row(o_sc, r0), row(o_rot, r0), row(o_shs, r0), _cabi.ptr(ws),
+                                           _cabi.current_stream(dev))
+                _cabi.check(rc, "gs4d_deform_forward")
+                if kept8:                          # the float32 activations of these rows end here
+                    rc = L.gs4d_deform_checkpoint_pack(C.byref(d), C.c_int(n), _cabi.ptr(ws), C.c_void_p(kept.data_ptr() + off),
+                                                       _cabi.current_stream(dev))
+                    _cabi.check(rc, "gs4d_deform_checkpoint_pack")
+        if kept8:
+            ws = kept
         ctx.cfg = cfg
         ctx.plan = plan
+        ctx.kept8 = kept8
         if plan is not None:
             # the parameters are not re-read through saved_tensors (50 unpacks per step); their versions are kept
             # instead, so that an in-place update between forward and backward is still refused
@@ -277,33 +315,48 @@ class _DeformFunction(torch.autograd.Function):
             g_shs = g_shs.clone()
         d_xyz, d_sc, d_rot = (torch.empty_like(t) for t in (points_, scales_, rot_))
         d_shs = g_shs            # shs' = shs + delta: the input gradient IS the upstream gradient (the C ABI allows the alias)
-        scratch = torch.empty(max(int(L.gs4d_deform_backward_scratch_bytes(C.byref(d), C.c_int(P))), 256),
+        chunks = _DeformFunction._chunks(L, d, P) if ctx.kept8 else [(0, P, 0)]
+        most = chunks[0][1]
+        scratch = torch.empty(max(int(L.gs4d_deform_backward_scratch_bytes(C.byref(d), C.c_int(most))), 256),
                               dtype=torch.uint8, device=dev)
+        kept = None
+        if ctx.kept8:                              # ws is the 8-bit checkpoint: a float32 workspace for one chunk at a time
+            kept, ws = ws, torch.empty(max(int(L.gs4d_deform_workspace_bytes(C.byref(d), C.c_int(most))), 256), dtype=torch.uint8, device=dev)
+            d.no_grad = 0                          # a later forward without a backward may have set it
         hook = cfg.get("data_grad_hook")
         order_cache = cfg.get("hex_order_cache")
         order_key = None
-        if order_cache is not None:
+        if order_cache is not None and len(chunks) == 1:
             order_key = order_cache.bind(g, P, int(d.L), dev)
-        else:
+        else:                                      # the cached order is one of all rows
             g.hex_order, g.hex_order_valid = None, 0
+        row = lambda t, r0: C.c_void_p(t.data_ptr() + 4 * t[0:1].numel() * r0) if P else C.c_void_p(0)
 
-        def run(phases):
+        def run(phases, chunks=chunks):
             with torch.cuda.device(dev):
-                rc = L.gs4d_deform_backward_phases(
-                    C.byref(d), C.byref(g), C.c_int(P), _cabi.ptr(points_), _cabi.ptr(scales_), _cabi.ptr(rot_),
-                    _cabi.ptr(time_), _cabi.ptr(force_), _cabi.ptr(g_xyz), _cabi.ptr(g_sc), _cabi.ptr(g_rot),
-                    _cabi.ptr(g_shs), _cabi.ptr(d_xyz), _cabi.ptr(d_sc), _cabi.ptr(d_rot), _cabi.ptr(d_shs), _cabi.ptr(ws),
-                    _cabi.ptr(scratch), _cabi.current_stream(dev), C.c_int(phases))
-            _cabi.check(rc, "gs4d_deform_backward_phases")
+                for r0, n, off in chunks:
+                    if kept is not None and phases & BWD_DATA:
+                        rc = L.gs4d_deform_checkpoint_unpack(
+                            C.byref(d), C.c_int(n), row(points_, r0), row(scales_, r0), row(rot_, r0), row(time_, r0),
+                            row(force_, r0), C.c_void_p(kept.data_ptr() + off), _cabi.ptr(ws), _cabi.current_stream(dev))
+                        _cabi.check(rc, "gs4d_deform_checkpoint_unpack")
+                    rc = L.gs4d_deform_backward_phases(
+                        C.byref(d), C.byref(g), C.c_int(n), row(points_, r0), row(scales_, r0), row(rot_, r0),
+                        row(time_, r0), row(force_, r0), row(g_xyz, r0), row(g_sc, r0), row(g_rot, r0),
+                        row(g_shs, r0), row(d_xyz, r0), row(d_sc, r0), row(d_rot, r0), row(d_shs, r0), _cabi.ptr(ws),
+                        _cabi.ptr(scratch), _cabi.current_stream(dev), C.c_int(phases))
+                    _cabi.check(rc, "gs4d_deform_backward_phases")
 
         if hook is None:
             run(BWD_DATA | BWD_WEIGHTS)
         else:
             # data-parallel overlap: everything but the Linear weight gradients is final after the data phase and can
             # start its all-reduce while the weight-gradient products run (parallel.GradBucket.early_reduce_many)
-            run(BWD_DATA)
+            # (several chunks: each chunk's two phases share its workspace, the hook follows the last data phase)
+            run(BWD_DATA | BWD_WEIGHTS, chunks[:-1])
+            run(BWD_DATA, chunks[-1:])
             hook(d_xyz, d_sc, d_rot, gp, g_ftw, g_ftb)
-            run(BWD_WEIGHTS)
+            run(BWD_WEIGHTS, chunks[-1:])
         if order_cache is not None:
             order_cache.recorded(order_key)
         param_grads = list(gp) + [None, g_ftw, g_ftb] + list(gt) + list(gh)
@@ -325,6 +378,9 @@ class Deformation(nn.Module):
         self.extra_opacity_dim = args.opacity_pe * 2 * 3
         self.prev_frames = args.prev_frames
         self.prev_frames_out_dim = 16
+        # 32: the backward reads the forward's float32 activations; 8: they are kept in 8 bits (gs4d_deform_checkpoint_pack),
+        # a fifth of the memory per row, and only CHECKPOINT_ROWS rows at a time have float32 ones
+        self.activation_bits = int(getattr(args, "activation_bits", 32))
         # optional callable(d_points, d_scales, d_rotations, plane_grads, ft_w_grad, ft_b_grad), called from the
         # backward as soon as those gradients are final (before the weight gradients are computed); see parallel.py
         self.data_grad_hook = None
@@ -337,6 +393,7 @@ class Deformation(nn.Module):
     def set_aabb(self, xyz_max, xyz_min):
         self.grid.set_aabb(xyz_max, xyz_min)      # replaces grid.aabb by a new Parameter: the cached plan is stale
         self._step_cache = None
+        self.thaw_planes()
         self.__dict__.pop("_hex_order_cache", None)   # other bounds, other cells: the cached point order is void
 
     def create_net(self):
@@ -379,6 +436,8 @@ class Deformation(nn.Module):
         if not a.no_do:
             raise NotImplementedError("no_do=False feeds opacity_deform the wrong input width in the reference "
                                       "(scene/deformation.py:101 vs :190) and cannot run there either")
+        if self.activation_bits not in (8, 32):
+            raise NotImplementedError(f"activation_bits must be 8 or 32, got {self.activation_bits}")
         if self.W != 64 or self.grid_pe != 0:
             raise NotImplementedError("net_width must be 64 and grid_pe 0")
         kc = a.kplanes_config
@@ -387,12 +446,12 @@ class Deformation(nn.Module):
                     force_pe=int(self.force_pe), no_dx=int(bool(a.no_dx)), no_ds=int(bool(a.no_ds)),
                     no_dr=int(bool(a.no_dr)), no_dshs=int(bool(a.no_dshs)), apply_rotation=int(bool(a.apply_rotation)),
                     use_time=int(bool(a.use_time)), use_force=int(bool(a.use_force)),
-                    data_grad_hook=self.data_grad_hook)
+                    data_grad_hook=self.data_grad_hook, activation_bits=self.activation_bits)
 
     def _flags(self):
         a = self.args
         return (bool(a.no_dx), bool(a.no_ds), bool(a.no_dr), bool(a.no_dshs), bool(a.apply_rotation), bool(a.use_time),
-                bool(a.use_force), bool(a.no_do), self.blend_time_force)
+                bool(a.use_force), bool(a.no_do), self.blend_time_force, self.activation_bits)
 
     def _params(self):
         planes = [p for level in self.grid.grids for p in level]
@@ -409,10 +468,12 @@ class Deformation(nn.Module):
         state = dict(super().__getstate__()) if hasattr(super(), "__getstate__") else dict(self.__dict__)
         state.pop("_step_cache", None)
         state.pop("_hex_order_cache", None)
+        state.pop("_frozen", None)
         return state
 
     def _apply(self, fn, *a, **k):                 # .to() / .cuda() / .float(): parameters may get new storage
         self._step_cache = None
+        self.thaw_planes()
         self.__dict__.pop("_hex_order_cache", None)
         return super()._apply(fn, *a, **k)
 
@@ -435,12 +496,62 @@ class Deformation(nn.Module):
         if oc is None:
             oc = self.__dict__["_hex_order_cache"] = HexOrderCache()
         cfg["hex_order_cache"] = oc
+        if torch.is_grad_enabled():
+            self.thaw_planes()                     # the planes are about to be trained
+        frozen, d = self.__dict__.get("_frozen"), cfg["plan"].desc
+        if frozen is not None and frozen[1] != [p._version for p in params[:cfg["plan"].n_planes]]:
+            raise RuntimeError("the planes were modified after freeze_planes(): freeze them again or call thaw_planes()")
+        if frozen is not None:
+            c = frozen[0]
+            d.static_codes, d.static_scales = c.codes.data_ptr(), c.scales.data_ptr()
+            d.static_rows, d.static_pitch, d.static_group, d.static_fmt = c.capacity, c.codes.shape[1], c.group, FORMATS[c.fmt]
+        else:
+            d.static_codes = None
         return params, cfg
+
+    @torch.no_grad()
+    def freeze_planes(self, points, fmt="int8", group=64):
+        """For rendering many frames of one model: keeps, in 8 bits, the product of every level's three spatial planes at
+        points [P, 3] (which no frame changes), so that a query without gradients samples three planes a level instead of six.
+        Queries are then of these points (P rows, or several copies of them as render_batch makes) until thaw_planes() or the
+        first query with gradients enabled; a change of bounds or device thaws as well.  The features are off by at most half
+        a step of the format (int8: 1 / 254 of the largest of 64 neighbouring ones)."""
+        self.thaw_planes()
+        if not isinstance(points, torch.Tensor) or points.dim() != 2 or points.shape[1] != 3 or points.shape[0] < 1 or points.dtype != torch.float32:
+            raise RuntimeError("freeze_planes: points must be float32 [P, 3] with at least one row")
+        if points.device.type != "cuda":
+            raise RuntimeError("freeze_planes: points must be on a HIP device; there is no CPU path")
+        L = _lib()
+        dev, P = points.device, points.shape[0]
+        params, cfg = self.cached_plan()
+        plan = cfg["plan"]
+        if not plan.in_place:
+            raise RuntimeError("freeze_planes: the field's parameters must be float32 and dense (planes channels-last)")
+        if params[0].device != dev:
+            raise RuntimeError(f"freeze_planes: points are on {dev}, the planes on {params[0].device}")
+        width = cfg["L"] * cfg["C"]
+        cache = RowCache(P, width, fmt, group, device=dev)
+        points = points.detach().contiguous()
+        rows = torch.empty(min(P, CHECKPOINT_ROWS), width, dtype=torch.float32, device=dev)
+        for r0 in range(0, P, CHECKPOINT_ROWS):
+            n = min(CHECKPOINT_ROWS, P - r0)
+            with torch.cuda.device(dev):
+                rc = L.gs4d_static_features(C.byref(plan.desc), C.c_int(n), C.c_void_p(points.data_ptr() + 12 * r0),
+                                            C.c_void_p(rows.data_ptr()), _cabi.current_stream(dev))
+            _cabi.check(rc, "gs4d_static_features")
+            cache.write(rows[:n], start=r0)
+        self.__dict__["_frozen"] = (cache, [p._version for p in params[:plan.n_planes]])
+        return cache
+
+    def thaw_planes(self):
+        """Queries sample all six planes again."""
+        self.__dict__.pop("_frozen", None)
 
     def forward_dynamic(self, points, scales, rotations, opacity, shs, time, force, prev_frames=None):
         if prev_frames is not None:
             raise NotImplementedError("prev_frames conditioning is outside the hot path (SURVEY.md section 8)")
         params, cfg = self.cached_plan()
+        cfg["grad"] = torch.is_grad_enabled()
         out = _DeformFunction.apply(points, scales, rotations, shs, time, force, cfg, *params)
         # opacity passes through (no_do): the reference's opacity[:, :1] is the tensor itself when it is (P, 1)
         return out[0], out[1], out[2], opacity if opacity.shape[1] == 1 else opacity[:, :1], out[3]
@@ -491,6 +602,12 @@ class deform_network(nn.Module):
 
     def forward(self, *args):
         return self.forward_dynamic(*args)
+
+    def freeze_planes(self, points, fmt="int8", group=64):
+        return self.deformation_net.freeze_planes(points, fmt, group)
+
+    def thaw_planes(self):
+        self.deformation_net.thaw_planes()
 
     def get_mlp_parameters(self):
         return self.deformation_net.get_mlp_parameters()

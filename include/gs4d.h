@@ -284,6 +284,15 @@ typedef struct gs4d_deform_desc {
     const float* head_b2[4];
     int no_grad;              /* 1: no backward will follow (render_for_image): the forward skips the activations only the
                                  backward reads (the workspace then cannot be passed to gs4d_deform_backward) */
+    /* Rendering with frozen planes (ABI 14; no counterpart in the reference; static_codes NULL: off).  With no_grad, row p of a
+     * call takes the product of the three spatial planes of every level from row p % static_rows of this cache of 8-bit rows
+     * (gs4d_rows8: L * C values; filled from gs4d_static_features) instead of sampling them; P must be a multiple of static_rows
+     * and the caller answers for the points and planes being those of the cache.  Without no_grad the planes are sampled. */
+    const unsigned char* static_codes;
+    const float* static_scales;
+    int static_rows, static_pitch, static_group, static_fmt;
+    int uniform_time;         /* 1: time and force hold one value each in all rows (ABI 14; a hint that rendering uses) */
+    int reserved_;
 } gs4d_deform_desc;
 
 /* Gradient destinations, same shapes as the parameters above; every one must be zero-initialised
@@ -326,6 +335,21 @@ int gs4d_deform_forward(const gs4d_deform_desc* d, int P,
                         const float* time, const float* force,
                         float* out_means3D, float* out_scales, float* out_rotations, float* out_shs,
                         char* workspace, void* stream);
+
+/* The product of each level's three spatial planes at points [P,3] -> out [P][L * C] (16-byte aligned): what the frozen-plane
+ * cache of gs4d_deform_desc holds. */
+int gs4d_static_features(const gs4d_deform_desc* d, int P, const float* points, float* out, void* stream);
+
+/* What the backward needs of a forward's workspace, in 8 bits (no counterpart in the reference): the inputs of every Linear in
+ * groups of 64 columns with one scale each (the definition of gs4d_rows8; rectified ones with 255 levels), the signs of the
+ * rectified ones as bits, the rotation head's output.  pack: workspace of a gs4d_deform_forward of these P rows -> checkpoint
+ * (gs4d_deform_checkpoint_bytes, 256-byte aligned), after which the workspace may be used for other rows; unpack: checkpoint and
+ * the forward's inputs -> a workspace for gs4d_deform_backward.  Input and plane gradients do not change by a bit (signs are
+ * exact, the encodings are computed again); weight gradients are taken with the kept values. */
+size_t gs4d_deform_checkpoint_bytes(const gs4d_deform_desc* d, int P);
+int gs4d_deform_checkpoint_pack(const gs4d_deform_desc* d, int P, char* workspace, char* checkpoint, void* stream);
+int gs4d_deform_checkpoint_unpack(const gs4d_deform_desc* d, int P, const float* points, const float* scales, const float* rotations,
+                                  const float* time, const float* force, char* checkpoint, char* workspace, void* stream);
 
 /* dL_d(out_*) -> dL_d(points, scales, rotations, shs) (written, not accumulated) and parameter
  * gradients accumulated into `g`.  scratch: gs4d_deform_backward_scratch_bytes().

@@ -339,6 +339,21 @@ def test_linear_shapes_strides_and_partial_gradients():
         assert torch.equal(g, full[i])
 
 
+def test_linear_keeps_nothing_without_gradients():
+    x, w, b, _ = make(4096, 256, 64, torch.float32)
+    xs, ws, bs = leaf(x), leaf(w), leaf(b)
+    sizes = []
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            y = lb().linear(xs, ws, bs, relu=True)
+            sizes.append(torch.cuda.memory_allocated() - before - y.numel() * 4)
+            del y
+    # 256 codes, 4 scales and 32 bytes of signs a row (the allocator may add up to 1 MiB to a block), not 1024 bytes
+    assert sizes[0] < 4096 and 4096 * 304 <= sizes[1] <= 4096 * 305 + (1 << 20), sizes
+
+
 def test_linear_without_rows():
     xs, ws, bs = leaf(torch.zeros(0, 8)), leaf(torch.zeros(5, 8)), leaf(torch.zeros(5))
     y = lb().linear(xs, ws, bs, relu=True)
