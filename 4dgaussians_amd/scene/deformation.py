@@ -61,12 +61,14 @@ class HexOrderCache:
     def clear(self):
         self.entries.clear()
 
-    def bind(self, g, P, L, dev):
-        """Points `g` at the order buffer for (P, L, dev) and says whether it holds a usable order."""
+    def bind(self, g, P, L, dev, rows=None):
+        """Points `g` at the order buffer for (P, L, dev) and says whether it holds a usable order.  rows: the backward runs
+        in calls of that many rows (the last one shorter), each with an order of its own, L * 3 * rows entries apart."""
+        rows = P if rows is None else min(rows, P)
         if self.refresh <= 0 or P == 0:
             g.hex_order, g.hex_order_valid = None, 0
             return
-        key = (P, L, dev.index)
+        key = (P, L, dev.index, rows)
         e = self.entries.get(key)
         if e is None:
             if len(self.entries) >= 4:
@@ -74,7 +76,8 @@ class HexOrderCache:
             # starts as the identity order of every (level, sort plane): should the recording backward fail half way
             # (an exception between its phases), what a later pass walks is still a permutation of the points -- the
             # order decides only how well adds are combined, a non-permutation would drop or double gradients
-            e = self.entries[key] = [torch.arange(P, dtype=torch.int32, device=dev).repeat(L * 3), self.refresh]
+            parts = [torch.arange(min(rows, P - r0), dtype=torch.int32, device=dev).repeat(L * 3) for r0 in range(0, P, rows)]
+            e = self.entries[key] = [parts[0] if len(parts) == 1 else torch.cat(parts), self.refresh]
         valid = e[1] < self.refresh
         if valid:
             e[1] += 1
@@ -326,10 +329,11 @@ class _DeformFunction(torch.autograd.Function):
         hook = cfg.get("data_grad_hook")
         order_cache = cfg.get("hex_order_cache")
         order_key = None
-        if order_cache is not None and len(chunks) == 1:
-            order_key = order_cache.bind(g, P, int(d.L), dev)
-        else:                                      # the cached order is one of all rows
+        if order_cache is not None:
+            order_key = order_cache.bind(g, P, int(d.L), dev, most)
+        else:
             g.hex_order, g.hex_order_valid = None, 0
+        order0 = g.hex_order
         row = lambda t, r0: C.c_void_p(t.data_ptr() + 4 * t[0:1].numel() * r0) if P else C.c_void_p(0)
 
         def run(phases, chunks=chunks):
@@ -340,6 +344,8 @@ class _DeformFunction(torch.autograd.Function):
                             C.byref(d), C.c_int(n), row(points_, r0), row(scales_, r0), row(rot_, r0), row(time_, r0),
                             row(force_, r0), C.c_void_p(kept.data_ptr() + off), _cabi.ptr(ws), _cabi.current_stream(dev))
                         _cabi.check(rc, "gs4d_deform_checkpoint_unpack")
+                    if order0:                     # each chunk's own order
+                        g.hex_order = order0 + 4 * r0 * int(d.L) * 3
                     rc = L.gs4d_deform_backward_phases(
                         C.byref(d), C.byref(g), C.c_int(n), row(points_, r0), row(scales_, r0), row(rot_, r0),
                         row(time_, r0), row(force_, r0), row(g_xyz, r0), row(g_sc, r0), row(g_rot, r0),
