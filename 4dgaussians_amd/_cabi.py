@@ -37,8 +37,11 @@ def lib() -> C.CDLL:
         L = C.CDLL(LIB_PATH)
         L.gs4d_last_error.restype = C.c_char_p
         for name in ("gs4d_geometry_bytes", "gs4d_binning_bytes", "gs4d_image_bytes", "gs4d_backward_scratch_bytes",
-                     "gs4d_l1_loss_scratch_bytes", "gs4d_linear8_keep_bytes", "gs4d_linear8_scratch_bytes"):
+                     "gs4d_l1_loss_scratch_bytes"):
             getattr(L, name).restype = C.c_size_t
+        for name, (res, args) in _PROTOTYPES.items():
+            f = getattr(L, name)
+            f.restype, f.argtypes = res, args
         L.gs4d_thread_state_release.restype = None
         L.gs4d_mailbox_stats.restype = None
         L.gs4d_forward_stats.restype = None
@@ -98,6 +101,46 @@ def ptr(t):
 
 def current_stream(device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# For operators whose kernels take a few microseconds, where the host is what counts: functions with declared argument types
+# take plain numbers and addresses (None: NULL), without a ctypes object per argument.
+_LL, _I, _P, _Z = C.c_longlong, C.c_int, C.c_void_p, C.c_size_t
+_PROTOTYPES = {
+    "gs4d_rows8_write": (_I, (_P, _P, _I, _LL, _LL, _P, _I, _LL, _P)),
+    "gs4d_rows8_read": (_I, (_P, _P, _I, _LL, _LL, _P, _I, _LL, _P)),
+    "gs4d_linear8_keep_bytes": (_Z, (_LL, _I, _I)),
+    "gs4d_linear8_scratch_bytes": (_Z, (_LL, _I, _I)),
+    "gs4d_linear8_forward": (_I, (_I, _LL, _I, _I, _P, _LL, _P, _P, _I, _I, _P, _P, _I, _P)),
+    "gs4d_linear8_backward": (_I, (_I, _LL, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P)),
+    "gs4d_frame_features": (_I, (_P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _LL, _P, _LL, _P)),
+}
+
+
+def address(t):
+    """ptr() as a plain number, for functions with declared argument types."""
+    return t.data_ptr() if t is not None else None
+
+
+def stream_of(device):
+    """current_stream() as a plain number."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_GUARD = _Here()
+
+
+def on_device(device):
+    """torch.cuda.device(device) where it is not the current one already."""
+    return _HERE_GUARD if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _live_allocators = {}          # key -> TensorAllocator, only while its C call is in flight

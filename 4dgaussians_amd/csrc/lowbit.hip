@@ -18,47 +18,37 @@ template <typename T> __device__ __forceinline__ float high16(unsigned w)
 
 // ------------------------------------------------------------------ row cache
 // Both directions move 16 bytes of the caller's rows per lane and step (COLS = 4 float32 or 8 16-bit numbers, neighbouring lanes
-// neighbouring addresses; VEC: rows are 16-byte aligned) and their codes as one word or two.  A workgroup owns rpb rows, i.e.
-// about ROWS8_ITEMS (row, columns) items; item e of it is row e / cpr by a multiply-high (exact: e * cpr < 2^32).
+// neighbouring addresses, at any alignment: gfx950 loads and stores 16 bytes from any address) and their codes as one word or two.
+// FULL: width is a multiple of COLS, so that no lane has a shorter share (1 M x 256 float32 read back: 217 us, without 327).
+// A workgroup owns rpb rows, i.e. about ROWS8_ITEMS (row, columns) items; item e of it is row e / cpr by a multiply-high (exact:
+// e * cpr < 2^32).
 #define ROWS8_ITEMS 2048
 #define ROWS8_ROWS 256
 
-// the maximum over the LANES neighbouring lanes of a group: four steps within 16 lanes, then across
-template <int LANES> __device__ __forceinline__ unsigned group_max(unsigned m)
+// the maximum over the 2^shift neighbouring lanes of a group (uniform): four steps within 16 lanes, then across
+__device__ __forceinline__ unsigned group_max(unsigned m, int shift)
 {
-    if constexpr (LANES > 1) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));    // lane ^ 1
-    if constexpr (LANES > 2) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));    // lane ^ 2
-    if constexpr (LANES > 4) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true));   // mirrored in 8
-    if constexpr (LANES > 8) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, true));   // mirrored in 16
-    if constexpr (LANES > 16) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
+    if (shift > 0) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));    // lane ^ 1
+    if (shift > 1) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));    // lane ^ 2
+    if (shift > 2) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true));   // mirrored in 8
+    if (shift > 3) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, true));   // mirrored in 16
+    if (shift > 4) m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
     return m;
 }
 
-// COLS consecutive numbers of a row from column col on; columns past width are zero
-template <typename T, int COLS, bool VEC>
-__device__ __forceinline__ void load_cols(float (&v)[COLS], const T* __restrict__ x, int col, int width)
+// where lanes read that must not read past the end of a caller's array
+__device__ const uint4 kZeroPage[2] = {};
+
+template <typename T> __device__ __forceinline__ uint4 load16(const T* p)
 {
-    if (VEC) {                                            // width is a multiple of COLS
-        const uint4 w = *reinterpret_cast<const uint4*>(x + min(col, width - COLS));
-        const unsigned e[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int q = 0; q < COLS; q++) {
-            if constexpr (sizeof(T) == 4) v[q] = __uint_as_float(e[q]);
-            else v[q] = (q & 1) ? high16<T>(e[q >> 1]) : low16<T>(e[q >> 1]);
-        }
-#pragma unroll
-        for (int q = 0; q < COLS; q++) v[q] = col < width ? v[q] : 0.f;
-    } else {
-#pragma unroll
-        for (int q = 0; q < COLS; q++) v[q] = lb_load(x[min(col + q, width - 1)]);
-#pragma unroll
-        for (int q = 0; q < COLS; q++) v[q] = col + q < width ? v[q] : 0.f;
-    }
+    uint4 w;
+    __builtin_memcpy(&w, p, 16);
+    return w;
 }
 
-template <int FMT, int LANES, typename T, typename S, bool VEC>
+template <int FMT, typename T, typename S, bool FULL>
 __global__ __launch_bounds__(256) void rows8_write_kernel(gs4d_rows8 c, const T* __restrict__ rows, long long ld, long long n,
-                                                          const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int dup)
+                                                          const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int lshift, int dup)
 {
     constexpr int COLS = 16 / (int)sizeof(T);
     __shared__ long long s_slot[ROWS8_ROWS], s_all[GS4D_ROWS8_SCAN];
@@ -86,33 +76,53 @@ __global__ __launch_bounds__(256) void rows8_write_kernel(gs4d_rows8 c, const T*
     __syncthreads();
     const int items = nrow * cpr, ng = (c.width + c.group - 1) / c.group;
     constexpr int U = 4;
+    const T* end = rows + (n - 1) * ld + c.width;
     for (int e0 = threadIdx.x; e0 < items; e0 += 256 * U) {
-        float v[U][COLS];
+        uint4 w[U];
         int ch[U];
         long long slot[U];
+        const T* x[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int e = min(e0 + 256 * u, items - 1);
             const int r = cpr == 1 ? e : (int)__umulhi((unsigned)e, rcp);
             ch[u] = e - r * cpr;
             slot[u] = e0 + 256 * u < items ? s_slot[r] : -1;
-            load_cols<T, COLS, VEC>(v[u], rows + (i0 + r) * ld, ch[u] * COLS, c.width);
+            // the last columns of a row are read with what follows them, those of the array's last row one by one (below)
+            x[u] = rows + (i0 + r) * ld + ch[u] * COLS;
+            // (FULL: a group's columns past the width are read from the row's last ones instead)
+            if (FULL) w[u] = load16(x[u] - max(ch[u] * COLS - (c.width - COLS), 0));
+            else w[u] = load16(x[u] + COLS <= end ? x[u] : reinterpret_cast<const T*>(kZeroPage));
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            float v[COLS];
+            if (!FULL && x[u] + COLS > end) {
+#pragma unroll
+                for (int q = 0; q < COLS; q++) v[q] = x[u] + q < end ? lb_load(x[u][q]) : 0.f;
+            } else {
+                const unsigned e[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+                for (int q = 0; q < COLS; q++) {
+                    if constexpr (sizeof(T) == 4) v[q] = __uint_as_float(e[q]);
+                    else v[q] = (q & 1) ? high16<T>(e[q >> 1]) : low16<T>(e[q >> 1]);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < COLS; q++) v[q] = ch[u] * COLS + (FULL ? 0 : q) < c.width ? v[q] : 0.f;
             unsigned m = 0;
 #pragma unroll
-            for (int q = 0; q < COLS; q++) m = max(m, lb_abs_bits(v[u][q]));
-            const LbScale sc = lb_scale<FMT>(group_max<LANES>(m));
+            for (int q = 0; q < COLS; q++) m = max(m, lb_abs_bits(v[q]));
+            const LbScale sc = lb_scale<FMT>(group_max(m, lshift));
             const int col = ch[u] * COLS;
             if (slot[u] < 0 || col >= c.width) continue;
             unsigned* out = reinterpret_cast<unsigned*>(c.codes + (size_t)slot[u] * c.pitch + col);
-            const unsigned w0 = lb_encode4<FMT>(v[u][0] * sc.inv, v[u][1] * sc.inv, v[u][2] * sc.inv, v[u][3] * sc.inv);
+            const unsigned w0 = lb_encode4<FMT>(v[0] * sc.inv, v[1] * sc.inv, v[2] * sc.inv, v[3] * sc.inv);
             if constexpr (COLS == 8)
-                *reinterpret_cast<uint2*>(out) = make_uint2(w0, lb_encode4<FMT>(v[u][4] * sc.inv, v[u][5] * sc.inv, v[u][6] * sc.inv, v[u][7] * sc.inv));
+                *reinterpret_cast<uint2*>(out) = make_uint2(w0, lb_encode4<FMT>(v[4] * sc.inv, v[5] * sc.inv, v[6] * sc.inv, v[7] * sc.inv));
             else
                 *out = w0;
-            if ((ch[u] & (LANES - 1)) == 0) c.scales[(size_t)slot[u] * ng + ch[u] / LANES] = sc.s;
+            if ((ch[u] & ((1 << lshift) - 1)) == 0) c.scales[(size_t)slot[u] * ng + (ch[u] >> lshift)] = sc.s;
         }
     }
 }
@@ -127,13 +137,11 @@ __global__ __launch_bounds__(256) void rows8_owner_kernel(gs4d_rows8 c, const S*
     if (slot >= 0 && slot < c.capacity) atomicMax(c.owner + slot, (int)(i + 1));
 }
 
-// VEC: the output's rows are 16-byte aligned and width a multiple of COLS; else one number per item, so that neighbouring lanes
-// still write neighbouring addresses
-template <int FMT, typename T, typename S, bool VEC>
+template <int FMT, typename T, typename S, bool FULL>
 __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __restrict__ out, long long ld, long long n,
                                                          const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int gshift)
 {
-    constexpr int COLS = VEC ? 16 / (int)sizeof(T) : 1;
+    constexpr int COLS = 16 / (int)sizeof(T);
     __shared__ long long s_slot[ROWS8_ROWS];
     const long long i0 = (long long)blockIdx.x * rpb;
     const int nrow = (int)min((long long)rpb, n - i0);
@@ -143,7 +151,7 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
     }
     __syncthreads();
     const int items = nrow * cpr, ng = (c.width + c.group - 1) / c.group;
-    constexpr int U = VEC ? 4 : 8;
+    constexpr int U = 4;
     for (int e0 = threadIdx.x; e0 < items; e0 += 256 * U) {
         unsigned w[U][2];
         float s[U];
@@ -157,8 +165,7 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
             const size_t at = slot < 0 ? 0 : (size_t)slot;
             const unsigned char* p = c.codes + at * c.pitch + col[u];
             if constexpr (COLS == 8) { const uint2 t = *reinterpret_cast<const uint2*>(p); w[u][0] = t.x; w[u][1] = t.y; }
-            else if constexpr (COLS == 4) w[u][0] = *reinterpret_cast<const unsigned*>(p);
-            else w[u][0] = *p;
+            else w[u][0] = *reinterpret_cast<const unsigned*>(p);
             s[u] = c.scales[at * ng + (col[u] >> gshift)];
             if (slot < 0) { w[u][0] = 0; w[u][1] = 0; s[u] = 0.f; }
         }
@@ -167,17 +174,17 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
             if (e0 + 256 * u >= items) break;
             T* y = out + (i0 + row[u]) * ld + col[u];
             const float4 a = lb_decode4<FMT>(w[u][0]);
+            T o[COLS] = {lb_store<T>(s[u] * a.x), lb_store<T>(s[u] * a.y), lb_store<T>(s[u] * a.z), lb_store<T>(s[u] * a.w)};
             if constexpr (COLS == 8) {
                 const float4 b = lb_decode4<FMT>(w[u][1]);
-                T o[8] = {lb_store<T>(s[u] * a.x), lb_store<T>(s[u] * a.y), lb_store<T>(s[u] * a.z), lb_store<T>(s[u] * a.w),
-                          lb_store<T>(s[u] * b.x), lb_store<T>(s[u] * b.y), lb_store<T>(s[u] * b.z), lb_store<T>(s[u] * b.w)};
-                uint4 q;
-                __builtin_memcpy(&q, o, 16);
-                *reinterpret_cast<uint4*>(y) = q;
-            } else if constexpr (COLS == 4) {
-                *reinterpret_cast<float4*>(y) = make_float4(s[u] * a.x, s[u] * a.y, s[u] * a.z, s[u] * a.w);
+                o[4] = lb_store<T>(s[u] * b.x); o[5] = lb_store<T>(s[u] * b.y); o[6] = lb_store<T>(s[u] * b.z); o[7] = lb_store<T>(s[u] * b.w);
+            }
+            if (FULL || col[u] + COLS <= c.width) {
+                __builtin_memcpy(y, o, 16);
             } else {
-                *y = lb_store<T>(s[u] * a.x);
+#pragma unroll
+                for (int q = 0; q < COLS - 1; q++)
+                    if (col[u] + q < c.width) y[q] = o[q];
             }
         }
     }
@@ -217,7 +224,7 @@ __global__ __launch_bounds__(256) void keep_jobs_kernel(Gs4dKeepJobs jobs, long 
                 }
                 m = max(m, lb_abs_bits(e[q]));
             }
-            m = group_max<16>(m);
+            m = group_max(m, 4);
             unsigned w;
             float s;
             if (J.relu) {
@@ -371,28 +378,39 @@ __device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b)
 template <typename T> struct Group { uint4 w[4]; };
 template <> struct Group<float> { uint4 w[8]; };
 
-// VEC: rows start on 16 bytes and C is a multiple of 8.  Columns past C are read somewhere inside the row; the caller clears them.
+// VEC: C is a multiple of 8.  Columns past C are read somewhere inside the row (VEC) or with whatever follows the row; the caller
+// clears them.  end: the end of the array, past which nothing is read (fix_end() reads the last row's last columns).
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_group(Group<T>& g, const T* __restrict__ row, int c0, int C)
+__device__ __forceinline__ void load_group(Group<T>& g, const T* __restrict__ row, int c0, int C, const T* __restrict__ end)
 {
     constexpr int PER = 16 / (int)sizeof(T);              // elements per 16 bytes
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        if constexpr (VEC) {
-            const T* p = row + min(c0 + 16 * t, C - 8);
+        const T* p = row + min(c0 + 16 * t, VEC ? C - 8 : C - 1);
+        if (!VEC) p = p + 8 <= end ? p : reinterpret_cast<const T*>(kZeroPage);
 #pragma unroll
-            for (int q = 0; q < 8 / PER; q++) g.w[t * (8 / PER) + q] = reinterpret_cast<const uint4*>(p)[q];
-        } else if constexpr (sizeof(T) == 4) {
-            unsigned e[8];
+        for (int q = 0; q < 8 / PER; q++) g.w[t * (8 / PER) + q] = load16(p + q * PER);
+    }
+}
+
+// the columns that load_group() did not read because 8 of them would pass the end of the array
+template <typename T>
+__device__ __forceinline__ void fix_end(Group<T>& g, const T* __restrict__ row, int c0, int C, const T* __restrict__ end)
+{
 #pragma unroll
-            for (int q = 0; q < 8; q++) e[q] = __float_as_uint(row[min(c0 + 16 * t + q, C - 1)]);
+    for (int t = 0; t < 4; t++) {
+        const int c = c0 + 16 * t;
+        if (c >= C || row + c + 8 <= end) continue;
+        unsigned e[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            if constexpr (sizeof(T) == 4) e[q] = __float_as_uint(row[min(c + q, C - 1)]);
+            else e[q] = reinterpret_cast<const unsigned short*>(row)[min(c + q, C - 1)];
+        }
+        if constexpr (sizeof(T) == 4) {
             g.w[2 * t] = make_uint4(e[0], e[1], e[2], e[3]);
             g.w[2 * t + 1] = make_uint4(e[4], e[5], e[6], e[7]);
         } else {
-            unsigned e[8];
-            const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-#pragma unroll
-            for (int q = 0; q < 8; q++) e[q] = p[min(c0 + 16 * t + q, C - 1)];
             g.w[t] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
     }
@@ -480,6 +498,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     const int C = a.C, F = a.F;
     int f0 = cb * a.blocks * NT * 32;
     const T* __restrict__ X = (const T*)a.x;
+    const T* __restrict__ end = X + (a.N - 1) * a.ldx + C;
     const T* __restrict__ W = (const T*)a.w;
     auto feature = [&](int nt, int l) { return f0 + (sizeof(T) == 4 ? nt * 32 + l : (nt >> 1) * 64 + 2 * l + (nt & 1)); };
     auto stage = [&](int g0, int n, uint4* s_w) {         // groups g0 .. g0 + n - 1 of the weight, for the features from f0 on
@@ -519,7 +538,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     // the memory channels at a time
     const int turn = a.chunk >= a.groups ? wave % a.groups : 0;
     auto group_at = [&](int gi) { const int g = gi + turn; return g < a.groups ? g : g - a.groups; };
-    load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C);      // in flight while the weight is staged
+    load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C, end);      // in flight while the weight is staged
     if constexpr (MODE == ROWS_WIDE) {
         for (int k = 0; k < a.blocks; k++) { stage(0, 1, s_w + k * BLOCK); f0 += NT * 32; }
         f0 -= a.blocks * NT * 32;
@@ -602,11 +621,14 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 stage(gi, min(a.chunk, a.groups - gi), s_w);
                 __syncthreads();
             }
-            if (g * 64 + 64 > Cn) clear_past(cur, g * 64 + 8 * h, Cn);
+            if (g * 64 + 64 > Cn) {
+                if (!VEC) fix_end(cur, row_of(tile), g * 64 + 8 * h, Cn, end);
+                clear_past(cur, g * 64 + 8 * h, Cn);
+            }
             const uint4* __restrict__ wl = s_w + (size_t)(a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
             const bool more = gi + 1 < a.groups;
             Group<T> nxt;
-            if (MODE == ROWS_MANY) load_group<T, VEC>(nxt, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn);
+            if (MODE == ROWS_MANY) load_group<T, VEC>(nxt, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn, end);
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
             float v[4][8];
@@ -717,7 +739,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 }
                 f0 -= a.blocks * NT * 32;
                 __builtin_amdgcn_sched_barrier(0);
-                load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn);
+                load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn, end);
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -731,7 +753,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                     cur = nxt;
                 } else {
                     __builtin_amdgcn_sched_barrier(0);
-                    load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn);
+                    load_group<T, VEC>(cur, row_of(tile + (long long)WAVES * a.nwg), 8 * h, Cn, end);
                 }
             }
         }
@@ -766,7 +788,9 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
     const bool mine = g < a.groups;
     const int gc = min(g, a.groups - 1), m = mt * 64 + 2 * i, kp = a.keep.kp, ng = kp / 64, M = a.M;
     const T* __restrict__ dy = (const T*)a.dy;
-    const int mc = VEC ? min(m, M - 2) : min(m, M - 1), second = m + 1 < M ? 1 : 0;
+    // VEC: two columns at once, at any alignment; an odd M's last column is the second of its pair
+    const int mc = VEC ? min(m, M - 2) : 0;
+    const bool shifted = VEC && m == M - 1;
     const unsigned char* __restrict__ codes = a.keep.codes + gc * 64;
     const float* __restrict__ scales = a.keep.scales + gc;
     // a load's address is the wave's row plus the lane's share, which does not change
@@ -785,11 +809,11 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
             }
             const T* p = reinterpret_cast<const T*>(pd);
             if constexpr (sizeof(T) == 4) {
-                if constexpr (VEC) { const uint2 w = *reinterpret_cast<const uint2*>(p); r.d[q][0] = w.x; r.d[q][1] = w.y; }
-                else { r.d[q][0] = __float_as_uint(p[0]); r.d[q][1] = __float_as_uint(p[second]); }
+                if constexpr (VEC) __builtin_memcpy(r.d[q], p, 8);
+                else r.d[q][0] = r.d[q][1] = __float_as_uint(p[0]);
             } else {
-                if constexpr (VEC) r.d[q][0] = *reinterpret_cast<const unsigned*>(p);
-                else { const unsigned short* u = reinterpret_cast<const unsigned short*>(p); r.d[q][0] = u[0] | (unsigned)u[second] << 16; }
+                if constexpr (VEC) __builtin_memcpy(r.d[q], p, 4);
+                else r.d[q][0] = *reinterpret_cast<const unsigned short*>(p);
             }
             r.c[q] = *reinterpret_cast<const unsigned short*>(pc);
         }
@@ -811,6 +835,7 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
             float s = h ? cur.hi[q] : cur.lo[q];
             if constexpr (sizeof(T) == 4) { d0[q] = __uint_as_float(cur.d[q][0]); d1[q] = __uint_as_float(cur.d[q][1]); }
             else { d0[q] = low16<T>(cur.d[q][0]); d1[q] = high16<T>(cur.d[q][0]); }
+            if (VEC) d0[q] = shifted ? d1[q] : d0[q];
             if (LAST && r0 + 8 * h + q >= n1) { d0[q] = 0.f; d1[q] = 0.f; s = 0.f; }
             if (g == 0) { db0 += d0[q]; db1 += d1[q]; }
             d0[q] *= s; d1[q] *= s;
@@ -1056,16 +1081,19 @@ int gs4d_rows8_write(const gs4d_rows8* c, const void* rows, int dtype, long long
         by_type(dtype, [&](auto t) {
             using T = decltype(t);
             constexpr int COLS = 16 / (int)sizeof(T);
-            const RowItems it = row_items(lb_groups(c->width, c->group) * (c->group / COLS), n);
-            const bool vec = c->width % COLS == 0 && ((uintptr_t)rows & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+            // lanes per group; a row shorter than a group takes as few as hold it
+            const int groups = lb_groups(c->width, c->group);
+            int lshift = 0;
+            while ((COLS << lshift) < (groups > 1 ? c->group : c->width)) lshift++;
+            const RowItems it = row_items(groups << lshift, n);
             return by_fmt(c->fmt, [&](auto f) {
                 constexpr int F = decltype(f)::value;
-                auto go = [&](auto v) {
-                    constexpr bool V = decltype(v)::value != 0;
-                    auto k = c->group == 32 ? rows8_write_kernel<F, 32 / COLS, T, S, V> : c->group == 64 ? rows8_write_kernel<F, 64 / COLS, T, S, V> : rows8_write_kernel<F, 128 / COLS, T, S, V>;
-                    hipLaunchKernelGGL(k, dim3(it.grid), dim3(256), 0, s, *c, (const T*)rows, ld, n, sl, start, it.cpr, it.rpb, it.rcp, dup);
+                auto go = [&](auto full) {
+                    constexpr bool FULL = decltype(full)::value != 0;
+                    hipLaunchKernelGGL((rows8_write_kernel<F, T, S, FULL>), dim3(it.grid), dim3(256), 0, s, *c, (const T*)rows, ld, n, sl, start, it.cpr, it.rpb, it.rcp, lshift, dup);
                 };
-                if (vec) go(Int<1>()); else go(Int<0>());
+                if (c->width % COLS == 0) go(Int<1>());
+                else go(Int<0>());
                 return 0;
             });
         });
@@ -1087,16 +1115,15 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
         constexpr int COLS = 16 / (int)sizeof(T);
-        const bool vec = c->width % COLS == 0 && ((uintptr_t)out & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
-        const RowItems it = row_items(vec ? c->width / COLS : c->width, n);
+        const RowItems it = row_items((c->width + COLS - 1) / COLS, n);
         return by_fmt(c->fmt, [&](auto f) {
             constexpr int F = decltype(f)::value;
-            auto go = [&](auto tag, auto v) {
+            auto go = [&](auto tag, auto full) {
                 using S = decltype(tag);
-                hipLaunchKernelGGL((rows8_read_kernel<F, T, S, decltype(v)::value != 0>), dim3(it.grid), dim3(256), 0, s, *c, (T*)out, ld, n, (const S*)slots, start, it.cpr, it.rpb, it.rcp, gshift);
+                hipLaunchKernelGGL((rows8_read_kernel<F, T, S, decltype(full)::value != 0>), dim3(it.grid), dim3(256), 0, s, *c, (T*)out, ld, n, (const S*)slots, start, it.cpr, it.rpb, it.rcp, gshift);
             };
             const bool narrow = slots && slot_bytes == 4;
-            if (vec) { if (narrow) go(int(), Int<1>()); else go((long long)0, Int<1>()); }
+            if (c->width % COLS == 0) { if (narrow) go(int(), Int<1>()); else go((long long)0, Int<1>()); }
             else { if (narrow) go(int(), Int<0>()); else go((long long)0, Int<0>()); }
             return 0;
         });
@@ -1139,7 +1166,7 @@ template <typename T, bool DX>
 static int launch_rows(RowsArgs& a, hipStream_t s)
 {
     constexpr int LDS = 144 * 1024;
-    const bool vec = a.C % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.ldx * sizeof(T)) % 16 == 0;
+    const bool vec = a.C % 8 == 0;
     const int nt = sizeof(T) == 4 ? (a.F <= 32 ? 1 : 2) : a.F <= 64 ? 2 : 4;
     a.groups = (a.C + 63) / 64;
     const int per = 4 * nt * kTerms<T> * 1024;
@@ -1177,7 +1204,7 @@ template <typename T>
 static int launch_dw(DwArgs& a, int fmt, void* dw, void* db, hipStream_t s)
 {
     if (dw) {
-        const bool vec = a.M % 2 == 0 && ((uintptr_t)a.dy & (2 * sizeof(T) - 1)) == 0;
+        const bool vec = a.M > 1;
         const unsigned grid = (unsigned)(a.chunks * a.mtiles * ((a.groups + a.gw - 1) / a.gw));
         by_fmt(fmt, [&](auto f) {
             constexpr int F = decltype(f)::value;

@@ -48,7 +48,7 @@ def _format(fmt):
 def _on_device(name, t, dev=None):
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} must be on a HIP device; there is no CPU path")
     if dev is not None and t.device != dev:
         raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
@@ -99,20 +99,21 @@ class RowCache:
         self.capacity, self.device = codes.shape[0], codes.device
         self._owner = None
         self._desc = Rows8(codes.data_ptr(), scales.data_ptr(), None, self.capacity, width, codes.shape[1], group, f)
+        self._ref = C.addressof(self._desc)
 
     def _at(self, slots, start, n):
-        """-> (pointer, bytes per slot, tensor to keep alive); checks what the host can see."""
+        """-> (address, bytes per slot, tensor to keep alive); checks what the host can see."""
         if slots is None:
             if start < 0 or start + n > self.capacity:
                 raise RuntimeError(f"RowCache: rows {start} .. {start + n} do not fit {self.capacity} slots")
-            return C.c_void_p(0), 0, None
+            return None, 0, None
         if start != 0:
             raise RuntimeError("RowCache: give either slots or start")
         _on_device("slots", slots, self.device)
         if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
             raise RuntimeError("RowCache: slots must be a vector of int32 or int64")
         slots = slots.contiguous()
-        return C.c_void_p(slots.data_ptr()), slots.element_size(), slots
+        return slots.data_ptr(), 8 if slots.dtype is torch.int64 else 4, slots
 
     def write(self, rows, slots=None, start=0):
         """rows [n, width] (float32, bfloat16 or float16, any row stride) to the slots start, start + 1, ... or to slots [n]
@@ -133,11 +134,11 @@ class RowCache:
         if slots is not None and n > SCAN and self._owner is None:
             self._owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
             self._desc.owner = self._owner.data_ptr()
-        with torch.cuda.device(self.device):
-            rc = _cabi.lib().gs4d_rows8_write(C.byref(self._desc), _cabi.ptr(rows), C.c_int(dt),
-                                              C.c_longlong(rows.stride(0) if n > 1 else self.width), C.c_longlong(n), p,
-                                              C.c_int(size), C.c_longlong(int(start)), _cabi.current_stream(self.device))
-        _cabi.check(rc, "gs4d_rows8_write")
+        with _cabi.on_device(self.device):
+            rc = _cabi.lib().gs4d_rows8_write(self._ref, rows.data_ptr(), dt, rows.stride(0) if n > 1 else self.width, n, p, size,
+                                              int(start), _cabi.stream_of(self.device))
+        if rc:
+            _cabi.check(rc, "gs4d_rows8_write")
 
     def read(self, slots=None, start=0, count=None, dtype=torch.float32):
         """-> [n, width] of `dtype`: the rows at slots [n] (zeros where a slot lies outside the cache), or `count` rows (all
@@ -157,11 +158,11 @@ class RowCache:
         out = torch.empty(n, self.width, dtype=dtype, device=self.device)
         if n == 0:
             return out
-        with torch.cuda.device(self.device):
-            rc = _cabi.lib().gs4d_rows8_read(C.byref(self._desc), _cabi.ptr(out), C.c_int(DTYPES[dtype]), C.c_longlong(self.width),
-                                             C.c_longlong(n), p, C.c_int(size), C.c_longlong(int(start)),
-                                             _cabi.current_stream(self.device))
-        _cabi.check(rc, "gs4d_rows8_read")
+        with _cabi.on_device(self.device):
+            rc = _cabi.lib().gs4d_rows8_read(self._ref, out.data_ptr(), DTYPES[dtype], self.width, n, p, size, int(start),
+                                             _cabi.stream_of(self.device))
+        if rc:
+            _cabi.check(rc, "gs4d_rows8_read")
         return out
 
 
@@ -193,13 +194,13 @@ def frame_features(cache, planes, aabb, points, t):
     aabb, points, t = aabb.detach().contiguous(), points.detach().contiguous(), t.detach().reshape(-1).contiguous()
     out = torch.empty(P, cache.width, dtype=torch.float32, device=dev)
     n = len(planes)
-    with torch.cuda.device(dev):
+    with _cabi.on_device(dev):
         rc = _cabi.lib().gs4d_frame_features(
-            C.byref(cache._desc), C.c_int(levels), C.c_int(ch), (C.c_void_p * n)(*[p.data_ptr() for p in planes]),
-            (C.c_int * n)(*[p.shape[3] for p in planes]), (C.c_int * n)(*[p.shape[2] for p in planes]), _cabi.ptr(aabb),
-            _cabi.ptr(points), _cabi.ptr(t), C.c_int(0 if t.numel() == 1 else 1), C.c_longlong(P), _cabi.ptr(out),
-            C.c_longlong(cache.width), _cabi.current_stream(dev))
-    _cabi.check(rc, "gs4d_frame_features")
+            cache._ref, levels, ch, (C.c_void_p * n)(*[p.data_ptr() for p in planes]), (C.c_int * n)(*[p.shape[3] for p in planes]),
+            (C.c_int * n)(*[p.shape[2] for p in planes]), aabb.data_ptr(), points.data_ptr(), t.data_ptr(),
+            0 if t.numel() == 1 else 1, P, out.data_ptr(), cache.width, _cabi.stream_of(dev))
+    if rc:
+        _cabi.check(rc, "gs4d_frame_features")
     return out
 
 
@@ -217,15 +218,14 @@ class _Linear(torch.autograd.Function):
         # needs_input_grad says what requires a gradient, grad whether one is recorded at all
         what = (KEEP_CODES if ctx.needs_input_grad[1] else 0) | (KEEP_SIGNS if relu and ctx.needs_input_grad[0] else 0) if grad else 0
         y = torch.empty(N, M, dtype=x.dtype, device=dev)
-        keep = torch.empty(int(L.gs4d_linear8_keep_bytes(C.c_longlong(N), C.c_int(K), C.c_int(what))) if what else 0,
-                           dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = L.gs4d_linear8_forward(C.c_int(dt), C.c_longlong(N), C.c_int(K), C.c_int(M), _cabi.ptr(rows),
-                                        C.c_longlong(rows.stride(0) if N > 1 else K), _cabi.ptr(w), _cabi.ptr(b), C.c_int(relu),
-                                        C.c_int(fmt), _cabi.ptr(y), _cabi.ptr(keep), C.c_int(what), _cabi.current_stream(dev))
-        _cabi.check(rc, "gs4d_linear8_forward")
+        keep = torch.empty(L.gs4d_linear8_keep_bytes(N, K, what), dtype=torch.uint8, device=dev) if what else None
+        with _cabi.on_device(dev):
+            rc = L.gs4d_linear8_forward(dt, N, K, M, rows.data_ptr(), rows.stride(0) if N > 1 else K, w.data_ptr(), _cabi.address(b),
+                                        relu, fmt, y.data_ptr(), _cabi.address(keep), what, _cabi.stream_of(dev))
+        if rc:
+            _cabi.check(rc, "gs4d_linear8_forward")
         ctx.save_for_backward(weight, keep)
-        ctx.args = (dt, N, K, M, int(relu), fmt, what, x.shape, None if bias is None else bias.shape)
+        ctx.args = (dt, N, K, M, relu, fmt, what, x.shape, None if bias is None else bias.shape)
         return y.view(*x.shape[:-1], M)
 
     @staticmethod
@@ -240,13 +240,13 @@ class _Linear(torch.autograd.Function):
         dx = torch.empty(N, K, dtype=g.dtype, device=dev) if need_x else None
         dw = torch.empty(M, K, dtype=g.dtype, device=dev) if need_w else None
         db = torch.empty(M, dtype=g.dtype, device=dev) if need_b else None
-        nb = int(L.gs4d_linear8_scratch_bytes(C.c_longlong(N), C.c_int(K), C.c_int(M))) if need_w or need_b else 0
-        scratch = torch.empty(nb, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = L.gs4d_linear8_backward(C.c_int(dt), C.c_longlong(N), C.c_int(K), C.c_int(M), _cabi.ptr(dy), _cabi.ptr(w),
-                                         C.c_int(relu), C.c_int(fmt), _cabi.ptr(keep), C.c_int(what), _cabi.ptr(dx), _cabi.ptr(dw),
-                                         _cabi.ptr(db), _cabi.ptr(scratch), _cabi.current_stream(dev))
-        _cabi.check(rc, "gs4d_linear8_backward")
+        scratch = torch.empty(L.gs4d_linear8_scratch_bytes(N, K, M), dtype=torch.uint8, device=dev) if need_w or need_b else None
+        with _cabi.on_device(dev):
+            rc = L.gs4d_linear8_backward(dt, N, K, M, dy.data_ptr() if N else None, w.data_ptr(), relu, fmt, _cabi.address(keep), what,
+                                         _cabi.address(dx), _cabi.address(dw), _cabi.address(db), _cabi.address(scratch),
+                                         _cabi.stream_of(dev))
+        if rc:
+            _cabi.check(rc, "gs4d_linear8_backward")
         return None if dx is None else dx.view(x_shape), dw, None if db is None else db.view(b_shape), None, None, None
 
 
@@ -267,4 +267,4 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
         _on_device("bias", bias, x.device)
         if bias.dtype != x.dtype or tuple(bias.shape) != (weight.shape[0],):
             raise RuntimeError(f"linear: bias must be {x.dtype} [{weight.shape[0]}], got {bias.dtype} {tuple(bias.shape)}")
-    return _Linear.apply(x, weight, bias, bool(relu), f, torch.is_grad_enabled())
+    return _Linear.apply(x, weight, bias, int(bool(relu)), f, torch.is_grad_enabled())
