@@ -502,30 +502,72 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     const T* __restrict__ W = (const T*)a.w;
     auto feature = [&](int nt, int l) { return f0 + (sizeof(T) == 4 ? nt * 32 + l : (nt >> 1) * 64 + 2 * l + (nt & 1)); };
     auto stage = [&](int g0, int n, uint4* s_w) {         // groups g0 .. g0 + n - 1 of the weight, for the features from f0 on
-        for (int e = tid; e < n * 4 * NT * 64; e += THREADS) {
-            const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
-            const int f = feature(nt, l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
-            const T* p = W + (long long)min(f, F - 1) * a.wf;
-            if constexpr (sizeof(T) == 4) {
-                float v[8];
+        // U items at a time, their loads in flight together: one after the other, a 512 x 512 weight took 35 us to arrive
+        constexpr int U = MODE == ROWS_MANY ? 4 : 1;     // (one group is few rounds, and the registers are worth more: 405 us, not 460)
+        const int total = n * 4 * NT * 64;
+        for (int e0 = tid; e0 < total; e0 += THREADS * U) {
+            unsigned v[U][8];
 #pragma unroll
-                for (int q = 0; q < 8; q++) {
-                    const float u = p[(long long)min(c + q, C - 1) * a.wc];
-                    v[q] = f < F && c + q < C ? u : 0.f;
+            for (int u = 0; u < U; u++) {
+                const int e = min(e0 + u * THREADS, total - 1);
+                const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
+                const int f = feature(nt, l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
+                const T* p = W + (long long)min(f, F - 1) * a.wf;
+                if (!DX && C >= 8) {                      // the row's columns, or its last 8
+                    const T* w = p + min(c, C - 8);
+                    if constexpr (sizeof(T) == 4) {
+                        const uint4 x = load16(w), y = load16(w + 4);
+                        v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+                        v[u][4] = y.x; v[u][5] = y.y; v[u][6] = y.z; v[u][7] = y.w;
+                    } else {
+                        const uint4 x = load16(w);
+                        v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const T* w = p + (long long)min(c + q, C - 1) * a.wc;
+                        if constexpr (sizeof(T) == 4) v[u][q] = __float_as_uint(*w);
+                        else v[u][q] = *reinterpret_cast<const unsigned short*>(w);
+                    }
                 }
-                uint4 o[TERMS];
-                split8<TERMS>(v, o);
+            }
 #pragma unroll
-                for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
-            } else {
-                unsigned v[8];
-                const unsigned short* ps = reinterpret_cast<const unsigned short*>(p);
+            for (int u = 0; u < U; u++) {
+                const int e = min(e0 + u * THREADS, total - 1);
+                const int l = e & 63, nt = (e >> 6) % NT, step = (e >> 6) / NT;
+                const int f = feature(nt, l & 31), c = g0 * 64 + step * 16 + 8 * (l >> 5);
+                if (!DX && C >= 8 && c > C - 8) {         // columns past C - 8: read again, one by one
+                    const T* p = W + (long long)min(f, F - 1) * a.wf;
+                    unsigned t[8];
 #pragma unroll
-                for (int q = 0; q < 8; q++) {
-                    const unsigned u = ps[(long long)min(c + q, C - 1) * a.wc];
-                    v[q] = f < F && c + q < C ? u : 0u;
+                    for (int q = 0; q < 8; q++) {
+                        if constexpr (sizeof(T) == 4) t[q] = __float_as_uint(p[min(c + q, C - 1)]);
+                        else t[q] = reinterpret_cast<const unsigned short*>(p)[min(c + q, C - 1)];
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        if constexpr (sizeof(T) == 4) v[u][q] = t[q];
+                        else if (q < 4) v[u][q] = t[2 * q] | t[2 * q + 1] << 16;
+                    }
                 }
-                s_w[(step * NT + nt) * 64 + l] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+                if constexpr (sizeof(T) == 4) {
+                    float x[8];
+#pragma unroll
+                    for (int q = 0; q < 8; q++) x[q] = f < F && c + q < C ? __uint_as_float(v[u][q]) : 0.f;
+                    uint4 o[TERMS];
+                    split8<TERMS>(x, o);
+#pragma unroll
+                    for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
+                } else {
+                    unsigned x[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        x[q] = !DX && C >= 8 ? v[u][q] : v[u][2 * q] | v[u][2 * q + 1] << 16;
+                        x[q] = f >= F || c + 2 * q >= C ? 0u : c + 2 * q + 1 < C ? x[q] : x[q] & 0xffffu;
+                    }
+                    s_w[(step * NT + nt) * 64 + l] = make_uint4(x[0], x[1], x[2], x[3]);
+                }
             }
         }
     };
@@ -728,6 +770,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                     if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs[t]);
                     else xs[t][0] = cur.w[t];
                 }
+#pragma unroll 1
                 for (int k = 0; k < a.blocks; k++) {
                     begin();
 #pragma unroll
@@ -759,6 +802,138 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
         }
         if (MODE != ROWS_WIDE) finish();
     }
+}
+
+// A few rows (a single query): 16 lanes per feature read its weights once, 4 columns each, and multiply them with
+// all the rows.  No staging, so the latency is one round trip to memory (one row of 64 -> 64: 2.6 us, with the matrix cores 6.8).
+#define FEW_ROWS 4            // per workgroup
+#define FEW_MOST 2048
+static bool few(int dtype, long long N, int K, int M) { return N <= FEW_MOST && N * K * M <= 1ll << (dtype == GS4D_F32 ? 28 : 27); }
+template <typename T>
+__global__ __launch_bounds__(256) void linear8_few_kernel(RowsArgs a)
+{
+    const int fblocks = (a.F + 15) / 16;
+    if ((int)blockIdx.x >= fblocks) {
+        const int ng = a.keep.kp / 64, here = min(FEW_ROWS, (int)a.N - (int)blockIdx.y * FEW_ROWS);
+        const int item = min(((int)blockIdx.x - fblocks) * 16 + (int)(threadIdx.x >> 4), here * ng - 1), row = blockIdx.y * FEW_ROWS + item / ng, g = item % ng, sub = threadIdx.x & 15,
+                  col = g * 64 + 4 * sub;
+        const T* __restrict__ x = (const T*)a.x + row * a.ldx;
+        float e[4];
+        unsigned m = 0, w0 = 0, w1 = 0;                   // the sign words: column c of the group is bit c & 31 of word c >> 5, or
+#pragma unroll                                            // bit c >> 1 of word c & 1 (16-bit types)
+        for (int q = 0; q < 4; q++) {
+            e[q] = col + q < a.C ? lb_load(x[min(col + q, a.C - 1)]) : 0.f;
+            if (!a.lowest && e[q] < 0.f) e[q] = 0.f;
+            m = max(m, lb_abs_bits(e[q]));
+            const unsigned positive = lb_abs_bits(e[q]) ? 1u : 0u;
+            const int c = 4 * sub + q;
+            if (sizeof(T) == 4) { if (c < 32) w0 |= positive << (c & 31); else w1 |= positive << (c & 31); }
+            else if (q & 1) w1 |= positive << (c >> 1);
+            else w0 |= positive << (c >> 1);
+        }
+        m = group_max(m, 4);
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) { w0 |= (unsigned)__shfl_xor((int)w0, k, 64); w1 |= (unsigned)__shfl_xor((int)w1, k, 64); }
+        if (a.keep.bits && sub == 0) *reinterpret_cast<uint2*>(a.keep.bits + (size_t)row * (a.keep.kp / 8) + g * 8) = make_uint2(w0, w1);
+        auto encode = [&](auto fm) {
+            constexpr int FMT = decltype(fm)::value;
+            const LbScale sc = lb_scale<FMT>(m);
+            *reinterpret_cast<unsigned*>(a.keep.codes + (size_t)row * a.keep.kp + col) = lb_encode4<FMT>(e[0] * sc.inv, e[1] * sc.inv, e[2] * sc.inv, e[3] * sc.inv);
+            if (sub == 0) a.keep.scales[(size_t)row * ng + g] = sc.s;
+        };
+        if (!a.keep.codes) return;
+        if (a.fmt == GS4D_FMT_INT8) encode(Int<GS4D_FMT_INT8>());
+        else if (a.fmt == GS4D_FMT_UINT8) encode(Int<GS4D_FMT_UINT8>());
+        else if (a.fmt == GS4D_FMT_E4M3) encode(Int<GS4D_FMT_E4M3>());
+        else encode(Int<GS4D_FMT_E5M2>());
+        return;
+    }
+    const int sub = threadIdx.x & 15, f = blockIdx.x * 16 + (threadIdx.x >> 4), fc = min(f, a.F - 1), C = a.C;
+    const T* __restrict__ w = (const T*)a.w + (long long)fc * a.wf;
+    const T* __restrict__ x = (const T*)a.x;
+    const float floor = a.lowest ? -INFINITY : 0.f;
+    const int r0 = blockIdx.y * FEW_ROWS, last = (int)a.N - 1;
+    float acc[FEW_ROWS] = {};
+    for (int c = 4 * sub; c < C; c += 64) {
+        float wv[4], xv[FEW_ROWS][4];
+        if (c + 4 <= C) {
+            T e[4], g[FEW_ROWS][4];
+            __builtin_memcpy(e, w + c, sizeof(e));
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; r++) __builtin_memcpy(g[r], x + min(r0 + r, last) * a.ldx + c, sizeof(e));
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                wv[q] = lb_load(e[q]);
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; r++) xv[r][q] = lb_load(g[r][q]);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int k = min(c + q, C - 1);
+                wv[q] = c + q < C ? lb_load(w[k]) : 0.f;
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; r++) xv[r][q] = c + q < C ? lb_load(x[min(r0 + r, last) * a.ldx + k]) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; r++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc[r] = fmaf(xv[r][q] < floor ? floor : xv[r][q], wv[q], acc[r]);      // a NaN stays one
+    }
+    const float b = a.bias ? lb_load(((const T*)a.bias)[fc]) : 0.f;
+#pragma unroll
+    for (int r = 0; r < FEW_ROWS; r++) {
+#pragma unroll
+        for (int k = 8; k > 0; k >>= 1) acc[r] += __shfl_xor(acc[r], k, 64);
+        if (sub == 0 && f < a.F && r0 + r <= last) ((T*)a.y)[(long long)(r0 + r) * a.F + f] = lb_store<T>(acc[r] + b);
+    }
+}
+
+// dx of a few rows: a workgroup takes 64 columns, 4 per lane, and deals the rows of the weight to 16 slices, summed through LDS
+template <typename T>
+__global__ __launch_bounds__(256) void linear8_few_dx_kernel(RowsArgs a)
+{
+    __shared__ float s_part[16][FEW_ROWS][64];
+    const int sub = threadIdx.x & 15, slice = threadIdx.x >> 4, k = blockIdx.x * 64 + 4 * sub, F = a.F, C = a.C;
+    const int r0 = blockIdx.y * FEW_ROWS, last = (int)a.N - 1;
+    const T* __restrict__ w = (const T*)a.w;
+    const T* __restrict__ dy = (const T*)a.x;
+    float acc[FEW_ROWS][4] = {};
+#pragma unroll 4
+    for (int m = slice; m < C; m += 16) {
+        float wv[4];
+        if (k + 4 <= F) {
+            T e[4];
+            __builtin_memcpy(e, w + (long long)m * F + k, sizeof(e));
+#pragma unroll
+            for (int q = 0; q < 4; q++) wv[q] = lb_load(e[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; q++) wv[q] = lb_load(w[(long long)m * F + min(k + q, F - 1)]);
+        }
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; r++) {
+            const float d = lb_load(dy[(long long)min(r0 + r, last) * a.ldx + m]);
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc[r][q] = fmaf(d, wv[q], acc[r][q]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < FEW_ROWS; r++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) s_part[slice][r][4 * sub + q] = acc[r][q];
+    __syncthreads();
+    const int r = threadIdx.x >> 6, c = threadIdx.x & 63, row = r0 + r, col = blockIdx.x * 64 + c;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; q++) v += s_part[q][r][c];
+    if (row > last || col >= F) return;
+    if (a.keep.bits) {
+        const unsigned* bits = reinterpret_cast<const unsigned*>(a.keep.bits) + (size_t)row * (a.keep.kp / 32) + 2 * blockIdx.x;
+        if (!(sizeof(T) == 4 ? bits[c >> 5] >> (c & 31) & 1u : bits[c & 1] >> (c >> 1) & 1u)) v = 0.f;
+    }
+    ((T*)a.y)[(long long)row * F + col] = lb_store<T>(v);
 }
 
 // dW[m][k] = sum over rows r of dy[r][m] s[r] c[r][k] with the kept codes c and their group's scale s.  The contraction runs over
@@ -1244,7 +1419,14 @@ int gs4d_linear8_forward(int dtype, long long N, int K, int M, const void* x, lo
     a.lowest = relu ? 0 : (int)0x80000000;
     if (what) a.keep = carve_keep(keep, N, K, what, nullptr);
     a.fmt = relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt;
-    const int rc = by_type(dtype, [&](auto t) { return launch_rows<decltype(t), false>(a, s); });
+    const int rc = by_type(dtype, [&](auto t) {
+        if (few(dtype, N, K, M)) {
+            const unsigned keepers = what ? (unsigned)((FEW_ROWS * (a.keep.kp / 64) + 15) / 16) : 0;
+            hipLaunchKernelGGL(linear8_few_kernel<decltype(t)>, dim3((unsigned)((M + 15) / 16) + keepers, (unsigned)((N + FEW_ROWS - 1) / FEW_ROWS)), dim3(256), 0, s, a);
+            return GS4D_OK;
+        }
+        return launch_rows<decltype(t), false>(a, s);
+    });
     if (rc) return rc;
     GS4D_LAUNCH_CHECK("linear8_forward", 0, s);
     return GS4D_OK;
@@ -1269,7 +1451,13 @@ int gs4d_linear8_backward(int dtype, long long N, int K, int M, const void* dy, 
         a.x = dy; a.ldx = M; a.w = w; a.wf = 1; a.wc = K; a.y = dx;
         a.lowest = (int)0x80000000;
         if (relu) a.keep = kp;
-        rc = by_type(dtype, [&](auto t) { return launch_rows<decltype(t), true>(a, s); });
+        rc = by_type(dtype, [&](auto t) {
+            if (few(dtype, N, K, M)) {
+                hipLaunchKernelGGL(linear8_few_dx_kernel<decltype(t)>, dim3((unsigned)((K + 63) / 64), (unsigned)((N + FEW_ROWS - 1) / FEW_ROWS)), dim3(256), 0, s, a);
+                return GS4D_OK;
+            }
+            return launch_rows<decltype(t), true>(a, s);
+        });
         if (rc) return rc;
     }
     if (dw || db) {

@@ -204,36 +204,42 @@ def frame_features(cache, planes, aabb, points, t):
     return out
 
 
+def _linear_forward(x, weight, bias, relu, fmt, what):
+    """-> y, the kept block (or None), rows; x, weight and bias detached."""
+    L = _cabi.lib()
+    dev = x.device
+    M, K = weight.shape
+    rows = x.reshape(-1, K)
+    N = rows.shape[0]
+    if N and ((K > 1 and rows.stride(1) != 1) or (N > 1 and rows.stride(0) < K)):
+        rows = rows.contiguous()
+    weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
+    y = torch.empty(*x.shape[:-1], M, dtype=x.dtype, device=dev)
+    keep = torch.empty(L.gs4d_linear8_keep_bytes(N, K, what), dtype=torch.uint8, device=dev) if what else None
+    with _cabi.on_device(dev):
+        rc = L.gs4d_linear8_forward(DTYPES[x.dtype], N, K, M, rows.data_ptr(), rows.stride(0) if N > 1 else K, weight.data_ptr(),
+                                    _cabi.address(bias), relu, fmt, y.data_ptr(), _cabi.address(keep), what, _cabi.stream_of(dev))
+    if rc:
+        _cabi.check(rc, "gs4d_linear8_forward")
+    return y, keep, N
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, relu, fmt, grad):
-        L = _cabi.lib()
-        dev, dt = x.device, DTYPES[x.dtype]
-        M, K = weight.shape
-        rows = x.detach().reshape(-1, K)
-        N = rows.shape[0]
-        if N and ((K > 1 and rows.stride(1) != 1) or (N > 1 and rows.stride(0) < K)):
-            rows = rows.contiguous()
-        w, b = weight.detach().contiguous(), None if bias is None else bias.detach().contiguous()
-        # needs_input_grad says what requires a gradient, grad whether one is recorded at all
-        what = (KEEP_CODES if ctx.needs_input_grad[1] else 0) | (KEEP_SIGNS if relu and ctx.needs_input_grad[0] else 0) if grad else 0
-        y = torch.empty(N, M, dtype=x.dtype, device=dev)
-        keep = torch.empty(L.gs4d_linear8_keep_bytes(N, K, what), dtype=torch.uint8, device=dev) if what else None
-        with _cabi.on_device(dev):
-            rc = L.gs4d_linear8_forward(dt, N, K, M, rows.data_ptr(), rows.stride(0) if N > 1 else K, w.data_ptr(), _cabi.address(b),
-                                        relu, fmt, y.data_ptr(), _cabi.address(keep), what, _cabi.stream_of(dev))
-        if rc:
-            _cabi.check(rc, "gs4d_linear8_forward")
+    def forward(ctx, x, weight, bias, relu, fmt):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        what = (KEEP_CODES if need_w else 0) | (KEEP_SIGNS if relu and need_x else 0)
+        y, keep, N = _linear_forward(x.detach(), weight.detach(), None if bias is None else bias.detach(), relu, fmt, what)
         ctx.save_for_backward(weight, keep)
-        ctx.args = (dt, N, K, M, relu, fmt, what, x.shape, None if bias is None else bias.shape)
-        return y.view(*x.shape[:-1], M)
+        ctx.args = (DTYPES[x.dtype], N, weight.shape[1], weight.shape[0], relu, fmt, what, x.shape)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         L = _cabi.lib()
         weight, keep = ctx.saved_tensors
-        dt, N, K, M, relu, fmt, what, x_shape, b_shape = ctx.args
+        dt, N, K, M, relu, fmt, what, x_shape = ctx.args
         dev = g.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy, w = g.reshape(N, M).contiguous(), weight.detach().contiguous()
@@ -247,7 +253,7 @@ class _Linear(torch.autograd.Function):
                                          _cabi.stream_of(dev))
         if rc:
             _cabi.check(rc, "gs4d_linear8_backward")
-        return None if dx is None else dx.view(x_shape), dw, None if db is None else db.view(b_shape), None, None, None
+        return None if dx is None else dx.view(x_shape), dw, db, None, None
 
 
 def linear(x, weight, bias=None, relu=False, fmt="int8"):
@@ -267,4 +273,7 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
         _on_device("bias", bias, x.device)
         if bias.dtype != x.dtype or tuple(bias.shape) != (weight.shape[0],):
             raise RuntimeError(f"linear: bias must be {x.dtype} [{weight.shape[0]}], got {bias.dtype} {tuple(bias.shape)}")
-    return _Linear.apply(x, weight, bias, int(bool(relu)), f, torch.is_grad_enabled())
+    relu = int(bool(relu))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _Linear.apply(x, weight, bias, relu, f)
+    return _linear_forward(x, weight, bias, relu, f, 0)[0]
