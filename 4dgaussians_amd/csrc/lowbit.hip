@@ -1222,6 +1222,14 @@ static int check_rows(const gs4d_rows8* c, const void* rows, int dtype, long lon
     return GS4D_OK;
 }
 
+// a launch holds 2^32 work items; wide rows take a workgroup each
+static bool too_many_rows(const gs4d_rows8* c, long long n, const char* who)
+{
+    if (c->width < 2048 || n < 1ll << 24) return false;
+    gs4d_set_error("%s: %lld rows of %d columns are too many for one call", who, n, c->width);
+    return true;
+}
+
 // items per row -> rows per workgroup, workgroups and the multiplier of the division by cpr
 struct RowItems { int cpr, rpb; unsigned rcp, grid; };
 static RowItems row_items(int cpr, long long n)
@@ -1246,6 +1254,7 @@ int gs4d_rows8_write(const gs4d_rows8* c, const void* rows, int dtype, long long
     hipStream_t s = (hipStream_t)stream;
     if (check_rows(c, rows, dtype, ld, n, slots, slot_bytes, start, "gs4d_rows8_write")) return GS4D_EINVAL;
     if (n == 0) return GS4D_OK;
+    if (too_many_rows(c, n, "gs4d_rows8_write")) return GS4D_EINVAL;
     const int dup = !slots || n == 1 ? 0 : n <= GS4D_ROWS8_SCAN ? 1 : 2;
     if (dup == 2 && !c->owner) { gs4d_set_error("gs4d_rows8_write: %lld rows at given slots need the cache's owner array", n); return GS4D_EINVAL; }
     const unsigned ogrid = (unsigned)((n + 255) / 256);
@@ -1286,6 +1295,7 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
     hipStream_t s = (hipStream_t)stream;
     if (check_rows(c, out, dtype, ld, n, slots, slot_bytes, start, "gs4d_rows8_read")) return GS4D_EINVAL;
     if (n == 0) return GS4D_OK;
+    if (too_many_rows(c, n, "gs4d_rows8_read")) return GS4D_EINVAL;
     const int gshift = c->group == 32 ? 5 : c->group == 64 ? 6 : 7;
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -1309,7 +1319,7 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
 
 static int check_linear(int dtype, long long N, int K, int M, int fmt, const char* who)
 {
-    if (dtype < GS4D_F32 || dtype > GS4D_F16 || N < 0 || N > 2147483647ll || K < 1 || M < 1 || K > 65535 * 64 || M > 65535 * 64 ||
+    if (dtype < GS4D_F32 || dtype > GS4D_F16 || N < 0 || N > 2147483647ll || K < 1 || M < 1 || (long long)K * M > 1ll << 28 ||
         fmt < GS4D_FMT_INT8 || fmt > GS4D_FMT_E5M2) {
         gs4d_set_error("%s: unsupported sizes or types", who);
         return GS4D_EINVAL;

@@ -131,11 +131,20 @@ class RowCache:
             return
         if (self.width > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < self.width):
             rows = rows.contiguous()
-        if slots is not None and n > SCAN and self._owner is None:
-            self._owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
-            self._desc.owner = self._owner.data_ptr()
+        ref = self._ref
+        if slots is not None and n > SCAN:
+            if self._owner is not None:
+                pass
+            elif torch.cuda.is_current_stream_capturing():
+                # its zeros are written when the graph runs, not now: an array of the graph's own
+                owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
+                d = Rows8.from_buffer_copy(self._desc)
+                d.owner, ref = owner.data_ptr(), C.addressof(d)
+            else:
+                self._owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
+                self._desc.owner = self._owner.data_ptr()
         with _cabi.on_device(self.device):
-            rc = _cabi.lib().gs4d_rows8_write(self._ref, rows.data_ptr(), dt, rows.stride(0) if n > 1 else self.width, n, p, size,
+            rc = _cabi.lib().gs4d_rows8_write(ref, rows.data_ptr(), dt, rows.stride(0) if n > 1 else self.width, n, p, size,
                                               int(start), _cabi.stream_of(self.device))
         if rc:
             _cabi.check(rc, "gs4d_rows8_write")
@@ -177,27 +186,30 @@ def frame_features(cache, planes, aabb, points, t):
     planes = list(planes)
     if not planes or len(planes) % 3 or len(planes) > 12:
         raise RuntimeError(f"frame_features: three planes for each of 1 to 4 levels, got {len(planes)} planes")
-    for i, p in enumerate(planes):
-        _on_device(f"planes[{i}]", p, dev)
-        if p.dtype != torch.float32 or p.dim() != 4 or p.shape[0] != 1 or p.shape[1] != planes[0].shape[1]:
+    shapes, data = [], []
+    for p in planes:
+        _on_device("planes", p, dev)
+        shape = p.shape
+        if p.dtype is not torch.float32 or len(shape) != 4 or shape[0] != 1 or (shapes and shape[1] != shapes[0][1]):
             raise RuntimeError("frame_features: planes must be float32 [1, C, T, axis] with one C")
+        shapes.append(shape)
+        data.append(p if p.is_contiguous(memory_format=torch.channels_last) else p.detach().contiguous(memory_format=torch.channels_last))
     for name, v in (("aabb", aabb), ("points", points), ("t", t)):
         _on_device(name, v, dev)
-        if v.dtype != torch.float32:
+        if v.dtype is not torch.float32:
             raise RuntimeError(f"frame_features: {name} must be float32, got {v.dtype}")
-    P, ch, levels = points.shape[0], planes[0].shape[1], len(planes) // 3
+    P, ch, levels = points.shape[0], shapes[0][1], len(planes) // 3
     if points.dim() != 2 or points.shape[1] != 3 or tuple(aabb.shape) != (2, 3) or t.numel() not in (1, P):
         raise RuntimeError("frame_features: points [P, 3], aabb [2, 3] and one or P values of t")
     if cache.width != levels * ch or P > cache.capacity:
         raise RuntimeError(f"frame_features: the cache holds {cache.capacity} rows of {cache.width}, expected at least {P} of {levels * ch}")
-    planes = [p.detach().contiguous(memory_format=torch.channels_last) for p in planes]
     aabb, points, t = aabb.detach().contiguous(), points.detach().contiguous(), t.detach().reshape(-1).contiguous()
     out = torch.empty(P, cache.width, dtype=torch.float32, device=dev)
     n = len(planes)
     with _cabi.on_device(dev):
         rc = _cabi.lib().gs4d_frame_features(
-            cache._ref, levels, ch, (C.c_void_p * n)(*[p.data_ptr() for p in planes]), (C.c_int * n)(*[p.shape[3] for p in planes]),
-            (C.c_int * n)(*[p.shape[2] for p in planes]), aabb.data_ptr(), points.data_ptr(), t.data_ptr(),
+            cache._ref, levels, ch, (C.c_void_p * n)(*[p.data_ptr() for p in data]), (C.c_int * n)(*[q[3] for q in shapes]),
+            (C.c_int * n)(*[q[2] for q in shapes]), aabb.data_ptr(), points.data_ptr(), t.data_ptr(),
             0 if t.numel() == 1 else 1, P, out.data_ptr(), cache.width, _cabi.stream_of(dev))
     if rc:
         _cabi.check(rc, "gs4d_frame_features")
@@ -260,7 +272,7 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
     """act(x) @ weight.T + bias with act = relu or nothing: x [..., K], weight [M, K], bias [M], all of one dtype (float32,
     bfloat16 or float16; sums in float32).  For the backward it keeps act(x) in 8 bits in groups of 64 columns ("int8": 255
     levels of a rectified input, 127 each way of a signed one) and, with relu, the signs of x -- a byte or so per number
-    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values."""
+    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  At most 2^28 weights."""
     f = _format(fmt)
     _on_device("x", x)
     _on_device("weight", weight, x.device)

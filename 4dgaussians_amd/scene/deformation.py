@@ -370,6 +370,8 @@ class _DeformFunction(torch.autograd.Function):
 
 
 class Deformation(nn.Module):
+    activation_bits = 32                           # of modules pickled before the switch existed
+
     def __init__(self, D=8, W=256, grid_pe=0, args=None):
         super().__init__()
         self.D, self.W, self.args = D, W, args

@@ -188,6 +188,27 @@ def test_cache_calls_follow_the_current_stream_and_replay():
         same(out, f32(R.quantise(np64(x), "e4m3", 32)[0]))
 
 
+def test_a_cache_captured_before_its_first_write():
+    """The helper array of many scattered rows must not be one whose zeros only a replay writes."""
+    c = lb().RowCache(500, 64)
+    x = rows(1000, 64).cuda()
+    slots = torch.randint(0, 500, (1000,), generator=torch.Generator().manual_seed(0)).cuda()
+    want = f32(R.write(np.zeros((500, 64)), np64(x), slots.tolist(), "int8", 64))
+    filler = torch.full((4096,), 2 ** 30, dtype=torch.int32, device="cuda")           # what uninitialised memory may hold
+    del filler
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.write(x, slots)
+    c.write(x, slots)                                                 # eager, before any replay
+    same(c.read(), want)
+    for _ in range(3):
+        c.write(torch.zeros(500, 64, device="cuda"))
+        graph.replay()
+        same(c.read(), want)
+        c.write(x, slots)
+        same(c.read(), want)
+
+
 # ------------------------------------------------------------------------------------------ frame features
 @pytest.mark.parametrize("levels,ch,res,res_t,n", [(1, 4, 5, 2, 1), (2, 32, 9, 7, 300), (1, 16, 1, 1, 65), (4, 8, 6, 3, 77), (2, 128, 12, 5, 130),
                                                    (1, 256, 4, 4, 9)])
@@ -458,6 +479,52 @@ def test_linear_step_replays_and_follows_the_stream():
         torch.cuda.synchronize()
         for out in outs:
             assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+@pytest.mark.parametrize("n,k,m,dtype", [(3000, 256, 300, torch.float32), (5000, 500, 70, torch.float16), (4000, 40, 600, torch.float32),
+                                         (6, 33, 17, torch.bfloat16)])
+def test_linear_replays_in_every_form(n, k, m, dtype):
+    """Several groups, a wide result, few rows: captured, replayed with other numbers, against the eager call."""
+    x, w, b, dy = make(n, k, m, dtype)
+    X, W, B, D = x.cuda(), w.cuda(), b.cuda(), dy.cuda()
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (X, W, B)]
+        y = lb().linear(*leaves, relu=True)
+        return (y.detach(), *torch.autograd.grad(y, leaves, D))
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(3):
+        X.copy_(rows(n, k, dtype, seed=90 + i))
+        g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+@pytest.mark.parametrize("n,k,m", [(4, 64, 64), (5, 64, 64), (2048, 64, 64), (2049, 64, 64), (600, 512, 500), (1100, 512, 512), (3000, 7, 200),
+                                   (2500, 9, 3), (2500, 1, 1), (2304, 100, 400), (2304, 576, 130)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_on_both_sides_of_every_rule(n, k, m, dtype):
+    check_linear(*make(n, k, m, dtype), True, "int8")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_at_any_alignment(dtype):
+    """Rows, weights and gradients whose first element is not on 16 bytes, pitches that are no multiple of anything."""
+    for n, k, m in ((70, 48, 33), (2500, 72, 66), (2500, 61, 5)):
+        x, w, b, dy = make(n, k, m, dtype)
+        pool = torch.empty(n * (k + 3) + 5, dtype=dtype, device="cuda")
+        xv = pool[1:1 + n * (k + 3)].view(n, k + 3)[:, 1:k + 1]
+        xv.copy_(x)
+        odd = lambda t: torch.cat([torch.zeros(1, dtype=dtype), t.flatten()]).cuda()[1:].view(t.shape)
+        leaves = [xv.detach().requires_grad_(True), odd(w).requires_grad_(True), odd(b).requires_grad_(True)]
+        y = lb().linear(*leaves, relu=True)
+        grads = torch.autograd.grad(y, leaves, odd(dy))
+        yy, gg = check_linear(x, w, b, dy, True, "int8")
+        assert torch.equal(y, yy) and all(torch.equal(a, c) for a, c in zip(grads, gg))
 
 
 def test_linear_refusals():

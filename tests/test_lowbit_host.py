@@ -54,6 +54,7 @@ def test_entry_points_refuse_bad_caches_and_rows(lb, name):
     for n, ld, dtype, slots, size, start in BAD_ROWS:
         assert call(desc(lb), n=n, ld=ld, dtype=dtype, slots=slots, size=size, start=start) == -1, (n, ld, dtype, slots, size, start)
     assert call(desc(lb), rows=0) == -1
+    assert call(desc(lb, capacity=1 << 25, width=4096, pitch=4096), n=1 << 24, ld=4096) == -1
     assert call(desc(lb), n=0) == 0                                   # nothing to do, nothing launched
     if name == "gs4d_rows8_write":                                    # many rows at given slots need the owner array
         assert call(desc(lb), n=lb.SCAN + 1, slots=4096, size=8) == -1
@@ -66,7 +67,7 @@ def test_linear_refuses(lb):
         C.c_int(dtype), C.c_longlong(N), C.c_int(K), C.c_int(M), C.c_void_p(x), C.c_longlong(ldx), C.c_void_p(w), C.c_void_p(b),
         C.c_int(relu), C.c_int(fmt), C.c_void_p(y), C.c_void_p(keep), C.c_int(what), C.c_void_p(0))
     for kw in (dict(dtype=3), dict(N=-1), dict(K=0), dict(M=0), dict(x=0), dict(w=0), dict(y=0), dict(ldx=7), dict(fmt=3), dict(what=1),
-               dict(what=1, keep=64), dict(what=2, keep=4096), dict(N=1 << 31)):
+               dict(what=1, keep=64), dict(what=2, keep=4096), dict(N=1 << 31), dict(K=1 << 15, M=1 << 14, ldx=1 << 15)):
         assert fwd(**kw) == -1, kw
     assert fwd(N=0, x=0, y=0) == 0
     bwd = lambda dtype=0, N=4, K=8, M=8, dy=4096, w=4096, relu=0, fmt=0, keep=4096, what=3, dx=4096, dw=4096, db=0, scratch=4096: \
