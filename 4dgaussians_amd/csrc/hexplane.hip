@@ -258,7 +258,9 @@ __global__ __launch_bounds__(256) void static_features_kernel(int P, int C, int 
 // workgroup blends the lines of its `slice` channels into LDS once and walks the points with half the corner rows, all of them in
 // LDS: what is left to memory is the cache row, the point and the result.  slice / 4 lanes per point, 4 channels of every level
 // each; workgroups that share points (other slices) differ by 8 in their number, i.e. sit behind one L2.
-#define FRAME_LINES_MIN 65536         // points * channels from which the lines pay
+// The lines cost 3 to 6 us before the first point.  2 levels of 128 channels: 8192 points 10 us (frame_features_kernel: 7), 16384
+// points 12.5 (11.5), 32768 points 17 (20), 131072 points 40 (70); of 32 channels: 32768 points 8.4 (7.0), 131072 points 16 (20).
+#define FRAME_LINES_MIN (1 << 21)     // points * channels from which they pay
 struct FrameArgs {
     gs4d_rows8 c; int L, C, slice, nslices, nwg, gshift;
     FramePlanes T; int row0[GS4D_MAX_LEVELS * 3];        // first LDS row of a line
@@ -270,8 +272,7 @@ __global__ __launch_bounds__(512) void frame_lines_kernel(FrameArgs a)
 {
     extern __shared__ float4 s_line[];                    // [row][slice / 4]
     const int lanes = a.slice >> 2, shift = __builtin_ctz(lanes);
-    const int rest = blockIdx.x >> 3, sl = (a.nwg & 7) ? blockIdx.x % a.nslices : rest % a.nslices;
-    const int wg = (a.nwg & 7) ? blockIdx.x / a.nslices : (rest / a.nslices) * 8 + (blockIdx.x & 7);
+    const int rest = blockIdx.x >> 3, sl = rest % a.nslices, wg = (rest / a.nslices) * 8 + (blockIdx.x & 7);     // nwg: a multiple of 8
     const int ch0 = sl * a.slice;
     const float tt = frame_time(a.ft, 0);
     for (int i = 0; i < 3 * L; i++) {
@@ -1083,21 +1084,17 @@ int gs4d_hex_launch_backward(const gs4d_deform_desc* d, const gs4d_deform_grads*
 static int launch_frame(const gs4d_rows8* c, int L, int C, const FramePlanes& T, const float* aabb, const float* points, const FrameTime& ft,
                         long long P, float* out, long long ld, hipStream_t s)
 {
-    // one t and enough points to pay for the lines: about 10 us of blending per workgroup against 60 ns a point and CU
-    int rows = 0;
+    // one t, lines that fit LDS twice per CU, and enough points to pay for blending them
+    long long rows = 0;
     FrameArgs f = {};
-    for (int i = 0; i < L * 3; i++) { f.row0[i] = rows; rows += T.w[i]; }
+    for (int i = 0; i < L * 3; i++) { f.row0[i] = (int)rows; rows += T.w[i]; }
     f.slice = C < 64 ? C : 64;
     while (f.slice > 4 && (size_t)rows * f.slice * sizeof(float) > 78 * 1024) f.slice >>= 1;
     const size_t lds = (size_t)rows * f.slice * sizeof(float);
     if (ft.stride == 0 && lds <= 78 * 1024 && (long long)P * C >= FRAME_LINES_MIN) {
         f.c = *c; f.L = L; f.C = C; f.nslices = C / f.slice; f.T = T; f.aabb = aabb; f.xyz = points; f.ft = ft; f.P = P; f.out = out; f.ld = ld;
         f.gshift = c->group == 32 ? 5 : c->group == 64 ? 6 : 7;
-        const long long ppw = 512 / (f.slice / 4), need = (P + ppw - 1) / ppw;
-        long long nwg = 512 / f.nslices;
-        if (nwg > need) nwg = need;
-        if (nwg >= 8) nwg = nwg / 8 * 8;
-        f.nwg = (int)(nwg < 1 ? 1 : nwg);
+        f.nwg = 512 / f.nslices;                          // 8 .. 512, and so many points are at least twice as many rounds
         auto go = [&](auto kern) -> int {
             if (lds > 64 * 1024) GS4D_HIP_CHECK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
             hipLaunchKernelGGL(kern, dim3((unsigned)(f.nwg * f.nslices)), dim3(512), lds, s, f);

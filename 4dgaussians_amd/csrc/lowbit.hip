@@ -51,21 +51,18 @@ __global__ __launch_bounds__(256) void rows8_write_kernel(gs4d_rows8 c, const T*
                                                           const S* __restrict__ slots, long long start, int cpr, int rpb, unsigned rcp, int lshift, int dup)
 {
     constexpr int COLS = 16 / (int)sizeof(T);
-    __shared__ long long s_slot[ROWS8_ROWS], s_all[GS4D_ROWS8_SCAN];
+    __shared__ long long s_slot[ROWS8_ROWS];
     const long long i0 = (long long)blockIdx.x * rpb;
     const int nrow = (int)min((long long)rpb, n - i0);
+    // few rows at given slots are one per workgroup, whose lanes look whether a later row has the same slot
+    bool later = false;
+    if (dup == 1) later = __syncthreads_or((int)threadIdx.x < n && (int)threadIdx.x > i0 && slots[min((int)threadIdx.x, (int)n - 1)] == slots[i0]);
     // where each row of this workgroup goes (-1: nowhere): one lane per row
-    if (dup == 1 && (int)threadIdx.x < n) s_all[threadIdx.x] = slots[threadIdx.x];
-    __syncthreads();
     if ((int)threadIdx.x < nrow) {
         const long long i = i0 + threadIdx.x;
         long long slot = slots ? (long long)slots[i] : start + i;
-        if (slot < 0 || slot >= c.capacity) slot = -1;
-        if (dup == 1) {                                   // few rows: does a later one have the same slot?
-            bool last = true;
-            for (int j = 0; j < (int)n; j++) last = last && (j <= (int)i || s_all[j] != slot);
-            if (!last) slot = -1;
-        } else if (dup == 2 && slot >= 0) {
+        if (slot < 0 || slot >= c.capacity || later) slot = -1;
+        if (dup == 2 && slot >= 0) {
             // rows8_owner_kernel left the last row's number.  It leaves the word zero again: a row that reads it later is not
             // the last one either way
             if (c.owner[slot] == (int)(i + 1)) c.owner[slot] = 0;
@@ -805,10 +802,18 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 }
 
 // A few rows (a single query): 16 lanes per feature read its weights once, 4 columns each, and multiply them with
-// all the rows.  No staging, so the latency is one round trip to memory (one row of 64 -> 64: 2.6 us, with the matrix cores 6.8).
+// all the rows.  No staging, so the latency is one round trip to memory (one row of 64 -> 64: 2.5 us, with the matrix cores 10).
+// These kernels take 1 us per 7 M products forward and per 16 M backward, the others have to split and stage the weight first, for
+// as long as some hundred rows take here: hence the rules.  Measured, these against those, in us: float32 forward 64 rows of 2048 ->
+// 1024 25 : 145, 2048 of 64 -> 512 20 : 27, 4096 of 64 -> 512 37 : 28; backward 1024 of 512 -> 512 18 : 30, 2048 33 : 31.  16-bit
+// forward 256 of 512 -> 512 13 : 18, 1024 of 64 -> 512 11 : 15, 2048 20 : 15, 4096 of 64 -> 64 7.0 : 6.3; backward 2048 of 512 -> 64
+// 9 : 19, 512 of 2048 -> 1024 71 : 40.
 #define FEW_ROWS 4            // per workgroup
-#define FEW_MOST 2048
-static bool few(int dtype, long long N, int K, int M) { return N <= FEW_MOST && N * K * M <= 1ll << (dtype == GS4D_F32 ? 28 : 27); }
+static bool few(int dtype, bool dx, long long N, int K, int M)
+{
+    if (dx) return N <= 4096 && (N - 200) * K * M <= 1ll << (dtype == GS4D_F32 ? 28 : 27);
+    return dtype == GS4D_F32 ? N <= 4096 && (N - 500) * K * M <= 1ll << 26 : N <= 2048 && (N - 200) * K * M <= 1ll << 25;
+}
 template <typename T>
 __global__ __launch_bounds__(256) void linear8_few_kernel(RowsArgs a)
 {
@@ -1255,6 +1260,7 @@ int gs4d_rows8_write(const gs4d_rows8* c, const void* rows, int dtype, long long
     if (check_rows(c, rows, dtype, ld, n, slots, slot_bytes, start, "gs4d_rows8_write")) return GS4D_EINVAL;
     if (n == 0) return GS4D_OK;
     if (too_many_rows(c, n, "gs4d_rows8_write")) return GS4D_EINVAL;
+    // rows for one slot: up to 256 rows each workgroup looks by itself (256 rows of 64: 3.2 us, with the owner array 5.2)
     const int dup = !slots || n == 1 ? 0 : n <= GS4D_ROWS8_SCAN ? 1 : 2;
     if (dup == 2 && !c->owner) { gs4d_set_error("gs4d_rows8_write: %lld rows at given slots need the cache's owner array", n); return GS4D_EINVAL; }
     const unsigned ogrid = (unsigned)((n + 255) / 256);
@@ -1319,7 +1325,8 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
 
 static int check_linear(int dtype, long long N, int K, int M, int fmt, const char* who)
 {
-    if (dtype < GS4D_F32 || dtype > GS4D_F16 || N < 0 || N > 2147483647ll || K < 1 || M < 1 || (long long)K * M > 1ll << 28 ||
+    if (dtype < GS4D_F32 || dtype > GS4D_F16 || N < 0 || N > 2147483647ll || K < 1 || M < 1 || K > 1 << 20 || M > 1 << 20 ||
+        (long long)K * M > 1ll << 28 ||
         fmt < GS4D_FMT_INT8 || fmt > GS4D_FMT_E5M2) {
         gs4d_set_error("%s: unsupported sizes or types", who);
         return GS4D_EINVAL;
@@ -1352,6 +1359,8 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
 {
     constexpr int LDS = 144 * 1024;
     const bool vec = a.C % 8 == 0;
+    // tiles per wave: as wide as the registers allow, so that the rows are read and split seldom (65536 x 512 -> 512 fp16: 4 tiles
+    // 71 us, 2 tiles 98), and no empty ones
     const int nt = sizeof(T) == 4 ? (a.F <= 32 ? 1 : 2) : a.F <= 64 ? 2 : 4;
     a.groups = (a.C + 63) / 64;
     const int per = 4 * nt * kTerms<T> * 1024;
@@ -1395,8 +1404,13 @@ static int launch_dw(DwArgs& a, int fmt, void* dw, void* db, hipStream_t s)
             constexpr int F = decltype(f)::value;
             auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3(grid), dim3(512), 0, s, a); };
             // 16-bit results: two terms of dy s (2^-16 of a product) where the float32 sum over the rows is itself no better
-            if (sizeof(T) == 2 && a.N >= 1024) { if (vec) go(linear8_dw_kernel<T, F, 2, true>); else go(linear8_dw_kernel<T, F, 2, false>); }
-            else { if (vec) go(linear8_dw_kernel<T, F, 3, true>); else go(linear8_dw_kernel<T, F, 3, false>); }
+            // (65536 x 512 -> 512 with its launches and host 185 us, with three terms 216; 1.2 M x 256 -> 64 240 : 266)
+            if constexpr (sizeof(T) == 2)
+                if (a.N >= 1024) {
+                    if (vec) go(linear8_dw_kernel<T, F, 2, true>); else go(linear8_dw_kernel<T, F, 2, false>);
+                    return 0;
+                }
+            if (vec) go(linear8_dw_kernel<T, F, 3, true>); else go(linear8_dw_kernel<T, F, 3, false>);
             return 0;
         });
     } else {
@@ -1430,7 +1444,7 @@ int gs4d_linear8_forward(int dtype, long long N, int K, int M, const void* x, lo
     if (what) a.keep = carve_keep(keep, N, K, what, nullptr);
     a.fmt = relu && fmt == GS4D_FMT_INT8 ? GS4D_FMT_UINT8 : fmt;
     const int rc = by_type(dtype, [&](auto t) {
-        if (few(dtype, N, K, M)) {
+        if (few(dtype, false, N, K, M)) {
             const unsigned keepers = what ? (unsigned)((FEW_ROWS * (a.keep.kp / 64) + 15) / 16) : 0;
             hipLaunchKernelGGL(linear8_few_kernel<decltype(t)>, dim3((unsigned)((M + 15) / 16) + keepers, (unsigned)((N + FEW_ROWS - 1) / FEW_ROWS)), dim3(256), 0, s, a);
             return GS4D_OK;
@@ -1462,7 +1476,7 @@ int gs4d_linear8_backward(int dtype, long long N, int K, int M, const void* dy, 
         a.lowest = (int)0x80000000;
         if (relu) a.keep = kp;
         rc = by_type(dtype, [&](auto t) {
-            if (few(dtype, N, K, M)) {
+            if (few(dtype, true, N, K, M)) {
                 hipLaunchKernelGGL(linear8_few_dx_kernel<decltype(t)>, dim3((unsigned)((K + 63) / 64), (unsigned)((N + FEW_ROWS - 1) / FEW_ROWS)), dim3(256), 0, s, a);
                 return GS4D_OK;
             }

@@ -133,14 +133,12 @@ class RowCache:
             rows = rows.contiguous()
         ref = self._ref
         if slots is not None and n > SCAN:
-            if self._owner is not None:
-                pass
-            elif torch.cuda.is_current_stream_capturing():
-                # its zeros are written when the graph runs, not now: an array of the graph's own
+            if torch.cuda.is_current_stream_capturing():
+                # an array of the graph's own: its zeros are written when the graph runs, and it lives as long as the graph
                 owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
                 d = Rows8.from_buffer_copy(self._desc)
                 d.owner, ref = owner.data_ptr(), C.addressof(d)
-            else:
+            elif self._owner is None:
                 self._owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
                 self._desc.owner = self._owner.data_ptr()
         with _cabi.on_device(self.device):
@@ -272,7 +270,7 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
     """act(x) @ weight.T + bias with act = relu or nothing: x [..., K], weight [M, K], bias [M], all of one dtype (float32,
     bfloat16 or float16; sums in float32).  For the backward it keeps act(x) in 8 bits in groups of 64 columns ("int8": 255
     levels of a rectified input, 127 each way of a signed one) and, with relu, the signs of x -- a byte or so per number
-    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  At most 2^28 weights."""
+    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  At most 2^28 weights, K and M at most 2^20."""
     f = _format(fmt)
     _on_device("x", x)
     _on_device("weight", weight, x.device)

@@ -670,7 +670,7 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
 
 /*
  * y [N][M] = act(x) w^T + b, x [N] rows of K with a pitch of ldx elements, w [M][K], b [M] or NULL, act = relu or nothing; all
- * of one dtype, sums in float32, K * M at most 2^28.  The backward does not need x: `keep` (gs4d_linear8_keep_bytes, 256-byte aligned) receives
+ * of one dtype, sums in float32, K and M at most 2^20, K * M at most 2^28.  The backward does not need x: `keep` (gs4d_linear8_keep_bytes, 256-byte aligned) receives
  *   GS4D_KEEP_CODES  act(x) in 8 bits in groups of 64 columns (int8 becomes uint8 with relu): the weight gradient's operand
  *   GS4D_KEEP_SIGNS  a bit per value, x > 0 (relu only): the input gradient's mask
  * as `what` says (0: nothing, keep may be NULL).

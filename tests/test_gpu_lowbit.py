@@ -209,6 +209,40 @@ def test_a_cache_captured_before_its_first_write():
         same(c.read(), want)
 
 
+def test_a_captured_write_outlives_its_cache_object():
+    """The caller keeps codes and scales; the graph must not use an array that goes with the cache object."""
+    codes, scales = torch.zeros(500, 64, dtype=torch.uint8, device="cuda"), torch.zeros(500, 1, device="cuda")
+    x = rows(1000, 64).cuda()
+    slots = torch.randint(0, 500, (1000,), generator=torch.Generator().manual_seed(1)).cuda()
+    want = f32(R.write(np.zeros((500, 64)), np64(x), slots.tolist(), "int8", 64))
+    c = lb().RowCache.from_buffers(codes, scales, 64)
+    c.write(x, slots)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.write(x, slots)
+    torch.cuda.synchronize()
+    del c
+    others = [torch.full((500,), 2 ** 30, dtype=torch.int32, device="cuda") for _ in range(64)]       # who may have the memory now
+    for _ in range(3):
+        codes.zero_()
+        graph.replay()
+        same(lb().RowCache.from_buffers(codes, scales, 64).read(), want)
+        assert all((o == 2 ** 30).all().item() for o in others)
+
+
+@pytest.mark.parametrize("size", [torch.int32, torch.int64])
+@pytest.mark.parametrize("n", [2, 63, 255, 256, 257, 511, 513])
+def test_the_last_of_several_rows_for_one_slot(n, size):
+    for capacity in (1, 5, n):
+        x = rows(n, 40, seed=n)
+        slots = torch.randint(-1, capacity + 1, (n,), generator=torch.Generator().manual_seed(n), dtype=size)
+        c = lb().RowCache(capacity, 40, group=32)
+        c.write(torch.zeros(capacity, 40, device="cuda"))
+        for _ in range(2):
+            c.write(x.cuda(), slots.cuda())
+            same(c.read(), f32(R.write(np.zeros((capacity, 40)), np64(x), slots.tolist(), "int8", 32)))
+
+
 # ------------------------------------------------------------------------------------------ frame features
 @pytest.mark.parametrize("levels,ch,res,res_t,n", [(1, 4, 5, 2, 1), (2, 32, 9, 7, 300), (1, 16, 1, 1, 65), (4, 8, 6, 3, 77), (2, 128, 12, 5, 130),
                                                    (1, 256, 4, 4, 9)])
@@ -255,6 +289,31 @@ def test_frame_features_of_many_points(levels, ch, res, res_t, n, fmt):
         assert np.abs(np64(got) / want - 1).max() <= tol
         each = lb().frame_features(c, *args, t.expand(n).contiguous().cuda())
         assert np.abs(np64(each) / want - 1).max() <= tol             # a value per point: the other kernel
+
+
+@pytest.mark.parametrize("levels,ch,res,res_t,n", [(2, 32, 64, 75, 65_537), (2, 128, 128, 25, 16_385), (1, 256, 9, 3, 8192),
+                                                   (1, 256, 1500, 2, 8200), (3, 64, 300, 6, 32_771), (4, 16, 30, 9, 131_100), (1, 4, 3, 1, 524_289)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_frame_features_from_blended_lines(levels, ch, res, res_t, n, fmt):
+    """A frame of so many points that the lines of its one t are blended first; against the kernel for a t per point and, at some
+    points, the definition."""
+    g = torch.Generator().manual_seed(n)
+    static = 0.1 + torch.rand(n, levels * ch, generator=g) * 2
+    c = lb().RowCache(n, levels * ch, fmt, 64)
+    c.write(static.cuda())
+    planes = [(0.5 + torch.rand(1, res_t, res << (lv % 2), ch, generator=g)).permute(0, 3, 1, 2) for lv in range(levels) for _ in range(3)]
+    aabb = torch.tensor([[1.3, 1.2, 1.1], [-1.3, -1.2, -1.0]])
+    pts = (torch.rand(n, 3, generator=g) * 2 - 1) * 1.6
+    args = [p.cuda() for p in planes], aabb.cuda(), pts.cuda()
+    at = torch.cat([torch.arange(600), torch.arange(n - 600, n), torch.randint(0, n, (800,), generator=g)])
+    held = R.quantise(np64(static[at]), fmt, 64)[0]
+    tol = (12 * 8 * 4 * max(2 * res, res_t) + 20) * 2.0 ** -24        # as above
+    for t in (torch.tensor([0.3721]), torch.tensor([1.0]), torch.tensor([-2.0])):
+        got = lb().frame_features(c, *args, t.cuda())
+        want = R.frame_features(held, [p[0].numpy() for p in planes], aabb.numpy(), pts[at].numpy(), t.expand(len(at)).numpy())
+        assert np.abs(np64(got.cpu()[at]) / want - 1).max() <= tol
+        each = lb().frame_features(c, *args, t.expand(n).contiguous().cuda())
+        assert (got / each - 1).abs().max().item() <= 2 * tol         # every point: two results within tol of one number
 
 
 def test_frame_features_refuses():
@@ -508,6 +567,13 @@ def test_linear_replays_in_every_form(n, k, m, dtype):
                                    (2500, 9, 3), (2500, 1, 1), (2304, 100, 400), (2304, 576, 130)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_on_both_sides_of_every_rule(n, k, m, dtype):
+    check_linear(*make(n, k, m, dtype), True, "int8")
+
+
+@pytest.mark.parametrize("n,k,m", [(4096, 64, 64), (4097, 64, 64), (1524, 256, 256), (1525, 256, 256), (712, 256, 256), (713, 256, 256),
+                                   (712, 512, 512), (713, 512, 512), (1224, 512, 512), (1225, 512, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_on_both_sides_of_the_rules_for_few_rows(n, k, m, dtype):
     check_linear(*make(n, k, m, dtype), True, "int8")
 
 

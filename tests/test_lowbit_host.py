@@ -119,3 +119,14 @@ def test_oracle_is_within_half_a_step_and_idempotent(fmt):
         q = t.to(torch.float8_e4m3fn if fmt == "e4m3" else torch.float8_e5m2).double().numpy()
         s = (np.abs(x[:, :64]).max(axis=1, keepdims=True) / np.float32(R.TOP[fmt])).astype(np.float64)
         assert (q * s == v[:, :64]).all()
+
+
+@pytest.mark.parametrize("k, m", [(1, (1 << 20) + 1), ((1 << 20) + 1, 1), (1, 1 << 28), (1 << 28, 1)])
+def test_linear_refuses_one_very_long_dimension(lb, k, m):
+    """Few weights, but eight rows of M or K elements no longer have 32-bit offsets."""
+    L = pkg("_cabi").lib()
+    p, z = C.c_void_p(4096), C.c_void_p(0)
+    assert L.gs4d_linear8_forward(C.c_int(0), C.c_longlong(4), C.c_int(k), C.c_int(m), p, C.c_longlong(k), p, z, C.c_int(0), C.c_int(0),
+                                  p, z, C.c_int(0), z) == -1
+    assert L.gs4d_linear8_backward(C.c_int(0), C.c_longlong(4), C.c_int(k), C.c_int(m), p, p, C.c_int(0), C.c_int(0), p, C.c_int(1),
+                                   z, p, z, p, z) == -1
