@@ -68,7 +68,7 @@ class HexOrderCache:
         if self.refresh <= 0 or P == 0:
             g.hex_order, g.hex_order_valid = None, 0
             return
-        key = (P, L, dev.index, rows)
+        key = (P, L, dev.index) if rows == P else (P, L, dev.index, rows)
         e = self.entries.get(key)
         if e is None:
             if len(self.entries) >= 4:
