@@ -7,9 +7,8 @@
 // opacity (1).
 //
 // The reference issues 10 global float atomics per contributing (pixel, Gaussian) pair.  Here:
-//  * a workgroup is two wave64; every lane owns TWO horizontally adjacent pixels, so the per-pair
-//    arithmetic runs on the packed-fp32 instructions (v_pk_fma/mul/add_f32: both pixels per issue) --
-//    this kernel is bound by VALU issue, not by memory;
+//  * a workgroup is two wave64; every lane owns TWO horizontally adjacent pixels, so that one pass
+//    over the list serves both -- this kernel is bound by VALU issue, not by memory;
 //  * a pixel that does not blend a Gaussian is not branched around: its alpha and G are replaced by 0,
 //    which turns every state update into the exact identity (T/(1-0), 0*c + 1*acc) and every gradient
 //    term into 0, so the two pixels of a lane never diverge;
@@ -60,8 +59,7 @@ __device__ __forceinline__ float row16_sum(float v)
     return v;
 }
 
-// the same for three values at once, as fused DPP adds (left to itself the compiler pairs two of the three into
-// v_pk_add_f32, which cannot take a DPP operand, and spends 5 instructions per step on moves).  A DPP read of a
+// the same for three values at once, as fused DPP adds.  A DPP read of a
 // register needs two wait states after the VALU write of it: s_nop 1 in front, and within the block every value is
 // touched again only after the other two.
 __device__ __forceinline__ void row16_sum3(float& a, float& b, float& c)

@@ -8,8 +8,8 @@
 //
 // gfx950 design:
 //  * one workgroup = one tile = 2 wave64; a wave owns 8 rows x 16 columns and every lane TWO
-//    horizontally adjacent pixels, so the per-pair arithmetic runs on the packed-fp32 instructions
-//    (v_pk_fma/mul/add_f32: both pixels per issue) -- the kernel is bound by VALU issue, not memory;
+//    horizontally adjacent pixels, so that one pass over the list (its LDS reads, culling and loop control)
+//    serves both -- the kernel is bound by VALU issue, not memory;
 //  * a pixel that does not blend a Gaussian runs the same arithmetic with alpha = 0 (exact identity:
 //    w = 0, T * (1 - 0)), so the two pixels of a lane never diverge;
 //  * each batch of 256 list entries is gathered ONCE per tile into LDS as three arrays

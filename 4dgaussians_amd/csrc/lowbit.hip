@@ -454,7 +454,9 @@ __device__ __forceinline__ void positive_nans(Group<T>& g)
 //   ROWS_WIDE  one group, several column blocks: the group's operands stay in registers for all of them
 //   ROWS_MANY  several groups: the next one is in flight while this one is multiplied, 8 waves (1.2 M x 256: 463 us; 16 waves
 //              without the prefetch 503)
-enum { ROWS_ONE, ROWS_WIDE, ROWS_MANY };
+//   ROWS_SPLIT several groups, few rows: the waves of a workgroup share a tile of rows, each takes groups of it, and the sums meet in
+//              LDS (SPLIT)
+enum { ROWS_ONE, ROWS_WIDE, ROWS_MANY, ROWS_SPLIT };
 template <typename T, int NT, bool VEC, int MODE> constexpr int kRowsThreads = VEC && NT <= 2 && MODE == ROWS_ONE ? 1024 : 512;
 
 struct RowsArgs {
@@ -480,7 +482,9 @@ template <typename T, int NT, bool VEC, bool DX, int MODE>
 __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows_kernel(RowsArgs a)
 {
     constexpr int TERMS = kTerms<T>, THREADS = kRowsThreads<T, NT, VEC, MODE>, WAVES = THREADS / 64, BLOCK = 4 * NT * TERMS * 64;
-    extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane]
+    constexpr bool SPLIT = MODE == ROWS_SPLIT;
+    constexpr int PAIR = NT < 2 ? NT : 2;                 // tiles whose results leave together
+    extern __shared__ uint4 s_w[];                        // [group][step][tile][term][lane], SPLIT: then [wave][tile of a pair][register][lane] of sums
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, h = lane >> 5;
     // workgroups that share rows differ by 8 in their number, i.e. run on one XCD behind one L2
     int cb, wg;
@@ -500,7 +504,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     auto feature = [&](int nt, int l) { return f0 + (sizeof(T) == 4 ? nt * 32 + l : (nt >> 1) * 64 + 2 * l + (nt & 1)); };
     auto stage = [&](int g0, int n, uint4* s_w) {         // groups g0 .. g0 + n - 1 of the weight, for the features from f0 on
         // U items at a time, their loads in flight together: one after the other, a 512 x 512 weight took 35 us to arrive
-        constexpr int U = MODE == ROWS_MANY ? 4 : 1;     // (one group is few rounds, and the registers are worth more: 405 us, not 460)
+        constexpr int U = MODE == ROWS_MANY || SPLIT ? 4 : 1;     // (one group is few rounds, and the registers are worth more: 405 us, not 460)
         const int total = n * 4 * NT * 64;
         for (int e0 = tid; e0 < total; e0 += THREADS * U) {
             unsigned v[U][8];
@@ -571,12 +575,13 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     const int ntile = (int)((a.N + 31) >> 5);
     const bool keeping = !DX && cb == 0 && (a.keep.codes || a.keep.bits);
     auto row_of = [&](long long tile) { const long long r = tile * 32 + j; return X + (r < a.N ? r : a.N - 1) * a.ldx; };
-    long long tile = (long long)wave * a.nwg + wg;
+    long long tile = SPLIT ? wg : (long long)wave * a.nwg + wg;
+    constexpr int TILES = SPLIT ? 1 : WAVES;              // per workgroup and round
     Group<T> cur;
     // the waves start at different groups: a row of several 256-byte groups, read by all waves in step, would keep to a fraction of
     // the memory channels at a time
-    const int turn = a.chunk >= a.groups ? wave % a.groups : 0;
-    auto group_at = [&](int gi) { const int g = gi + turn; return g < a.groups ? g : g - a.groups; };
+    const int turn = SPLIT ? wave : a.chunk >= a.groups ? wave % a.groups : 0;
+    auto group_at = [&](int gi) { const int g = gi + turn; return SPLIT || g < a.groups ? g : g - a.groups; };
     load_group<T, VEC>(cur, row_of(tile), turn * 64 + 8 * h, C, end);      // in flight while the weight is staged
     if constexpr (MODE == ROWS_WIDE) {
         for (int k = 0; k < a.blocks; k++) { stage(0, 1, s_w + k * BLOCK); f0 += NT * 32; }
@@ -585,7 +590,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
         stage(0, a.groups, s_w);
     }
     __syncthreads();
-    for (long long base = 0; base * a.nwg < ntile; base += WAVES, tile += (long long)WAVES * a.nwg) {      // uniform: every wave takes part in the barriers
+    for (long long base = 0; base * a.nwg < ntile; base += TILES, tile += (long long)TILES * a.nwg) {      // uniform: every wave takes part in the barriers
         const long long row = tile * 32 + j;
         const bool live = row < a.N;
         f32x16 acc[NT];
@@ -593,7 +598,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
         auto begin = [&]() {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float b = !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt, j), F - 1)]) : 0.f;
+                const float b = !SPLIT && !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt, j), F - 1)]) : 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; r++) acc[nt][r] = b;
             }
@@ -616,46 +621,76 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
         };
-        // register r is the row (r & 3) + 8 (r >> 2) + 4 h of the tile
+        // register r is the row rr + 4 h of the tile, rr = (r & 3) + 8 (r >> 2); o: its results of the tiles nt, nt + 1
+        auto put = [&](T* __restrict__ yt, bool whole, int rr, int nt, const float (&o)[PAIR]) {
+            if (!whole && tile * 32 + rr + 4 * h >= a.N) return;
+            T* __restrict__ y = yt + (long long)rr * F + feature(nt, j);
+            if constexpr (sizeof(T) == 2) {
+                const T two[2] = {lb_store<T>(o[0]), lb_store<T>(o[1])};
+                if (feature(nt, j) + 1 < F) __builtin_memcpy(y, two, 4);
+                else if (feature(nt, j) < F) *y = two[0];
+            } else {
+#pragma unroll
+                for (int u = 0; u < PAIR; u++)
+                    if (feature(nt + u, j) < F) y[32 * u] = o[u];
+            }
+        };
         auto finish = [&]() {
             const bool whole = tile * 32 + 32 <= a.N;
-            T* __restrict__ y = (T*)a.y + (tile * 32 + 4 * h) * F;
-            const bool pairs = sizeof(T) == 2 && (F & 1) == 0 && ((uintptr_t)a.y & 3) == 0;
+            T* __restrict__ yt = (T*)a.y + (tile * 32 + 4 * h) * F;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int rr = (r & 3) + 8 * (r >> 2);
-                if (!whole && tile * 32 + rr + 4 * h >= a.N) continue;
-                float o[NT];
+            for (int r = 0; r < 16; r++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    o[nt] = acc[nt][r];
-                    if (DX && a.keep.bits) {
-                        const unsigned long long lanes = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(sign[nt], rr + 4) << 32 | (unsigned)__builtin_amdgcn_readlane(sign[nt], rr);
-                        o[nt] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? o[nt] : 0.f;
+                for (int nt = 0; nt < NT; nt += PAIR) {
+                    float o[PAIR];
+#pragma unroll
+                    for (int u = 0; u < PAIR; u++) {
+                        o[u] = acc[nt + u][r];
+                        if (DX && a.keep.bits) {
+                            const int rr = (r & 3) + 8 * (r >> 2);
+                            const unsigned long long lanes = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(sign[nt + u], rr + 4) << 32 | (unsigned)__builtin_amdgcn_readlane(sign[nt + u], rr);
+                            o[u] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? o[u] : 0.f;
+                        }
                     }
+                    put(yt, whole, (r & 3) + 8 * (r >> 2), nt, o);
                 }
-                T* __restrict__ yr = y + (long long)rr * F;
-                if (pairs) {
+        };
+        // the waves' sums of a pair of tiles side by side in LDS, then two of the 16 registers per wave
+        auto join = [&]() {
+            const bool whole = tile * 32 + 32 <= a.N;
+            T* __restrict__ yt = (T*)a.y + (tile * 32 + 4 * h) * F;
+            float* __restrict__ part = reinterpret_cast<float*>(s_w + (size_t)a.groups * BLOCK);
+            const int parts = min(a.groups, WAVES);
 #pragma unroll
-                    for (int nt = 0; nt + 1 < NT; nt += 2) {
-                        const T two[2] = {lb_store<T>(o[nt]), lb_store<T>(o[nt + 1])};
-                        unsigned w;
-                        __builtin_memcpy(&w, two, 4);
-                        if (feature(nt, j) < F) *reinterpret_cast<unsigned*>(yr + feature(nt, j)) = w;
+            for (int nt = 0; nt < NT; nt += PAIR) {
+                if (wave < parts) {
+#pragma unroll
+                    for (int u = 0; u < PAIR; u++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) part[((wave * PAIR + u) * 16 + r) * 64 + lane] = acc[nt + u][r];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < 16 / WAVES; k++) {
+                    const int r = wave * (16 / WAVES) + k, rr = (r & 3) + 8 * (r >> 2);
+                    float o[PAIR];
+#pragma unroll
+                    for (int u = 0; u < PAIR; u++) {
+                        o[u] = !DX && a.bias ? lb_load(((const T*)a.bias)[min(feature(nt + u, j), F - 1)]) : 0.f;
+                        for (int q = 0; q < parts; q++) o[u] += part[((q * PAIR + u) * 16 + r) * 64 + lane];
+                        if (DX && a.keep.bits) o[u] = (unsigned)__shfl((int)sign[nt + u], rr + 4 * h, 64) >> j & 1u ? o[u] : 0.f;
                     }
-                } else {
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        if (feature(nt, j) < F) yr[feature(nt, j)] = lb_store<T>(o[nt]);
+                    put(yt, whole, rr, nt, o);
                 }
+                __syncthreads();
             }
         };
         if (MODE != ROWS_WIDE) begin();
-        for (int gi = 0; gi < a.groups; gi++) {
+        for (int gi = 0; gi < (SPLIT ? a.groups - wave : a.groups); gi += SPLIT ? WAVES : 1) {
             const int g = group_at(gi);
             int Cn = a.C;
             asm("" : "+s"(Cn));                           // column limits are recomputed: kept over the loop they would spill
-            if (a.chunk < a.groups && gi % a.chunk == 0) {
+            if (!SPLIT && a.chunk < a.groups && gi % a.chunk == 0) {
                 __syncthreads();
                 stage(gi, min(a.chunk, a.groups - gi), s_w);
                 __syncthreads();
@@ -664,10 +699,11 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 if (!VEC) fix_end(cur, row_of(tile), g * 64 + 8 * h, Cn, end);
                 clear_past(cur, g * 64 + 8 * h, Cn);
             }
-            const uint4* __restrict__ wl = s_w + (size_t)(a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
-            const bool more = gi + 1 < a.groups;
+            const uint4* __restrict__ wl = s_w + (size_t)(!SPLIT && a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
+            constexpr int NEXT = SPLIT ? WAVES : 1;
+            const bool more = SPLIT ? g + NEXT < a.groups : gi + 1 < a.groups;
             Group<T> nxt;
-            if (MODE == ROWS_MANY) load_group<T, VEC>(nxt, row_of(more ? tile : tile + (long long)WAVES * a.nwg), group_at(more ? gi + 1 : 0) * 64 + 8 * h, Cn, end);
+            if (MODE == ROWS_MANY || SPLIT) load_group<T, VEC>(nxt, row_of(more ? tile : tile + (long long)TILES * a.nwg), group_at(more ? gi + NEXT : 0) * 64 + 8 * h, Cn, end);
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
             float v[4][8];
@@ -789,7 +825,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                     else xs[0] = cur.w[t];
                     step(xs, wl + t * NT * TERMS * 64);
                 }
-                if (MODE == ROWS_MANY) {
+                if (MODE == ROWS_MANY || SPLIT) {
                     cur = nxt;
                 } else {
                     __builtin_amdgcn_sched_barrier(0);
@@ -797,7 +833,8 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 }
             }
         }
-        if (MODE != ROWS_WIDE) finish();
+        if constexpr (SPLIT) join();
+        else if (MODE != ROWS_WIDE) finish();
     }
 }
 
@@ -947,7 +984,9 @@ __global__ __launch_bounds__(256) void linear8_few_dx_kernel(RowsArgs a)
 // Tile t of the result then holds the columns 2 i + t.  The codes are exact in bfloat16 (8 significant bits), so the rounding
 // lies in dy s alone, which is split into TERMS bfloat16 numbers: three are its 24 bits.
 // A workgroup: 64 columns m, GW groups of 64 columns k (a wave each) and 8 / GW row slices per group, summed through LDS;
-// one slab of partial sums per workgroup.
+// one slab of partial sums per workgroup.  Bound by the vector instructions that form and split dy s, once per group of columns:
+// 180 of them and 12 MFMAs a step of 16 rows (float32, int8).  1.2 M x 256 -> 64: 238 us (reading once: 135), 65536 x 512 -> 512
+// fp16 118 us, 100 k x 64 -> 64 12 us.
 struct DwArgs {
     long long N; int K, M;
     const void* dy; Keep keep;
@@ -955,6 +994,12 @@ struct DwArgs {
     int gw, groups, mtiles, chunks;
     float* slabs;                         // [chunk][m tile][group][64 registers][64 lanes], then [chunk][m tile][64] of db
 };
+
+// lane Q of the lane's 16
+template <int Q> __device__ __forceinline__ float row_lane(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + Q, 0xF, 0xF, true));
+}
 
 template <typename T, int FMT, int TERMS, bool VEC>
 __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
@@ -975,14 +1020,18 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
     const float* __restrict__ scales = a.keep.scales + gc;
     // a load's address is the wave's row plus the lane's share, which does not change
     const unsigned dlane = (unsigned)((8 * h * M + mc) * (int)sizeof(T)), clane = (unsigned)(8 * h * kp + 2 * i);
-    struct Rows { unsigned d[8][sizeof(T) / 2]; unsigned short c[8]; float lo[8], hi[8]; };
+    struct Rows { unsigned d[8][sizeof(T) / 2]; unsigned short c[8]; float s; };
     // rows r0 + 8 h + q; LAST: some of them may lie past the end
     auto load = [&](Rows& r, long long r0, auto last) {
         constexpr bool LAST = decltype(last)::value != 0;
+        unsigned dl = dlane, cl = clane;
+        asm("" : "+v"(dl), "+v"(cl));                     // no address kept over the loop: the row's part stays scalar, the lane's 32 bits
 #pragma unroll
         for (int q = 0; q < 8; q++) {
-            const char* pd = reinterpret_cast<const char*>(dy + (r0 + q) * M) + dlane;
-            const char* pc = reinterpret_cast<const char*>(codes + (r0 + q) * kp) + clane;
+            const char* pd = reinterpret_cast<const char*>(dy + (r0 + q) * M);
+            const char* pc = reinterpret_cast<const char*>(codes + (r0 + q) * kp);
+            pd += dl;
+            pc += cl;
             if (LAST && r0 + 8 * h + q >= a.N) {          // the last row instead
                 pd = reinterpret_cast<const char*>(dy + (a.N - 1) * M + mc);
                 pc = reinterpret_cast<const char*>(codes + (a.N - 1) * kp + 2 * i);
@@ -997,28 +1046,37 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
             }
             r.c[q] = *reinterpret_cast<const unsigned short*>(pc);
         }
-        // the scales are the same for 32 lanes: scalar loads, one of two per lane
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-            const long long u = r0 + q < a.N ? r0 + q : a.N - 1, v = r0 + 8 + q < a.N ? r0 + 8 + q : a.N - 1;
-            r.lo[q] = scales[(LAST ? u : r0 + q) * ng];
-            r.hi[q] = scales[(LAST ? v : r0 + 8 + q) * ng];
-        }
+        // lane q of 16 has the scale of row r0 + 8 h + q (q < 8), broadcast where it is used.  (As scalar loads, which return in any
+        // order, they made each step wait for the loads of the next: 1.2 M x 256 -> 64 292 us.)
+        const long long n = r0 + 8 * h + (lane & 7);
+        r.s = scales[(LAST && n >= a.N ? a.N - 1 : n) * ng];
+        if (LAST && n >= n1) r.s = 0.f;
     };
     f32x16 acc[2][2] = {};
     float db0 = 0.f, db1 = 0.f;
+    int turn = wave % a.gw;
     auto add = [&](const Rows& cur, long long r0, auto last) {
         constexpr bool LAST = decltype(last)::value != 0;
         float d0[8], d1[8], c0[8], c1[8];
+        const float sq[8] = {row_lane<0>(cur.s), row_lane<1>(cur.s), row_lane<2>(cur.s), row_lane<3>(cur.s),
+                             row_lane<4>(cur.s), row_lane<5>(cur.s), row_lane<6>(cur.s), row_lane<7>(cur.s)};
 #pragma unroll
         for (int q = 0; q < 8; q++) {
-            float s = h ? cur.hi[q] : cur.lo[q];
             if constexpr (sizeof(T) == 4) { d0[q] = __uint_as_float(cur.d[q][0]); d1[q] = __uint_as_float(cur.d[q][1]); }
             else { d0[q] = low16<T>(cur.d[q][0]); d1[q] = high16<T>(cur.d[q][0]); }
             if (VEC) d0[q] = shifted ? d1[q] : d0[q];
-            if (LAST && r0 + 8 * h + q >= n1) { d0[q] = 0.f; d1[q] = 0.f; s = 0.f; }
-            if (g == 0) { db0 += d0[q]; db1 += d1[q]; }
-            d0[q] *= s; d1[q] *= s;
+            if (LAST && r0 + 8 * h + q >= n1) { d0[q] = 0.f; d1[q] = 0.f; }
+        }
+        // the groups' waves of a slice take turns at the column sums of dy
+        if (turn == 0) {
+            asm volatile("");                             // a branch: as selects the sums would be formed by all
+#pragma unroll
+            for (int q = 0; q < 8; q++) { db0 += d0[q]; db1 += d1[q]; }
+        }
+        turn = turn == 0 ? a.gw - 1 : turn - 1;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            d0[q] *= sq[q]; d1[q] *= sq[q];
             if constexpr (FMT == GS4D_FMT_E4M3 || FMT == GS4D_FMT_E5M2) {
                 const float4 f = lb_decode4<FMT>(cur.c[q]);
                 c0[q] = f.x; c1[q] = f.y;
@@ -1042,7 +1100,7 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
         const long long stride = 16ll * slices, end = n1 - 15;
         long long r0 = n0 + 16 * slice;
         if (r0 < end) {
-            // three steps in flight: with one, a step took as long as its loads (4900 cycles for 2900 of work)
+            // three steps in flight: with one, a step took as long as its loads (1.2 M x 256 -> 64 358 us, with three 280 at that time)
             Rows ring[3];
             load(ring[0], r0, Int<0>());
             load(ring[1], r0 + stride < end ? r0 + stride : r0, Int<0>());
@@ -1096,14 +1154,14 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
 #pragma unroll
                 for (int r = 0; r < 16; r++) p[((t * 2 + y) * 16 + r) * 64 + lane] = acc[t][y][r];
     }
-    if (z == 0) {                                         // db: the waves of group 0 have the column sums of their slices
+    if (z == 0) {                                         // db: each of the 8 waves has the column sums of its turns
         db0 += __shfl_xor(db0, 32, 64);
         db1 += __shfl_xor(db1, 32, 64);
         if (h == 0) { s_db[wave][2 * i] = db0; s_db[wave][2 * i + 1] = db1; }
         __syncthreads();
         if (tid < 64) {
             float s = 0.f;
-            for (int q = 0; q < slices; q++) s += s_db[q * a.gw][tid];
+            for (int q = 0; q < 8; q++) s += s_db[q][tid];
             a.slabs[(size_t)a.chunks * a.mtiles * a.groups * 4096 + cell * 64 + tid] = s;
         }
     }
@@ -1114,35 +1172,36 @@ template <typename T>
 __global__ __launch_bounds__(512) void linear8_db_kernel(DwArgs a)
 {
     __shared__ float s_db[8][64];
-    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, i = lane & 31, h = lane >> 5, slices = 8 / a.gw;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 31, h = lane >> 5;
     const int chunk = blockIdx.x % a.chunks, mt = blockIdx.x / a.chunks;
     const long long n0 = chunk * a.per, n1 = n0 + a.per < a.N ? n0 + a.per : a.N;
     const int m0 = min(mt * 64 + 2 * i, a.M - 1), m1 = min(mt * 64 + 2 * i + 1, a.M - 1);
     const T* __restrict__ dy = (const T*)a.dy;
     float d0 = 0.f, d1 = 0.f;
-    if (slice < slices)
-        for (long long r0 = n0 + 16 * slice; r0 < n1; r0 += 16ll * slices) {
-            float v0[8], v1[8];
+    // wave slice * gw + turn of 8: the steps of its slice, every gw-th from `turn` on
+    const int slices = 8 / a.gw, slice = wave / a.gw, turn = wave % a.gw;
+    for (long long r0 = n0 + 16 * (slice + (long long)slices * turn); r0 < n1; r0 += 128) {
+        float v0[8], v1[8];
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const long long n = r0 + 8 * h + q, row = n < a.N ? n : a.N - 1;
-                v0[q] = lb_load(dy[row * a.M + m0]);
-                v1[q] = lb_load(dy[row * a.M + m1]);
-            }
-#pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const bool in = r0 + 8 * h + q < n1;
-                d0 += in ? v0[q] : 0.f;
-                d1 += in ? v1[q] : 0.f;
-            }
+        for (int q = 0; q < 8; q++) {
+            const long long n = r0 + 8 * h + q, row = n < a.N ? n : a.N - 1;
+            v0[q] = lb_load(dy[row * a.M + m0]);
+            v1[q] = lb_load(dy[row * a.M + m1]);
         }
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const bool in = r0 + 8 * h + q < n1;
+            d0 += in ? v0[q] : 0.f;
+            d1 += in ? v1[q] : 0.f;
+        }
+    }
     d0 += __shfl_xor(d0, 32, 64);
     d1 += __shfl_xor(d1, 32, 64);
-    if (h == 0) { s_db[slice][2 * i] = d0; s_db[slice][2 * i + 1] = d1; }
+    if (h == 0) { s_db[wave][2 * i] = d0; s_db[wave][2 * i + 1] = d1; }
     __syncthreads();
     if (threadIdx.x < 64) {
         float s = 0.f;
-        for (int q = 0; q < slices; q++) s += s_db[q][threadIdx.x];
+        for (int q = 0; q < 8; q++) s += s_db[q][threadIdx.x];
         a.slabs[((size_t)chunk * a.mtiles + mt) * 64 + threadIdx.x] = s;
     }
 }
@@ -1367,11 +1426,16 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
     a.chunk = LDS / per < a.groups ? LDS / per : a.groups;
     // a contraction of one group: a workgroup takes as many of the column blocks as its LDS holds (a row's result in one go)
     const int all = (a.F + nt * 32 - 1) / (nt * 32);
-    const int mode = a.groups > 1 ? ROWS_MANY : all > 1 ? ROWS_WIDE : ROWS_ONE;
+    const long long ntile = (a.N + 31) / 32;
+    const size_t joined = (size_t)(a.groups < 8 ? a.groups : 8) * (nt < 2 ? nt : 2) * 4096;
+    // up to two rounds of tiles (float32; one and a bit for the 16-bit types, whose groups are shorter work), measured against ROWS_MANY:
+    // float32 8192 x 256 -> 64 15 us against 23, 16384 19 against 23, 32768 26 against 25; bf16 8192 x 384 -> 128 12 against 16, 16384 the same
+    const bool split = a.groups > 1 && ntile * 4 <= (sizeof(T) == 4 ? 8 : 5) * (LB_CUS / all) && (size_t)a.groups * per + joined <= 160 * 1024;
+    const int mode = split ? ROWS_SPLIT : a.groups > 1 ? ROWS_MANY : all > 1 ? ROWS_WIDE : ROWS_ONE;
     a.blocks = mode == ROWS_WIDE ? (LDS / per < all ? LDS / per : all) : 1;
     a.ncb = (all + a.blocks - 1) / a.blocks;
-    const size_t lds = (size_t)a.chunk * a.blocks * per;
-    const long long ntile = (a.N + 31) / 32;
+    if (split) a.chunk = a.groups;
+    const size_t lds = (size_t)a.chunk * a.blocks * per + (split ? joined : 0);
     auto launch = [&](auto n, auto v, auto o) {
         constexpr int THREADS = kRowsThreads<T, decltype(n)::value, decltype(v)::value != 0, decltype(o)::value>;
         auto k = linear8_rows_kernel<T, decltype(n)::value, decltype(v)::value != 0, DX, decltype(o)::value>;
@@ -1386,7 +1450,7 @@ static int launch_rows(RowsArgs& a, hipStream_t s)
         return GS4D_OK;
     };
     auto with_nt = [&](auto n) {
-        auto with_mode = [&](auto v) { return mode == ROWS_MANY ? launch(n, v, Int<ROWS_MANY>()) : mode == ROWS_WIDE ? launch(n, v, Int<ROWS_WIDE>()) : launch(n, v, Int<ROWS_ONE>()); };
+        auto with_mode = [&](auto v) { return mode == ROWS_SPLIT ? launch(n, v, Int<ROWS_SPLIT>()) : mode == ROWS_MANY ? launch(n, v, Int<ROWS_MANY>()) : mode == ROWS_WIDE ? launch(n, v, Int<ROWS_WIDE>()) : launch(n, v, Int<ROWS_ONE>()); };
         return vec ? with_mode(Int<1>()) : with_mode(Int<0>());
     };
     if (nt == 2) return with_nt(Int<2>());

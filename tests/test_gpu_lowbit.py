@@ -577,6 +577,15 @@ def test_linear_on_both_sides_of_the_rules_for_few_rows(n, k, m, dtype):
     check_linear(*make(n, k, m, dtype), True, "int8")
 
 
+@pytest.mark.parametrize("n,k,m", [(4097, 333, 129), (5000, 128, 64), (4100, 320, 40), (3000, 70, 257), (8000, 384, 128), (16384, 65, 64),
+                                   (16385, 65, 64), (4321, 600, 30), (2333, 77, 500), (6000, 130, 130)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_several_groups_and_few_tiles(n, k, m, dtype):
+    """The waves of a workgroup share a tile of rows, each a part of the contraction; and the sizes next to that."""
+    check_linear(*make(n, k, m, dtype), True, "int8")
+    check_linear(*make(n, k, m, dtype, bias=False), False, "e4m3")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_at_any_alignment(dtype):
     """Rows, weights and gradients whose first element is not on 16 bytes, pitches that are no multiple of anything."""
