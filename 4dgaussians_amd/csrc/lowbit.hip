@@ -20,6 +20,8 @@ template <typename T> __device__ __forceinline__ float high16(unsigned w)
 // Both directions move 16 bytes of the caller's rows per lane and step (COLS = 4 float32 or 8 16-bit numbers, neighbouring lanes
 // neighbouring addresses, at any alignment: gfx950 loads and stores 16 bytes from any address) and their codes as one word or two.
 // FULL: width is a multiple of COLS, so that no lane has a shorter share (1 M x 256 float32 read back: 217 us, without 327).
+// Bound by memory: 1 M x 256 float32 is written in 278 us (4.7 TB/s of rows and codes, a copy's rate) and read in 214; 333 k scattered
+// rows of 64 are read in 25 us (4.5 TB/s), odd widths at about 3 TB/s.
 // A workgroup owns rpb rows, i.e. about ROWS8_ITEMS (row, columns) items; item e of it is row e / cpr by a multiply-high (exact:
 // e * cpr < 2^32).
 #define ROWS8_ITEMS 2048
@@ -188,7 +190,8 @@ __global__ __launch_bounds__(256) void rows8_read_kernel(gs4d_rows8 c, T* __rest
 }
 
 // ------------------------------------------------------------------ several matrices of rows at once (Gs4dKeepJobs)
-// blockIdx.y: a group of 64 columns of one of the matrices; 16 lanes of 4 columns each, 64 rows per workgroup
+// blockIdx.y: a group of 64 columns of one of the matrices; 16 lanes of 4 columns each, 64 rows per workgroup.  Bound by memory: 5 M rows
+// of 1000 columns are packed in 4.9 ms and unpacked in 5.1 (about 5 TB/s of both sides).
 template <bool WRITE>
 __global__ __launch_bounds__(256) void keep_jobs_kernel(Gs4dKeepJobs jobs, long long rows)
 {

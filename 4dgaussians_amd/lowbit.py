@@ -196,9 +196,9 @@ def frame_features(cache, planes, aabb, points, t):
         _on_device(name, v, dev)
         if v.dtype is not torch.float32:
             raise RuntimeError(f"frame_features: {name} must be float32, got {v.dtype}")
-    P, ch, levels = points.shape[0], shapes[0][1], len(planes) // 3
-    if points.dim() != 2 or points.shape[1] != 3 or tuple(aabb.shape) != (2, 3) or t.numel() not in (1, P):
+    if points.dim() != 2 or points.shape[1] != 3 or tuple(aabb.shape) != (2, 3) or t.numel() not in (1, points.shape[0]):
         raise RuntimeError("frame_features: points [P, 3], aabb [2, 3] and one or P values of t")
+    P, ch, levels = points.shape[0], shapes[0][1], len(planes) // 3
     if cache.width != levels * ch or P > cache.capacity:
         raise RuntimeError(f"frame_features: the cache holds {cache.capacity} rows of {cache.width}, expected at least {P} of {levels * ch}")
     aabb, points, t = aabb.detach().contiguous(), points.detach().contiguous(), t.detach().reshape(-1).contiguous()

@@ -328,6 +328,13 @@ def test_frame_features_refuses():
             lb().frame_features(*args)
 
 
+def test_frame_features_refuses_a_single_number_for_points():
+    c = lb().RowCache(10, 16)
+    z = lambda *s: torch.zeros(*s, device="cuda")
+    with pytest.raises(RuntimeError, match="points"):
+        lb().frame_features(c, [z(1, 16, 3, 3)] * 3, z(2, 3), z(1)[0], z(1))
+
+
 # ------------------------------------------------------------------------------------------ linear
 def leaf(t):
     return t.cuda().requires_grad_(True)
