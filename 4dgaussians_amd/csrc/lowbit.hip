@@ -985,7 +985,7 @@ __global__ __launch_bounds__(256) void linear8_few_dx_kernel(RowsArgs a)
 // the ROWS, and any 8 rows may be the 8 elements a lane supplies as long as both operands agree: a lane loads column pairs
 // (2 i, 2 i + 1) of dy and of the codes straight from memory, row after row, coalesced, and no transposition through LDS is needed.
 // Tile t of the result then holds the columns 2 i + t.  The codes are exact in bfloat16 (8 significant bits), so the rounding
-// lies in dy s alone, which is split into TERMS bfloat16 numbers: three are its 24 bits.
+// lies in dy s alone, a float32 number, whose 24 bits are three bfloat16 numbers, for every type of dy.
 // A workgroup: 64 columns m, GW groups of 64 columns k (a wave each) and 8 / GW row slices per group, summed through LDS;
 // one slab of partial sums per workgroup.  Bound by the vector instructions that form and split dy s, once per group of columns:
 // 180 of them and 12 MFMAs a step of 16 rows (float32, int8).  1.2 M x 256 -> 64: 238 us (reading once: 135), 65536 x 512 -> 512
@@ -1004,9 +1004,10 @@ template <int Q> __device__ __forceinline__ float row_lane(float x)
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + Q, 0xF, 0xF, true));
 }
 
-template <typename T, int FMT, int TERMS, bool VEC>
+template <typename T, int FMT, bool VEC>
 __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
 {
+    constexpr int TERMS = 3;
     __shared__ float s_red[4][64 * 64];
     __shared__ float s_db[8][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
@@ -1470,14 +1471,7 @@ static int launch_dw(DwArgs& a, int fmt, void* dw, void* db, hipStream_t s)
         by_fmt(fmt, [&](auto f) {
             constexpr int F = decltype(f)::value;
             auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3(grid), dim3(512), 0, s, a); };
-            // 16-bit results: two terms of dy s (2^-16 of a product) where the float32 sum over the rows is itself no better
-            // (65536 x 512 -> 512 with its launches and host 185 us, with three terms 216; 1.2 M x 256 -> 64 240 : 266)
-            if constexpr (sizeof(T) == 2)
-                if (a.N >= 1024) {
-                    if (vec) go(linear8_dw_kernel<T, F, 2, true>); else go(linear8_dw_kernel<T, F, 2, false>);
-                    return 0;
-                }
-            if (vec) go(linear8_dw_kernel<T, F, 3, true>); else go(linear8_dw_kernel<T, F, 3, false>);
+            if (vec) go(linear8_dw_kernel<T, F, true>); else go(linear8_dw_kernel<T, F, false>);
             return 0;
         });
     } else {
