@@ -335,9 +335,8 @@ template <typename T> __device__ __forceinline__ f32x16 mfma(const uint4& a, con
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ float top8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// two numbers -> their TERMS bfloat16 parts, packed.  The remainder of an infinity is a NaN, which the clamp (no remainder of a
-// finite number is larger) turns into a number: the infinity stays one.
-template <int TERMS, bool CLAMP>
+// two finite numbers -> their TERMS bfloat16 parts, packed
+template <int TERMS>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
@@ -346,22 +345,34 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
         if (t + 1 < TERMS) {
             a -= top8(a);
             b -= top8(b);
-            if (CLAMP && t == 0) {
-                a = __builtin_amdgcn_fmed3f(a, -0x1p120f, 0x1p120f);
-                b = __builtin_amdgcn_fmed3f(b, -0x1p120f, 0x1p120f);
-            }
         }
     }
 }
 
-template <int TERMS, bool CLAMP = true>
+template <int TERMS>
 __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 {
     unsigned w[4][TERMS];
 #pragma unroll
-    for (int q = 0; q < 4; q++) split2<TERMS, CLAMP>(v[2 * q], v[2 * q + 1], w[q]);
+    for (int q = 0; q < 4; q++) split2<TERMS>(v[2 * q], v[2 * q + 1], w[q]);
 #pragma unroll
     for (int t = 0; t < TERMS; t++) o[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+}
+
+// An infinity or a NaN of either operand of the float32 products.  Among three terms it would meet lower terms that are 0 and give a
+// NaN where the product is an infinity.  So it is represented by its sign as a leading term, 1 or -1, and stands itself where it
+// meets the other operand's leading term alone: a weight's as its third term, one of x in a product of its own.  What the
+// representatives add to the sum is finite and of no account beside an infinity; the sums of other rows and features come out the same.
+__device__ __forceinline__ bool is_finite(unsigned bits) { return (bits & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ float stand_in(unsigned bits) { return __uint_as_float(is_finite(bits) ? bits : 0x3f800000u | (bits & 0x80000000u)); }
+__device__ __forceinline__ unsigned special16(unsigned bits)      // as a bfloat16 number; 0 for a finite one
+{
+    return is_finite(bits) ? 0u : (bits & 0x7fffffffu) > 0x7f800000u ? 0x7fc0u : bits >> 16;
+}
+__device__ __forceinline__ uint4 specials8(const unsigned (&e)[8])
+{
+    return make_uint4(special16(e[0]) | special16(e[1]) << 16, special16(e[2]) | special16(e[3]) << 16,
+                      special16(e[4]) | special16(e[5]) << 16, special16(e[6]) | special16(e[7]) << 16);
 }
 
 // relu on the bits: a number with its sign bit set is a negative integer.  lowest = 0: relu, INT_MIN / -32768: nothing.
@@ -558,9 +569,14 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 if constexpr (sizeof(T) == 4) {
                     float x[8];
 #pragma unroll
-                    for (int q = 0; q < 8; q++) x[q] = f < F && c + q < C ? __uint_as_float(v[u][q]) : 0.f;
+                    for (int q = 0; q < 8; q++) {
+                        v[u][q] = f < F && c + q < C ? v[u][q] : 0u;
+                        x[q] = stand_in(v[u][q]);
+                    }
                     uint4 o[TERMS];
                     split8<TERMS>(x, o);
+                    const uint4 sp = specials8(v[u]);
+                    o[TERMS - 1] = make_uint4(o[TERMS - 1].x | sp.x, o[TERMS - 1].y | sp.y, o[TERMS - 1].z | sp.z, o[TERMS - 1].w | sp.w);
 #pragma unroll
                     for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
                 } else {
@@ -623,6 +639,12 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 for (int z = 0; z <= u; z++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
+        };
+        // a step's infinities and NaNs times the leading terms of the weights
+        auto add_specials = [&](const unsigned (&e)[8], const uint4* __restrict__ wl) {
+            const uint4 sp = specials8(e);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(sp, wl[nt * TERMS * 64], acc[nt]);
         };
         // register r is the row rr + 4 h of the tile, rr = (r & 3) + 8 (r >> 2); o: its results of the tiles nt, nt + 1
         auto put = [&](T* __restrict__ yt, bool whole, int rr, int nt, const float (&o)[PAIR]) {
@@ -720,7 +742,8 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 for (int t = 0; t < 4; t++) o2 = max_u16x2(max_u16x2(o2, max_u16x2(cur.w[t].x & 0x7fff7fffu, cur.w[t].y & 0x7fff7fffu)), max_u16x2(cur.w[t].z & 0x7fff7fffu, cur.w[t].w & 0x7fff7fffu));
                 odd = max(o2 & 0xffffu, o2 >> 16) >= (__is_same(T, LbF16) ? 0x7c00u : 0x7f80u);
             }
-            if (!DX && __builtin_amdgcn_ballot_w64(odd)) positive_nans(cur);
+            const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+            if (!DX && any) positive_nans(cur);
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -798,6 +821,20 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                     else encode(Int<GS4D_FMT_E5M2>());
                 }
             }
+            if constexpr (TERMS > 1)
+                if (any) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        if constexpr (MODE != ROWS_WIDE) {
+                            unsigned e[8];
+#pragma unroll
+                            for (int q = 0; q < 8; q++) e[q] = __float_as_uint(v[t][q]);
+                            add_specials(e, wl + t * NT * TERMS * 64);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 8; q++) v[t][q] = stand_in(__float_as_uint(v[t][q]));
+                    }
+                }
             if constexpr (MODE == ROWS_WIDE) {
                 // one group: its operands stay in registers for all of the workgroup's features
                 uint4 xs[4][TERMS];
@@ -809,6 +846,16 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 #pragma unroll 1
                 for (int k = 0; k < a.blocks; k++) {
                     begin();
+                    if constexpr (TERMS > 1)
+                        if (any) {
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                unsigned e[8];
+#pragma unroll
+                                for (int q = 0; q < 8; q++) e[q] = relu_bits(reinterpret_cast<const unsigned*>(&cur.w[2 * t])[q], a.lowest);
+                                add_specials(e, s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
+                            }
+                        }
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
                         step(xs[t], s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
@@ -1088,10 +1135,10 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
             else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
         }
         uint4 da[2][TERMS], cc[2][1];
-        split8<1, false>(c0, cc[0]);
-        split8<1, false>(c1, cc[1]);
-        split8<TERMS, false>(d0, da[0]);
-        split8<TERMS, false>(d1, da[1]);
+        split8<1>(c0, cc[0]);
+        split8<1>(c1, cc[1]);
+        split8<TERMS>(d0, da[0]);
+        split8<TERMS>(d1, da[1]);
 #pragma unroll
         for (int u = TERMS - 1; u >= 0; u--)
 #pragma unroll

@@ -53,3 +53,97 @@ def test_weight_gradient_of_rows_that_cancel(n, dtype):
     lost = (len(dy[:-1:2]) * (float(scale) - float((scale.view(np.uint32) & np.uint32(0xffffff00)).view(np.float32)))) * codes.double().numpy()
     assert (lost > 1.2 * tol).all(), (lost / tol).min()
     assert (np.abs(np64(dw) - want) <= tol).all(), (np.abs(np64(dw) - want) / tol).max()
+
+
+# (rows, contraction, features) of each way to walk the products over the rows: one group of columns and one block of features, with
+# and without a multiple of 8 columns; several blocks; several groups with few and with many rows; a weight that does not fit LDS
+WALKS = [(5000, 64, 64), (4100, 64, 20), (4500, 61, 64), (4500, 64, 200), (5000, 256, 64), (4300, 333, 129), (70_000, 128, 32), (70_000, 100, 64),
+         (20_000, 450, 66), (20_000, 512, 66)]
+LOW_NAN = float(np.uint32(0x7f800001).view(np.float32))               # its upper half is an infinity's
+
+
+def products(x, w):
+    """sum_c x[r, c] w[f, c] as it is defined, infinities and NaNs among them, a few rows at a time."""
+    with np.errstate(invalid="ignore"):
+        return np.concatenate([(r[:, None, :] * w[None]).sum(-1) for r in np.array_split(x, max(1, len(x) // 64))])
+
+
+def _plain(x, w):
+    with torch.no_grad():
+        return lb().linear(x.cuda(), w.cuda())
+
+
+@np.errstate(invalid="ignore")
+def magnitude(x, w):
+    return np.abs(x) @ np.abs(w).T
+
+
+def same_specials(got, want, most, terms):
+    got = np64(got)
+    assert (np.isnan(got) == np.isnan(want)).all()
+    assert ((got == np.inf) == (want == np.inf)).all() and ((got == -np.inf) == (want == -np.inf)).all()
+    f = np.isfinite(want)
+    assert (np.abs(got[f] - want[f]) <= (terms + 8) * 2.0 ** -24 * most[f]).all()
+
+
+def special_operands(n, c, f, seed):
+    """A few rows and features with infinities and NaNs, weights of few significant bits and zeros among them."""
+    g = torch.Generator().manual_seed(seed)
+    x, w = rows(n, c, seed=seed), torch.randn(f, c, generator=g)
+    w[::3] = w[::3].bfloat16().float()
+    w[1::3, ::2], w[1::3, 1::2] = 0.5, -1.0
+    w[2, ::5] = 0
+    at = torch.randperm(n, generator=g)[:40]
+    col = torch.randint(0, c, (40,), generator=g)
+    inf = float("inf")
+    for i, v in enumerate([inf, -inf, float("nan"), LOW_NAN, -LOW_NAN] * 8):
+        x[at[i], col[i]] = v
+    x[at[5:10], (col[5:10] + 7) % c] = inf                            # two in a row: the same or opposite ones
+    x[at[10], :] = inf
+    x[n - 1, c - 1] = -inf
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[at] = hit[n - 1] = True
+    return x, w, hit, torch.cat([at, torch.tensor([n - 1]), torch.randint(0, n, (60,), generator=g)])
+
+
+@pytest.mark.parametrize("n,c,f", WALKS)
+def test_infinities_and_nans_of_the_rows(n, c, f):
+    x, w, hit, look = special_operands(n, c, f, n + c)
+    X, W = np64(x), np64(w)
+    for relu in (False, True):
+        with torch.no_grad():
+            y = lb().linear(x.cuda(), w.cuda(), relu=relu)
+            clean = lb().linear(torch.where(hit[:, None], 0, x).cuda(), w.cuda(), relu=relu)
+        A = np.maximum(X, 0) if relu else X                           # (keeps NaNs)
+        same_specials(y.cpu()[look], products(A[look], W), magnitude(A[look], W), c)
+        assert torch.equal(y.cpu()[~hit], clean.cpu()[~hit])          # the other rows: not another bit
+        leaf_x = leaf(x)
+        kept = lb().linear(leaf_x, leaf(w), relu=relu)
+        assert torch.equal(torch.nan_to_num(kept), torch.nan_to_num(y)) and torch.equal(kept.isnan(), y.isnan())
+    # the same numbers as an upstream gradient: dx = dy W over the features of dy
+    xs = leaf(torch.ones(n, f))
+    for relu in (False, True):
+        dx, = torch.autograd.grad(lb().linear(xs, w.t().contiguous().cuda(), relu=relu), xs, x.cuda())
+        same_specials(dx.cpu()[look], products(X[look], W), magnitude(X[look], W), c)
+
+
+@pytest.mark.parametrize("n,c,f", WALKS)
+def test_infinities_and_nans_of_the_weight(n, c, f):
+    x, w, hit, look = special_operands(n, c, f, n + f)
+    x = torch.where(torch.isfinite(x), x, 1.0)
+    x[5, :] = 0
+    inf = float("inf")
+    w2 = w.clone()
+    for i, v in enumerate([inf, -inf, float("nan"), LOW_NAN]):
+        w2[(7 * i) % f, (5 + 11 * i) % c] = v
+    w2[f - 1, c - 1], w2[f - 2, :] = -inf, inf
+    look = torch.cat([look, torch.tensor([5])])
+    y = _plain(x, w2).cpu()
+    same_specials(y[look], products(np64(x[look]), np64(w2)), magnitude(np64(x[look]), np64(w2)), c)
+    fine = torch.isfinite(w2).all(dim=1)
+    assert torch.equal(y[:, fine], _plain(x, w).cpu()[:, fine])
+    # both at once: where they meet and where they do not
+    x2 = x.clone()
+    x2[:4, 5 % c], x2[4, 0], x2[6, c - 1] = torch.tensor([inf, -inf, float("nan"), LOW_NAN]), inf, -inf
+    at = torch.arange(8)
+    same_specials(_plain(x2, w2).cpu()[at], products(np64(x2[at]), np64(w2)), magnitude(np64(x2[at]), np64(w2)), c)
