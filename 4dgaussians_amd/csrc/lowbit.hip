@@ -1106,8 +1106,8 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
     f32x16 acc[2][2] = {};
     float db0 = 0.f, db1 = 0.f;
     int turn = wave % a.gw;
-    auto add = [&](const Rows& cur, long long r0, auto last) {
-        constexpr bool LAST = decltype(last)::value != 0;
+    auto add = [&](const Rows& cur, long long r0, auto last, auto any) {
+        constexpr bool LAST = decltype(last)::value != 0, ANY = decltype(any)::value != 0;
         float d0[8], d1[8], c0[8], c1[8];
         const float sq[8] = {row_lane<0>(cur.s), row_lane<1>(cur.s), row_lane<2>(cur.s), row_lane<3>(cur.s),
                              row_lane<4>(cur.s), row_lane<5>(cur.s), row_lane<6>(cur.s), row_lane<7>(cur.s)};
@@ -1137,8 +1137,21 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
         uint4 da[2][TERMS], cc[2][1];
         split8<1>(c0, cc[0]);
         split8<1>(c1, cc[1]);
-        split8<TERMS>(d0, da[0]);
-        split8<TERMS>(d1, da[1]);
+        if constexpr (ANY) {                              // infinities and NaNs: stand_in()
+            auto split = [&](float (&d)[8], uint4 (&o)[TERMS]) {
+                unsigned e[8];
+#pragma unroll
+                for (int q = 0; q < 8; q++) { e[q] = __float_as_uint(d[q]); d[q] = stand_in(e[q]); }
+                split8<TERMS>(d, o);
+                const uint4 sp = specials8(e);            // (the codes are one term)
+                o[TERMS - 1] = make_uint4(o[TERMS - 1].x | sp.x, o[TERMS - 1].y | sp.y, o[TERMS - 1].z | sp.z, o[TERMS - 1].w | sp.w);
+            };
+            split(d0, da[0]);
+            split(d1, da[1]);
+        } else {
+            split8<TERMS>(d0, da[0]);
+            split8<TERMS>(d1, da[1]);
+        }
 #pragma unroll
         for (int u = TERMS - 1; u >= 0; u--)
 #pragma unroll
@@ -1146,7 +1159,7 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
 #pragma unroll
                 for (int y = 0; y < 2; y++) acc[t][y] = mfma<LbBf16>(da[t][u], cc[y][0], acc[t][y]);
     };
-    if (mine) {
+    auto sweep = [&](auto any) {
         // whole steps of 16 rows, the next one in flight; the chunk's last, shorter step follows
         const long long stride = 16ll * slices, end = n1 - 15;
         long long r0 = n0 + 16 * slice;
@@ -1159,7 +1172,7 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
 #pragma unroll
                 for (int u = 0; u < 3; u++) {
                     load(ring[(u + 2) % 3], r0 + 2 * stride < end ? r0 + 2 * stride : r0, Int<0>());
-                    add(ring[u], r0, Int<0>());
+                    add(ring[u], r0, Int<0>(), any);
                     r0 += stride;
                     if (r0 >= end) { more = false; break; }
                 }
@@ -1168,7 +1181,27 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
         if (r0 < n1) {
             Rows cur;
             load(cur, r0, Int<1>());
-            add(cur, r0, Int<1>());
+            add(cur, r0, Int<1>(), any);
+        }
+    };
+    if (mine) {
+        sweep(Int<0>());
+        // an infinity has left NaNs (its remainder is one): the wave's rows once more, with what that costs
+        bool nan = false;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int y = 0; y < 2; y++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) nan |= acc[t][y][r] != acc[t][y][r];
+        if (__builtin_amdgcn_ballot_w64(nan)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) acc[t][y] = f32x16{};
+            db0 = db1 = 0.f;
+            turn = wave % a.gw;
+            sweep(Int<1>());
         }
     }
     // ---- the slices of a group, in a fixed order: the upper half adds to the lower half until one is left

@@ -59,7 +59,7 @@ def test_weight_gradient_of_rows_that_cancel(n, dtype):
 # and without a multiple of 8 columns; several blocks; several groups with few and with many rows; a weight that does not fit LDS
 WALKS = [(5000, 64, 64), (4100, 64, 20), (4500, 61, 64), (4500, 64, 200), (5000, 256, 64), (4300, 333, 129), (70_000, 128, 32), (70_000, 100, 64),
          (20_000, 450, 66), (20_000, 512, 66)]
-LOW_NAN = float(np.uint32(0x7f800001).view(np.float32))               # its upper half is an infinity's
+LOW_NAN = 0x7f800001                                                  # a NaN whose upper half is an infinity's
 
 
 def products(x, w):
@@ -96,11 +96,13 @@ def special_operands(n, c, f, seed):
     at = torch.randperm(n, generator=g)[:40]
     col = torch.randint(0, c, (40,), generator=g)
     inf = float("inf")
-    for i, v in enumerate([inf, -inf, float("nan"), LOW_NAN, -LOW_NAN] * 8):
+    for i, v in enumerate([inf, -inf, float("nan"), 0.0, 0.0] * 8):
         x[at[i], col[i]] = v
     x[at[5:10], (col[5:10] + 7) % c] = inf                            # two in a row: the same or opposite ones
     x[at[10], :] = inf
     x[n - 1, c - 1] = -inf
+    bits = x.view(torch.int32)
+    bits[at[13], col[13]], bits[at[14], col[14]] = LOW_NAN, LOW_NAN - 2 ** 31
     hit = torch.zeros(n, dtype=torch.bool)
     hit[at] = hit[n - 1] = True
     return x, w, hit, torch.cat([at, torch.tensor([n - 1]), torch.randint(0, n, (60,), generator=g)])
@@ -134,8 +136,9 @@ def test_infinities_and_nans_of_the_weight(n, c, f):
     x[5, :] = 0
     inf = float("inf")
     w2 = w.clone()
-    for i, v in enumerate([inf, -inf, float("nan"), LOW_NAN]):
+    for i, v in enumerate([inf, -inf, float("nan")]):
         w2[(7 * i) % f, (5 + 11 * i) % c] = v
+    w2.view(torch.int32)[11 % f, 3] = LOW_NAN
     w2[f - 1, c - 1], w2[f - 2, :] = -inf, inf
     look = torch.cat([look, torch.tensor([5])])
     y = _plain(x, w2).cpu()
@@ -144,6 +147,37 @@ def test_infinities_and_nans_of_the_weight(n, c, f):
     assert torch.equal(y[:, fine], _plain(x, w).cpu()[:, fine])
     # both at once: where they meet and where they do not
     x2 = x.clone()
-    x2[:4, 5 % c], x2[4, 0], x2[6, c - 1] = torch.tensor([inf, -inf, float("nan"), LOW_NAN]), inf, -inf
+    x2[:4, 5 % c], x2[4, 0], x2[6, c - 1] = torch.tensor([inf, -inf, float("nan"), inf]), inf, -inf
     at = torch.arange(8)
     same_specials(_plain(x2, w2).cpu()[at], products(np64(x2[at]), np64(w2)), magnitude(np64(x2[at]), np64(w2)), c)
+
+
+@pytest.mark.parametrize("n,k,m", [(300, 64, 64), (3000, 100, 65), (129, 5, 1), (5001, 600, 70), (40_000, 64, 3)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_and_nans_of_the_gradient(n, k, m, fmt, dtype):
+    """Weight and bias gradients: the columns of dy that hold them get what the sum is, the other columns keep their bits."""
+    g = torch.Generator().manual_seed(n + k)
+    x, dy = rows(n, k, dtype, seed=n), (1e-2 * torch.randn(n, m, generator=g)).to(dtype)
+    x[7, :] = 0                                                       # an infinity times 0
+    clean, bad = dy.clone(), sorted({0, m // 2, m - 1})
+    inf = float("inf")
+    dy[n // 3, bad[0]] = inf
+    dy[n - 1, bad[-1]] = -inf
+    dy[torch.randint(8, n, (5,), generator=g), bad[len(bad) // 2]] = inf
+    if m > 64:
+        dy[5, 33], dy[9, 34], dy[11, 34], dy[7, 35] = float("nan"), inf, -inf, inf
+        bad += [33, 34, 35]
+    ws, bs = leaf(torch.zeros(m, k, dtype=dtype)), leaf(torch.zeros(m, dtype=dtype))
+    run = lambda d: [t.cpu() for t in torch.autograd.grad(lb().linear(x.cuda(), ws, bs, relu=True, fmt=fmt), (ws, bs), d.cuda())]
+    got, fine = run(dy), run(clean)
+    others = [c for c in range(m) if c not in bad]
+    assert all(torch.equal(a[others], b[others]) for a, b in zip(got, fine))
+    kept = R.quantise(np.maximum(np64(x), 0), "uint8" if fmt == "int8" else fmt, 64)[0]
+    with np.errstate(invalid="ignore"):
+        want = np.stack([(np64(dy[:, c, None]) * kept).sum(0) for c in bad])
+        wdb = np64(dy[:, bad]).sum(0)
+    for a, b in ((got[0][bad], want), (got[1][bad], wdb)):
+        a = np64(a)
+        assert (np.isnan(a) == np.isnan(b)).all() and (a[~np.isnan(b)] == b[~np.isnan(b)]).all()      # nothing finite is left
+    assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(run(dy), got))
