@@ -87,7 +87,7 @@ class FusedAdamW(torch.optim.Optimizer):
             base = torch.tensor(counts, dtype=torch.float32)
             for i, (_, _, st) in enumerate(items):
                 st["step"] = base[i]
-            plan.append(dict(key=key, items=items, rec=rec, gidx=np.array([gi for gi, _, _ in items]),
+            plan.append(dict(key=key, items=items, rec=rec, params=[p for _, p, _ in items], gidx=np.array([gi for gi, _, _ in items]),
                              steps=np.array(counts, dtype=np.float64), base=base))
         return plan
 
@@ -138,6 +138,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 rc = L.gs4d_adamw_step(C.c_int(len(rec)), C.c_void_p(rec.ctypes.data), C.c_double(beta1), C.c_double(beta2),
                                        C.c_double(eps), _cabi.current_stream(dev))
             _cabi.check(rc, "gs4d_adamw_step")
+            # the kernel writes through pointers: whoever keeps something made from the parameters (a graph whose backward is to
+            # come, planes frozen for rendering) sees by their versions that they are others now, as after torch's optimizers
+            torch.autograd.graph.increment_version(b["params"])
             b["steps"] = steps
             b["base"] += 1.0
             del keep

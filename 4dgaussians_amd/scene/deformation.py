@@ -522,8 +522,10 @@ class Deformation(nn.Module):
         """For rendering many frames of one model: keeps, in 8 bits, the product of every level's three spatial planes at
         points [P, 3] (which no frame changes), so that a query without gradients samples three planes a level instead of six.
         Queries are then of these points (P rows, or several copies of them as render_batch makes) until thaw_planes() or the
-        first query with gradients enabled; a change of bounds or device thaws as well.  The features are off by at most half
-        a step of the format (int8: 1 / 254 of the largest of 64 neighbouring ones)."""
+        first query with gradients enabled; a change of bounds or device thaws as well.  Planes whose version has changed since (in
+        place, or by an optimizer) make the next query raise; a replayed graph that trains and a write through `.data` change no
+        version: thaw after them.  The features are off by at most half a step of the format (int8: 1 / 254 of the largest of 64
+        neighbouring ones)."""
         self.thaw_planes()
         if not isinstance(points, torch.Tensor) or points.dim() != 2 or points.shape[1] != 3 or points.shape[0] < 1 or points.dtype != torch.float32:
             raise RuntimeError("freeze_planes: points must be float32 [P, 3] with at least one row")
