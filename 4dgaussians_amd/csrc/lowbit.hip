@@ -310,13 +310,16 @@ template <typename F> static int by_fmt(int fmt, F f)
 }
 
 // What the matrix cores work on: 8 consecutive elements of a row per lane (lane & 31: the row of the operand, lane >> 5: which
-// half of 16), as 16-bit numbers.  A float32 number is the sum of three bfloat16 numbers -- its leading 8 significant bits, the
-// next 8 and the last 8, by truncation, so the sum is exact above 2^-110 -- and a product of two of them is taken from the six
-// largest of the nine term products; the three left out are below 2^-23 of it together.  Six bfloat16 MFMAs against the
-// float32 one: 2.7 times its rate.
+// half of 16), as 16-bit numbers.  A float32 number is the sum of three bfloat16 numbers: itself rounded to nearest, what is left
+// rounded to nearest, and what is left then (exact above 2^-100).  The second is below 2^-8 of the first and the third below 2^-17,
+// each of either sign, and a product of two numbers is taken from the six largest of the nine term products: the three left out are
+// below 2^-24 (1 + 2^-8) of it together, a rounding's worth.  (Terms cut off instead of rounded leave out up to 2^-21, always in one
+// direction.)  A product within 2^-7 of the largest float32 number may become an infinity.  Six bfloat16 MFMAs against the float32
+// one: 2.7 times its rate.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
@@ -335,26 +338,28 @@ template <typename T> __device__ __forceinline__ f32x16 mfma(const uint4& a, con
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ float top8(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// two finite numbers -> their TERMS bfloat16 parts, packed
-template <int TERMS>
+// two finite numbers -> their TERMS bfloat16 parts, packed.  ROUND: rounded to nearest (fits() says which numbers that is for), else
+// the leading 8 bits each: of a sum of terms times ONE term all products are taken, and either is exact.
+template <int TERMS, bool ROUND>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
     for (int t = 0; t < TERMS; t++) {
-        o[t] = hi16(__float_as_uint(a), __float_as_uint(b));
+        if constexpr (ROUND) o[t] = __builtin_bit_cast(unsigned, __builtin_convertvector((lb_float2){a, b}, bf16x2));
+        else o[t] = hi16(__float_as_uint(a), __float_as_uint(b));
         if (t + 1 < TERMS) {
-            a -= top8(a);
-            b -= top8(b);
+            a -= ROUND ? __uint_as_float(o[t] << 16) : top8(a);
+            b -= ROUND ? __uint_as_float(o[t] & 0xffff0000u) : top8(b);
         }
     }
 }
 
-template <int TERMS>
+template <int TERMS, bool ROUND>
 __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 {
     unsigned w[4][TERMS];
 #pragma unroll
-    for (int q = 0; q < 4; q++) split2<TERMS>(v[2 * q], v[2 * q + 1], w[q]);
+    for (int q = 0; q < 4; q++) split2<TERMS, ROUND>(v[2 * q], v[2 * q + 1], w[q]);
 #pragma unroll
     for (int t = 0; t < TERMS; t++) o[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
 }
@@ -363,16 +368,42 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 // NaN where the product is an infinity.  So it is represented by its sign as a leading term, 1 or -1, and stands itself where it
 // meets the other operand's leading term alone: a weight's as its third term, one of x in a product of its own.  What the
 // representatives add to the sum is finite and of no account beside an infinity; the sums of other rows and features come out the same.
+// A number that would be rounded to an infinity has its leading 8 bits as a term beside the three of what is left.
 __device__ __forceinline__ bool is_finite(unsigned bits) { return (bits & 0x7f800000u) != 0x7f800000u; }
-__device__ __forceinline__ float stand_in(unsigned bits) { return __uint_as_float(is_finite(bits) ? bits : 0x3f800000u | (bits & 0x80000000u)); }
-__device__ __forceinline__ unsigned special16(unsigned bits)      // as a bfloat16 number; 0 for a finite one
+__device__ __forceinline__ bool fits(unsigned bits) { return (bits & 0x7fffffffu) < 0x7f7f8000u; }
+__device__ __forceinline__ float stand_in(unsigned bits)
 {
-    return is_finite(bits) ? 0u : (bits & 0x7fffffffu) > 0x7f800000u ? 0x7fc0u : bits >> 16;
+    const float x = __uint_as_float(bits);
+    const unsigned left = __float_as_uint(x - top8(x)), one = 0x3f800000u | (bits & 0x80000000u);
+    const unsigned fit = (unsigned)((int)((bits & 0x7fffffffu) - 0x7f7f8000u) >> 31), fin = (unsigned)((int)((bits & 0x7fffffffu) - 0x7f800000u) >> 31);
+    return __uint_as_float((bits & fit) | (((left & fin) | (one & ~fin)) & ~fit));       // masks: 32 of these as branches cost registers
 }
-__device__ __forceinline__ uint4 specials8(const unsigned (&e)[8])
+// as bfloat16 numbers, 0 where there is nothing to represent
+__device__ __forceinline__ unsigned special16(unsigned bits)
 {
-    return make_uint4(special16(e[0]) | special16(e[1]) << 16, special16(e[2]) | special16(e[3]) << 16,
-                      special16(e[4]) | special16(e[5]) << 16, special16(e[6]) | special16(e[7]) << 16);
+    const unsigned a = bits & 0x7fffffffu, fin = (unsigned)((int)(a - 0x7f800000u) >> 31), nan = (unsigned)((int)(0x7f800000u - a) >> 31);
+    return ((bits >> 16) | (nan & 0x40u)) & ~fin;
+}
+__device__ __forceinline__ unsigned large16(unsigned bits)
+{
+    const unsigned a = bits & 0x7fffffffu, fit = (unsigned)((int)(a - 0x7f7f8000u) >> 31), fin = (unsigned)((int)(a - 0x7f800000u) >> 31);
+    return (bits >> 16) & ~fit & fin;
+}
+template <typename F> __device__ __forceinline__ uint4 pack8(const unsigned (&e)[8], F f)
+{
+    return make_uint4(f(e[0]) | f(e[1]) << 16, f(e[2]) | f(e[3]) << 16, f(e[4]) | f(e[5]) << 16, f(e[6]) | f(e[7]) << 16);
+}
+__device__ __forceinline__ uint4 specials8(const unsigned (&e)[8]) { return pack8(e, [](unsigned b) { return special16(b); }); }
+__device__ __forceinline__ uint4 larges8(const unsigned (&e)[8]) { return pack8(e, [](unsigned b) { return large16(b); }); }
+// bfloat16 numbers with 0 in place of infinities and NaNs
+__device__ __forceinline__ uint4 finite_only(const uint4& v)
+{
+    auto word = [](unsigned x) {
+        if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+        if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
+        return x;
+    };
+    return make_uint4(word(v.x), word(v.y), word(v.z), word(v.w));
 }
 
 // relu on the bits: a number with its sign bit set is a negative integer.  lowest = 0: relu, INT_MIN / -32768: nothing.
@@ -568,15 +599,30 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 }
                 if constexpr (sizeof(T) == 4) {
                     float x[8];
+                    bool fit = true;
 #pragma unroll
                     for (int q = 0; q < 8; q++) {
                         v[u][q] = f < F && c + q < C ? v[u][q] : 0u;
-                        x[q] = stand_in(v[u][q]);
+                        x[q] = __uint_as_float(v[u][q]);
+                        fit = fit && fits(v[u][q]);
                     }
                     uint4 o[TERMS];
-                    split8<TERMS>(x, o);
-                    const uint4 sp = specials8(v[u]);
-                    o[TERMS - 1] = make_uint4(o[TERMS - 1].x | sp.x, o[TERMS - 1].y | sp.y, o[TERMS - 1].z | sp.z, o[TERMS - 1].w | sp.w);
+                    if (fit) {
+                        split8<TERMS, true>(x, o);
+                    } else {                              // a weight has no term to spare: its leading bits and two terms of what is left
+                        auto join = [](const uint4& a, const uint4& b) { return make_uint4(a.x | b.x, a.y | b.y, a.z | b.z, a.w | b.w); };
+                        auto first = [](unsigned b) {     // (what rounding gives, but for numbers that do not fit)
+                            const float x = __uint_as_float(b);
+                            return fits(b) ? (unsigned)__builtin_bit_cast(unsigned short, (__bf16)x) : is_finite(b) ? b >> 16 : 0x3f80u | b >> 31 << 15;
+                        };
+                        uint4 two[2];
+#pragma unroll
+                        for (int q = 0; q < 8; q++) x[q] = is_finite(v[u][q]) ? x[q] - __uint_as_float(first(v[u][q]) << 16) : 0.f;
+                        split8<2, true>(x, two);
+                        o[0] = pack8(v[u], first);
+                        o[1] = two[0];
+                        o[TERMS - 1] = join(two[1], specials8(v[u]));
+                    }
 #pragma unroll
                     for (int t = 0; t < TERMS; t++) s_w[((step * NT + nt) * TERMS + t) * 64 + l] = o[t];
                 } else {
@@ -640,11 +686,20 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(xs[u - z], ws[nt][z], acc[nt]);
         };
-        // a step's infinities and NaNs times the leading terms of the weights
+        // what stand_in() leaves out of a step
         auto add_specials = [&](const unsigned (&e)[8], const uint4* __restrict__ wl) {
-            const uint4 sp = specials8(e);
+            const uint4 sp = specials8(e), lg = larges8(e);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) acc[nt] = mfma<T>(sp, wl[nt * TERMS * 64], acc[nt]);
+            for (int nt = 0; nt < NT; nt++) {
+                __builtin_amdgcn_sched_barrier(0);        // rare: few registers count, not time
+                acc[nt] = mfma<T>(sp, wl[nt * TERMS * 64], acc[nt]);
+#pragma unroll
+                for (int u = TERMS - 1; u >= 0; u--) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    acc[nt] = mfma<T>(lg, finite_only(wl[(nt * TERMS + u) * 64]), acc[nt]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         };
         // register r is the row rr + 4 h of the tile, rr = (r & 3) + 8 (r >> 2); o: its results of the tiles nt, nt + 1
         auto put = [&](T* __restrict__ yt, bool whole, int rr, int nt, const float (&o)[PAIR]) {
@@ -715,7 +770,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
             const int g = group_at(gi);
             int Cn = a.C;
             asm("" : "+s"(Cn));                           // column limits are recomputed: kept over the loop they would spill
-            if (!SPLIT && a.chunk < a.groups && gi % a.chunk == 0) {
+            if (MODE == ROWS_MANY && a.chunk < a.groups && gi % a.chunk == 0) {
                 __syncthreads();
                 stage(gi, min(a.chunk, a.groups - gi), s_w);
                 __syncthreads();
@@ -724,7 +779,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 if (!VEC) fix_end(cur, row_of(tile), g * 64 + 8 * h, Cn, end);
                 clear_past(cur, g * 64 + 8 * h, Cn);
             }
-            const uint4* __restrict__ wl = s_w + (size_t)(!SPLIT && a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
+            const uint4* __restrict__ wl = s_w + (size_t)(MODE == ROWS_MANY && a.chunk < a.groups ? gi % a.chunk : g) * 4 * NT * TERMS * 64 + lane;
             constexpr int NEXT = SPLIT ? WAVES : 1;
             const bool more = SPLIT ? g + NEXT < a.groups : gi + 1 < a.groups;
             Group<T> nxt;
@@ -735,7 +790,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int t = 0; t < 8; t++) odd = max(max(odd, max(cur.w[t].x & 0x7fffffffu, cur.w[t].y & 0x7fffffffu)), max(cur.w[t].z & 0x7fffffffu, cur.w[t].w & 0x7fffffffu));
-                odd = odd >= 0x7f800000u;
+                odd = odd >= 0x7f7f8000u;                 // !fits()
             } else {
                 unsigned o2 = 0;
 #pragma unroll
@@ -840,7 +895,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 uint4 xs[4][TERMS];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs[t]);
+                    if constexpr (sizeof(T) == 4) split8<TERMS, true>(v[t], xs[t]);
                     else xs[t][0] = cur.w[t];
                 }
 #pragma unroll 1
@@ -871,7 +926,7 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 for (int t = 0; t < 4; t++) {
                     if (MODE == ROWS_ONE) __builtin_amdgcn_sched_barrier(0);      // a step at a time: hoisted splits and weights would spill
                     uint4 xs[TERMS];
-                    if constexpr (sizeof(T) == 4) split8<TERMS>(v[t], xs);
+                    if constexpr (sizeof(T) == 4) split8<TERMS, true>(v[t], xs);
                     else xs[0] = cur.w[t];
                     step(xs, wl + t * NT * TERMS * 64);
                 }
@@ -1135,22 +1190,22 @@ __global__ __launch_bounds__(512) void linear8_dw_kernel(DwArgs a)
             else { c0[q] = (float)(int)(signed char)cur.c[q]; c1[q] = (float)((int)(short)cur.c[q] >> 8); }
         }
         uint4 da[2][TERMS], cc[2][1];
-        split8<1>(c0, cc[0]);
-        split8<1>(c1, cc[1]);
+        split8<1, false>(c0, cc[0]);
+        split8<1, false>(c1, cc[1]);
         if constexpr (ANY) {                              // infinities and NaNs: stand_in()
             auto split = [&](float (&d)[8], uint4 (&o)[TERMS]) {
                 unsigned e[8];
 #pragma unroll
-                for (int q = 0; q < 8; q++) { e[q] = __float_as_uint(d[q]); d[q] = stand_in(e[q]); }
-                split8<TERMS>(d, o);
+                for (int q = 0; q < 8; q++) { e[q] = __float_as_uint(d[q]); d[q] = is_finite(e[q]) ? d[q] : stand_in(e[q]); }
+                split8<TERMS, false>(d, o);
                 const uint4 sp = specials8(e);            // (the codes are one term)
                 o[TERMS - 1] = make_uint4(o[TERMS - 1].x | sp.x, o[TERMS - 1].y | sp.y, o[TERMS - 1].z | sp.z, o[TERMS - 1].w | sp.w);
             };
             split(d0, da[0]);
             split(d1, da[1]);
         } else {
-            split8<TERMS>(d0, da[0]);
-            split8<TERMS>(d1, da[1]);
+            split8<TERMS, false>(d0, da[0]);
+            split8<TERMS, false>(d1, da[1]);
         }
 #pragma unroll
         for (int u = TERMS - 1; u >= 0; u--)

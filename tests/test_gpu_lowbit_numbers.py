@@ -181,3 +181,55 @@ def test_infinities_and_nans_of_the_gradient(n, k, m, fmt, dtype):
         a = np64(a)
         assert (np.isnan(a) == np.isnan(b)).all() and (a[~np.isnan(b)] == b[~np.isnan(b)]).all()      # nothing finite is left
     assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(run(dy), got))
+
+
+@pytest.mark.parametrize("n,c,f", [(5000, 1, 64), (4100, 1, 20), (4500, 1, 200), (5000, 65, 64), (70_000, 129, 32), (20_000, 513, 66)])
+def test_a_product_of_two_float32_numbers_is_rounded_like_one(n, c, f):
+    """One product per result (the other columns of x are zeros), of numbers with all 24 bits set or drawn.  At most 2^-24 (1 + 2^-8)
+    of it is left out and the sums of the terms' products are rounded: five below 2^-6 of the product, then one that may be half a
+    step or, cut off, a step of 2^-23 off."""
+    g = torch.Generator().manual_seed(n + c)
+    at = torch.randint(0, c, (n,), generator=g)
+    v = (1 + torch.rand(n, generator=g)) * torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0) * torch.exp(4 * torch.randn(n, generator=g))
+    v[:500] = 1 + 2.0 ** -7 - 2.0 ** -23
+    v[500:1000] = -(1 + 2.0 ** -8 + 2.0 ** -9 - 2.0 ** -23)
+    x = torch.zeros(n, c)
+    x[torch.arange(n), at] = v
+    w = (1 + torch.rand(f, c, generator=g)) * torch.where(torch.rand(f, c, generator=g) < 0.5, -1.0, 1.0)
+    w[::4] = 1 + 2.0 ** -7 - 2.0 ** -23
+    w[1::4] = 1 + 2.0 ** -8 + 2.0 ** -9 - 2.0 ** -23
+    want = np64(v)[:, None] * np64(w).T[at.numpy()]
+    y = np64(_plain(x, w))
+    bound = (1.01 + 5 * 2.0 ** -6 + 2) * 2.0 ** -24
+    assert (np.abs(y - want) <= bound * np.abs(want)).all(), (np.abs(y - want) / np.abs(want)).max() * 2.0 ** 24
+    xs = leaf(torch.ones(n, f))
+    dx, = torch.autograd.grad(lb().linear(xs, w.t().contiguous().cuda()), xs, x.cuda())
+    dx = np64(dx)
+    assert (np.abs(dx - want) <= bound * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("n,c,f", WALKS)
+def test_numbers_next_to_the_largest(n, c, f):
+    """Rows and weights that rounding to 8 bits would make infinite, the type's lowest number among them, against small ones."""
+    g = torch.Generator().manual_seed(n + c + f)
+    x, w = rows(n, c, seed=n), torch.randn(f, c, generator=g) * 1e-3
+    big = torch.finfo(torch.float32)
+    at, col = torch.randperm(n, generator=g)[:30], torch.randint(0, c, (30,), generator=g)
+    x[at, col] = torch.tensor([big.max, big.min, 3.3961e38, -3.399e38, 3.3960e38] * 6)
+    w2 = w.clone()
+    for i, v in enumerate([big.max, big.min, 3.397e38]):
+        w2[(5 * i) % f, (3 + 7 * i) % c] = v
+    look = torch.cat([at, torch.randint(0, n, (50,), generator=g)])
+    small = torch.where(x.abs() > 1e38, 1e-3 * torch.ones(()), x.clamp(-0.4, 0.4))
+    for a, b in ((x, w), (small, w2)):
+        want = products(np64(a[look]), np64(b))
+        assert np.isfinite(want.astype(np.float32)).all()
+        same_specials(_plain(a, b).cpu()[look], want, magnitude(np64(a[look]), np64(b)), c)
+        xs = leaf(torch.ones(n, f))
+        dx, = torch.autograd.grad(lb().linear(xs, b.t().contiguous().cuda()), xs, a.cuda())
+        same_specials(dx.cpu()[look], want, magnitude(np64(a[look]), np64(b)), c)
+    # both: a row's largest number meets an infinite weight, a weight's an infinite number
+    x3, w3 = x.clone(), w2.clone()
+    x3[0, :], w3[1 % f, :] = big.max, float("inf")
+    x3[1, :] = float("-inf")
+    assert (_plain(x3, w3).cpu()[0, 1 % f] == float("inf")) and (_plain(x3, w3).cpu()[1, 1 % f] == float("-inf"))
