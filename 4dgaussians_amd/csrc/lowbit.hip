@@ -642,6 +642,11 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
     auto row_of = [&](long long tile) { const long long r = tile * 32 + j; return X + (r < a.N ? r : a.N - 1) * a.ldx; };
     long long tile = SPLIT ? wg : (long long)wave * a.nwg + wg;
     constexpr int TILES = SPLIT ? 1 : WAVES;              // per workgroup and round
+    // one group of columns, float32: rows whose numbers are not all fits() are done again at the end, one by one, where registers are
+    // free (taken care of among the others they cost a 64 -> 64 input gradient of 100 k rows 28 us instead of 18); bit i: in the rounds i modulo 64
+    constexpr bool AGAIN = TERMS > 1 && (MODE == ROWS_ONE || MODE == ROWS_WIDE);
+    unsigned long long again = 0;
+    const long long tile0 = tile;
     Group<T> cur;
     // the waves start at different groups: a row of several 256-byte groups, read by all waves in step, would keep to a fraction of
     // the memory channels at a time
@@ -770,7 +775,9 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
             const int g = group_at(gi);
             int Cn = a.C;
             asm("" : "+s"(Cn));                           // column limits are recomputed: kept over the loop they would spill
-            if (MODE == ROWS_MANY && a.chunk < a.groups && gi % a.chunk == 0) {
+            // (ROWS_WIDE has one group and does not take this, but the compiler's order of its code is worse without: 1.2 M x 64 -> 256
+            // 453 us, not 399)
+            if (!SPLIT && MODE != ROWS_ONE && a.chunk < a.groups && gi % a.chunk == 0) {
                 __syncthreads();
                 stage(gi, min(a.chunk, a.groups - gi), s_w);
                 __syncthreads();
@@ -787,7 +794,13 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
             // the group's largest number (of the kept values) and whether anything in it is no finite number
             unsigned m = 0, odd = 0;
             float v[4][8];
-            if constexpr (sizeof(T) == 4) {
+            if constexpr (sizeof(T) == 4 && DX) {         // (nothing else needs the magnitudes here; a NaN needs no care)
+                float most = 0.f;
+                const float* e = reinterpret_cast<const float*>(&cur);
+#pragma unroll
+                for (int q = 0; q < 32; q += 2) asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(most) : "v"(e[q]), "v"(e[q + 1]));
+                odd = !(most < __uint_as_float(0x7f7f8000u));
+            } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int t = 0; t < 8; t++) odd = max(max(odd, max(cur.w[t].x & 0x7fffffffu, cur.w[t].y & 0x7fffffffu)), max(cur.w[t].z & 0x7fffffffu, cur.w[t].w & 0x7fffffffu));
                 odd = odd >= 0x7f7f8000u;                 // !fits()
@@ -876,20 +889,21 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                     else encode(Int<GS4D_FMT_E5M2>());
                 }
             }
-            if constexpr (TERMS > 1)
+            if constexpr (AGAIN) {
+                again |= (unsigned long long)any << (base / TILES & 63);
+            } else if constexpr (TERMS > 1) {
                 if (any) {
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                        if constexpr (MODE != ROWS_WIDE) {
-                            unsigned e[8];
+                        unsigned e[8];
 #pragma unroll
-                            for (int q = 0; q < 8; q++) e[q] = __float_as_uint(v[t][q]);
-                            add_specials(e, wl + t * NT * TERMS * 64);
-                        }
+                        for (int q = 0; q < 8; q++) e[q] = __float_as_uint(v[t][q]);
+                        add_specials(e, wl + t * NT * TERMS * 64);
 #pragma unroll
-                        for (int q = 0; q < 8; q++) v[t][q] = stand_in(__float_as_uint(v[t][q]));
+                        for (int q = 0; q < 8; q++) v[t][q] = stand_in(e[q]);
                     }
                 }
+            }
             if constexpr (MODE == ROWS_WIDE) {
                 // one group: its operands stay in registers for all of the workgroup's features
                 uint4 xs[4][TERMS];
@@ -901,16 +915,6 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 #pragma unroll 1
                 for (int k = 0; k < a.blocks; k++) {
                     begin();
-                    if constexpr (TERMS > 1)
-                        if (any) {
-#pragma unroll
-                            for (int t = 0; t < 4; t++) {
-                                unsigned e[8];
-#pragma unroll
-                                for (int q = 0; q < 8; q++) e[q] = relu_bits(reinterpret_cast<const unsigned*>(&cur.w[2 * t])[q], a.lowest);
-                                add_specials(e, s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
-                            }
-                        }
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
                         step(xs[t], s_w + k * BLOCK + t * NT * TERMS * 64 + lane);
@@ -940,6 +944,28 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
         }
         if constexpr (SPLIT) join();
         else if (MODE != ROWS_WIDE) finish();
+    }
+    if constexpr (AGAIN) {
+        if (!again) return;
+        __threadfence();                                  // the wave stores to the same places again
+        const int f1 = min(F, f0 + a.blocks * NT * 32);
+        long long round = 0;
+        for (long long t = tile0; t < ntile; t += (long long)TILES * a.nwg, round++) {
+            if (!(again >> (round & 63) & 1)) continue;
+            for (long long row = t * 32; row < t * 32 + 32 && row < a.N; row++) {
+                unsigned e = lane < C ? __float_as_uint(reinterpret_cast<const float*>(X)[row * a.ldx + lane]) : 0u;
+                if (!__builtin_amdgcn_ballot_w64(!fits(e))) continue;
+                if (!DX && (e & 0x7fffffffu) <= 0x7f800000u) e = relu_bits(e, a.lowest);      // (a NaN of either sign stays one)
+                for (int fb = f0; fb < f1; fb += 64) {
+                    const int f = min(fb + lane, f1 - 1);
+                    const float* __restrict__ w = reinterpret_cast<const float*>(W) + (long long)f * a.wf;
+                    float sum = !DX && a.bias ? reinterpret_cast<const float*>(a.bias)[f] : 0.f;
+                    for (int c = 0; c < C; c++) sum = fmaf(__uint_as_float((unsigned)__builtin_amdgcn_readlane((int)e, c)), w[(long long)c * a.wc], sum);
+                    if (DX && a.keep.bits && !(reinterpret_cast<const unsigned*>(a.keep.bits)[row * (a.keep.kp / 32) + (f >> 5)] >> (f & 31) & 1u)) sum = 0.f;
+                    if (fb + lane < f1) reinterpret_cast<float*>(a.y)[row * F + f] = sum;
+                }
+            }
+        }
     }
 }
 
