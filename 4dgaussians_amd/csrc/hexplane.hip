@@ -180,8 +180,8 @@ __device__ __forceinline__ float frame_time(const FrameTime& a, long long p)
     const float f = a.force[p * a.stride];
     return (a.use_time ? v : v * 0.0f) * a.ft_w[0] + (a.use_force ? f : f * 0.0f) * a.ft_w[1] + a.ft_b[0];
 }
-// the cache row of row p: the rows of a call may be several copies of the cache's points
-__device__ __forceinline__ long long cache_row(long long p, long long P, unsigned rows) { return P > rows ? (long long)((unsigned)p % rows) : p; }
+// the cache row of row p: the rows of a call may be several copies of the cache's points (P is an int where it is above `rows`)
+__device__ __forceinline__ long long cache_row(long long p, long long P, long long rows) { return P > rows ? (long long)((unsigned)p % (unsigned)rows) : p; }
 
 struct FramePlanes { const float* p[GS4D_MAX_LEVELS * 3]; int w[GS4D_MAX_LEVELS * 3]; int h[GS4D_MAX_LEVELS * 3]; };
 
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256) void frame_features_kernel(gs4d_rows8 c, int L
         u[a] = (xyz[3 * p + a] - lo) * (2.0f / (hi - lo)) - 1.0f;
     }
     const float tt = frame_time(ft, p);
-    const long long row = cache_row(p, P, (unsigned)c.capacity);
+    const long long row = cache_row(p, P, c.capacity);
     const int ng = (c.width + c.group - 1) / c.group, q = C >> 2;
     for (int l = 0; l < L; l++) {
         const int col = l * C + 4 * sub;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(512) void frame_lines_kernel(FrameArgs a)
     struct Point { float x[3], s[L]; unsigned k[L]; } cur, nxt;
     auto load = [&](Point& o, long long p) {
         p = p < a.P ? p : a.P - 1;
-        const long long row = cache_row(p, a.P, (unsigned)a.c.capacity);
+        const long long row = cache_row(p, a.P, a.c.capacity);
 #pragma unroll
         for (int k = 0; k < 3; k++) o.x[k] = a.xyz[3 * p + k];
 #pragma unroll

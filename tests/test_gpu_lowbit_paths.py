@@ -1,0 +1,41 @@
+"""Calls of the 8-bit operators that only some sizes, streams or modes reach, on the GPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import pkg
+from oracle import lowbit_ref as R
+from test_gpu_lowbit import DTYPES, check_linear, f32, leaf, lb, make, near, np64, rows, same
+
+pytestmark = pytest.mark.gpu
+
+
+def raw_frame(cache, capacity, planes, aabb, pts, t):
+    """gs4d_frame_features with a cache that says it has `capacity` rows; the call reads the first len(pts) of them."""
+    n, ch = pts.shape[0], planes[0].shape[1]
+    d = type(cache._desc).from_buffer_copy(cache._desc)
+    d.capacity = capacity
+    out = torch.empty(n, cache.width, device="cuda")
+    rc = pkg("_cabi").lib().gs4d_frame_features(
+        C.addressof(d), len(planes) // 3, ch, (C.c_void_p * len(planes))(*[p.data_ptr() for p in planes]),
+        (C.c_int * len(planes))(*[p.shape[3] for p in planes]), (C.c_int * len(planes))(*[p.shape[2] for p in planes]),
+        aabb.data_ptr(), pts.data_ptr(), t.data_ptr(), 0 if t.numel() == 1 else 1, n, out.data_ptr(), cache.width,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return out
+
+
+@pytest.mark.parametrize("n,ch", [(9, 4), (8200, 256)])               # the general kernel, and lines blended first
+def test_frame_features_of_a_cache_of_more_than_32_bits_of_rows(n, ch):
+    g = torch.Generator().manual_seed(n)
+    c = lb().RowCache(n, ch)
+    c.write((0.1 + torch.rand(n, ch, generator=g)).cuda())
+    planes = [(0.5 + torch.rand(1, 5, 7, ch, generator=g)).permute(0, 3, 1, 2).cuda() for _ in range(3)]
+    aabb = torch.tensor([[1.3, 1.2, 1.1], [-1.3, -1.2, -1.0]]).cuda()
+    pts, t = (torch.rand(n, 3, generator=g) * 2 - 1).cuda(), torch.tensor([0.25], device="cuda")
+    want = lb().frame_features(c, planes, aabb, pts, t)
+    assert len(want.unique(dim=0)) > 5
+    for capacity in (n, 2 ** 31 + 5, 2 ** 32, 2 ** 32 + 5):
+        assert torch.equal(raw_frame(c, capacity, planes, aabb, pts, t), want), capacity
