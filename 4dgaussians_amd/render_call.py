@@ -51,6 +51,18 @@ def _usable(t) -> bool:
     return t.dtype == torch.float32 and t.device.type == "cuda" and t.is_contiguous() and t.data_ptr() % 16 == 0
 
 
+def one_value_column(n, value, device):
+    """An (n, 1) column of one value that says so (_one_value), for as long as nothing is written to it."""
+    t = torch.full((n, 1), value, dtype=torch.float32, device=device)
+    t.one_value_version = t._version
+    return t
+
+
+def _one_value(t):
+    v = getattr(t, "one_value_version", None)
+    return v is not None and v == t._version
+
+
 class RenderCall:
     """Everything of one render() call that is not a differentiable tensor: the camera, the per-point time / force
     columns, the optional L1 target and the data-parallel hooks."""
@@ -59,7 +71,7 @@ class RenderCall:
 
     def __init__(self, cam, bg, scale_modifier, sh_degree, debug, deform_net, time, force, target, shs_grad_hook):
         self.grad = torch.is_grad_enabled()          # the autograd function's forward cannot see it
-        self.uniform_time = bool(getattr(type(cam), "uniform_columns", False))       # one time and force for all rows
+        self.uniform_time = _one_value(time) and _one_value(force)
         self.H, self.W = int(cam.image_height), int(cam.image_width)
         self.tanfovx, self.tanfovy = math.tan(cam.FoVx * 0.5), math.tan(cam.FoVy * 0.5)
         self.bg, self.view, self.proj, self.campos = bg, cam.world_view_transform, cam.full_proj_transform, cam.camera_center

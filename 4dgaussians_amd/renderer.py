@@ -19,7 +19,7 @@ import torch.nn as nn
 
 from .diff_gaussian_rasterization import GaussianRasterizationSettings, GaussianRasterizer, _shared_zeros
 from .fused import activate
-from .render_call import RenderCall, render_call, render_step
+from .render_call import RenderCall, one_value_column, render_call, render_step
 
 
 class GaussianParams(nn.Module):
@@ -37,8 +37,6 @@ class GaussianParams(nn.Module):
 
 
 class Camera:
-    uniform_columns = True                       # time_force_columns() holds one time and one force in all rows
-
     def __init__(self, cam, device, time: float = 0.0, force: float = 0.0):
         self.image_width, self.image_height = cam.image_width, cam.image_height
         self.FoVx, self.FoVy = cam.FoVx, cam.FoVy
@@ -55,8 +53,8 @@ class Camera:
         cols = self._columns.get(key)
         if cols is None:
             self._columns.clear()
-            cols = self._columns[key] = (torch.full((n, 1), self.time, dtype=torch.float32, device=device),
-                                         torch.full((n, 1), self.force, dtype=torch.float32, device=device))
+            with torch.inference_mode(False):    # tensors whose changes are counted
+                cols = self._columns[key] = tuple(one_value_column(n, v, device) for v in (self.time, self.force))
         return cols
 
 

@@ -50,3 +50,54 @@ def test_the_fused_optimizer_changes_versions():
     opt.step()
     with pytest.raises(RuntimeError, match="modified in place"):
         out[0].sum().backward()
+
+
+def test_frozen_frame_of_a_camera_with_a_time_per_row():
+    """Which frames have one time is read off the columns themselves, not off the camera's class."""
+    wl, rd = pkg("workload"), pkg("renderer")
+    sc = wl.build_scene("C1", torch.device("cuda"), P=3000)
+    net, pc, cam, bg = sc["deform"], sc["pc"], sc["cam"], sc["bg"]
+    g = torch.Generator().manual_seed(0)
+    times = torch.rand(3000, 1, generator=g).cuda()
+    one = torch.full((3000, 1), cam.time, device="cuda"), torch.full((3000, 1), cam.force, device="cuda")
+
+    class Rolling(type(cam)):
+        def time_force_columns(self, n, device):
+            return times, one[1]
+
+    def frame(c, t, f):
+        """(the frame, the same from a query of the field and a scene without one)"""
+        q = net.forward_dynamic(pc._xyz, pc._scaling, pc._rotation, pc._opacity, pc._features, t, f, None)
+        still = type("Still", (), dict(zip(("_xyz", "_scaling", "_rotation", "_opacity", "_features"), q), active_sh_degree=pc.active_sh_degree))
+        return rd.render_for_image(c, pc, net, bg), rd.render_for_image(c, still, None, bg)
+    rolling = copy.copy(cam)
+    rolling.__class__ = Rolling
+    with torch.no_grad():
+        net.freeze_planes(pc._xyz)
+        got, want = frame(rolling, times, one[1])
+        assert torch.equal(got, want)
+        plain, want1 = frame(cam, *one)
+        assert torch.equal(plain, want1) and not torch.equal(plain, got)
+        cam.time_force_columns(3000, pc._xyz.device)[0].copy_(times)  # the camera's own columns, written to
+        assert torch.equal(rd.render_for_image(cam, pc, net, bg), want)
+        cam._columns.clear()
+    with torch.inference_mode():
+        assert torch.equal(rd.render_for_image(cam, pc, net, bg), plain)
+        t, f = cam.time_force_columns(3000, pc._xyz.device)
+        assert not t.is_inference() and t.one_value_version == t._version
+
+
+def test_frozen_frame_of_columns_made_in_inference_mode():
+    """Tensors without a version are columns like any others."""
+    wl, rd = pkg("workload"), pkg("renderer")
+    sc = wl.build_scene("C1", torch.device("cuda"), P=500)
+    net, pc, cam, bg = sc["deform"], sc["pc"], sc["cam"], sc["bg"]
+
+    class Own(type(cam)):
+        def time_force_columns(self, n, device):
+            return torch.full((n, 1), self.time, device=device), torch.full((n, 1), self.force, device=device)
+    own = copy.copy(cam)
+    own.__class__ = Own
+    with torch.inference_mode():
+        net.freeze_planes(pc._xyz)
+        assert torch.equal(rd.render_for_image(own, pc, net, bg), rd.render_for_image(cam, pc, net, bg))
