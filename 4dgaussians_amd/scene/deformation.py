@@ -511,6 +511,7 @@ class Deformation(nn.Module):
             raise RuntimeError("the planes were modified after freeze_planes(): freeze them again or call thaw_planes()")
         if frozen is not None:
             c = frozen[0]
+            self._hold_frozen(c, frozen[2])
             d.static_codes, d.static_scales = c.codes.data_ptr(), c.scales.data_ptr()
             d.static_rows, d.static_pitch, d.static_group, d.static_fmt = c.capacity, c.codes.shape[1], c.group, FORMATS[c.fmt]
         else:
@@ -524,8 +525,7 @@ class Deformation(nn.Module):
         Queries are then of these points (P rows, or several copies of them as render_batch makes) until thaw_planes() or the
         first query with gradients enabled; a change of bounds or device thaws as well.  Planes whose version has changed since (in
         place, or by an optimizer) make the next query raise; a replayed graph that trains and a write through `.data` change no
-        version: thaw after them.  The features are off by at most half a step of the format (int8: 1 / 254 of the largest of 64
-        neighbouring ones)."""
+        version: thaw after them.  The features are off by at most half a step of the format (int8: 1 / 254 of the largest of 64 neighbouring ones)."""
         self.thaw_planes()
         if not isinstance(points, torch.Tensor) or points.dim() != 2 or points.shape[1] != 3 or points.shape[0] < 1 or points.dtype != torch.float32:
             raise RuntimeError("freeze_planes: points must be float32 [P, 3] with at least one row")
@@ -550,8 +550,17 @@ class Deformation(nn.Module):
                                             C.c_void_p(rows.data_ptr()), _cabi.current_stream(dev))
             _cabi.check(rc, "gs4d_static_features")
             cache.write(rows[:n], start=r0)
-        self.__dict__["_frozen"] = (cache, [p._version for p in params[:plan.n_planes]])
+        self.__dict__["_frozen"] = (cache, [p._version for p in params[:plan.n_planes]], _cabi.stream_of(dev))
         return cache
+
+    def _hold_frozen(self, cache, stream):
+        """A query is about to read the cache on the current stream.  Its memory came from another one, perhaps, and thaw_planes(),
+        which training calls by itself, may free it while that query runs."""
+        with _cabi.on_device(cache.device):
+            if _cabi.stream_of(cache.device) != stream:
+                s = torch.cuda.current_stream(cache.device)
+                cache.codes.record_stream(s)
+                cache.scales.record_stream(s)
 
     def thaw_planes(self):
         """Queries sample all six planes again."""

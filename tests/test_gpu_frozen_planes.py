@@ -101,3 +101,25 @@ def test_frozen_frame_of_columns_made_in_inference_mode():
     with torch.inference_mode():
         net.freeze_planes(pc._xyz)
         assert torch.equal(rd.render_for_image(own, pc, net, bg), rd.render_for_image(cam, pc, net, bg))
+
+
+def test_thawing_does_not_take_the_cache_from_a_frame_on_another_stream():
+    net = field(32)
+    x, t, f, ws = inputs(4000)
+    args = [x[k] for k in NAMES]
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        cache = net.freeze_planes(x["points"])
+        sizes = [cache.codes.shape, cache.scales.shape]
+        del cache
+        want = [o.clone() for o in net.forward_dynamic(*args, t, f, None)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)                            # some 50 ms before the frame's turn
+            got = net.forward_dynamic(*args, t, f, None)
+    step(net, x, t, f, ws)                                            # thaws by itself
+    assert "_frozen" not in net.deformation_net.__dict__
+    others = [torch.full(s, 77, dtype=d, device="cuda") for s, d in zip(sizes, (torch.uint8, torch.float32)) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del others
