@@ -477,6 +477,7 @@ class Deformation(nn.Module):
         state.pop("_step_cache", None)
         state.pop("_hex_order_cache", None)
         state.pop("_frozen", None)
+        state.pop("_captured", None)
         return state
 
     def _apply(self, fn, *a, **k):                 # .to() / .cuda() / .float(): parameters may get new storage
@@ -525,7 +526,8 @@ class Deformation(nn.Module):
         Queries are then of these points (P rows, or several copies of them as render_batch makes) until thaw_planes() or the
         first query with gradients enabled; a change of bounds or device thaws as well.  Planes whose version has changed since (in
         place, or by an optimizer) make the next query raise; a replayed graph that trains and a write through `.data` change no
-        version: thaw after them.  The features are off by at most half a step of the format (int8: 1 / 254 of the largest of 64 neighbouring ones)."""
+        version: thaw after them.  A captured query goes on reading the cache it was captured with, which is kept for it.  The
+        features are off by at most half a step of the format (int8: 1 / 254 of the largest of 64 neighbouring ones)."""
         self.thaw_planes()
         if not isinstance(points, torch.Tensor) or points.dim() != 2 or points.shape[1] != 3 or points.shape[0] < 1 or points.dtype != torch.float32:
             raise RuntimeError("freeze_planes: points must be float32 [P, 3] with at least one row")
@@ -555,9 +557,13 @@ class Deformation(nn.Module):
 
     def _hold_frozen(self, cache, stream):
         """A query is about to read the cache on the current stream.  Its memory came from another one, perhaps, and thaw_planes(),
-        which training calls by itself, may free it while that query runs."""
+        which training calls by itself, may free it while that query runs; a captured query reads it whenever it is replayed."""
         with _cabi.on_device(cache.device):
-            if _cabi.stream_of(cache.device) != stream:
+            if torch.cuda.is_current_stream_capturing():
+                held = self.__dict__.setdefault("_captured", [])       # for as long as the module lives
+                if not any(c is cache for c in held):
+                    held.append(cache)
+            elif _cabi.stream_of(cache.device) != stream:
                 s = torch.cuda.current_stream(cache.device)
                 cache.codes.record_stream(s)
                 cache.scales.record_stream(s)

@@ -123,3 +123,28 @@ def test_thawing_does_not_take_the_cache_from_a_frame_on_another_stream():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     del others
+
+
+def test_a_captured_frame_keeps_its_cache():
+    net = field(32)
+    x, t, f, ws = inputs(700)
+    args = [x[k] for k in NAMES]
+    with torch.no_grad():
+        cache = net.freeze_planes(x["points"])
+        sizes = [cache.codes.shape, cache.scales.shape]
+        del cache
+        want = [o.clone() for o in net.forward_dynamic(*args, t, f, None)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = net.forward_dynamic(*args, t, f, None)
+    step(net, x, t, f, ws)
+    others = [torch.full(s, 77, dtype=d, device="cuda") for s, d in zip(sizes, (torch.uint8, torch.float32)) for _ in range(8)]
+    for _ in range(3):
+        for o in (got[0], got[1], got[2], got[4]):                    # (the opacity is the caller's own tensor)
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        step(net, x, t, f, ws)
+    assert copy.deepcopy(net).deformation_net.__dict__.get("_captured") is None
+    del others
