@@ -132,18 +132,21 @@ class RowCache:
         if (self.width > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < self.width):
             rows = rows.contiguous()
         ref = self._ref
-        if slots is not None and n > SCAN:
-            if torch.cuda.is_current_stream_capturing():
-                # an array of the graph's own: its zeros are written when the graph runs, and it lives as long as the graph
-                owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
-                d = Rows8.from_buffer_copy(self._desc)
-                d.owner, ref = owner.data_ptr(), C.addressof(d)
-            elif self._owner is None:
-                self._owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
-                self._desc.owner = self._owner.data_ptr()
         with _cabi.on_device(self.device):
+            stream = _cabi.stream_of(self.device)
+            if slots is not None and n > SCAN:
+                if torch.cuda.is_current_stream_capturing():
+                    # an array of the graph's own: its zeros are written when the graph runs, and it lives as long as the graph
+                    owner = torch.zeros(self.capacity, dtype=torch.int32, device=self.device)
+                    d = Rows8.from_buffer_copy(self._desc)
+                    d.owner, ref = owner.data_ptr(), C.addressof(d)
+                elif self._owner is None:
+                    self._owner, self._owner_stream = torch.zeros(self.capacity, dtype=torch.int32, device=self.device), stream
+                    self._desc.owner = self._owner.data_ptr()
+                elif stream != self._owner_stream:
+                    self._owner.record_stream(torch.cuda.current_stream(self.device))      # the caller cannot, and may drop the cache
             rc = _cabi.lib().gs4d_rows8_write(ref, rows.data_ptr(), dt, rows.stride(0) if n > 1 else self.width, n, p, size,
-                                              int(start), _cabi.stream_of(self.device))
+                                              int(start), stream)
         if rc:
             _cabi.check(rc, "gs4d_rows8_write")
 

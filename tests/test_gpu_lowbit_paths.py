@@ -39,3 +39,23 @@ def test_frame_features_of_a_cache_of_more_than_32_bits_of_rows(n, ch):
     assert len(want.unique(dim=0)) > 5
     for capacity in (n, 2 ** 31 + 5, 2 ** 32, 2 ** 32 + 5):
         assert torch.equal(raw_frame(c, capacity, planes, aabb, pts, t), want), capacity
+
+
+def test_a_write_on_another_stream_outlives_its_cache_object():
+    """The caller keeps codes and scales; the helper array of many scattered rows goes with the object, but not before the write."""
+    codes, scales = torch.zeros(5000, 64, dtype=torch.uint8, device="cuda"), torch.zeros(5000, 1, device="cuda")
+    x = rows(3000, 64).cuda()
+    slots = torch.randint(0, 5000, (3000,), generator=torch.Generator().manual_seed(1)).cuda()
+    want = f32(R.write(np.zeros((5000, 64)), np64(x), slots.tolist(), "int8", 64))
+    c = lb().RowCache.from_buffers(codes, scales, 64)
+    c.write(torch.zeros_like(x), slots)                               # the helper array comes from this stream
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        c.write(x, slots)
+    del c
+    others = [torch.full((5000,), 2 ** 30, dtype=torch.int32, device="cuda") for _ in range(16)]       # who may have the memory now
+    torch.cuda.synchronize()
+    same(lb().RowCache.from_buffers(codes, scales, 64).read(), want)
+    assert all((o == 2 ** 30).all().item() for o in others)
