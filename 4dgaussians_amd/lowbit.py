@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
@@ -273,7 +274,7 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
     """act(x) @ weight.T + bias with act = relu or nothing: x [..., K], weight [M, K], bias [M], all of one dtype (float32,
     bfloat16 or float16; sums in float32).  For the backward it keeps act(x) in 8 bits in groups of 64 columns ("int8": 255
     levels of a rectified input, 127 each way of a signed one) and, with relu, the signs of x -- a byte or so per number
-    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  At most 2^28 weights, K and M at most 2^20."""
+    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  No forward-mode derivative.  At most 2^28 weights, K and M at most 2^20."""
     f = _format(fmt)
     _on_device("x", x)
     _on_device("weight", weight, x.device)
@@ -286,6 +287,8 @@ def linear(x, weight, bias=None, relu=False, fmt="int8"):
         _on_device("bias", bias, x.device)
         if bias.dtype != x.dtype or tuple(bias.shape) != (weight.shape[0],):
             raise RuntimeError(f"linear: bias must be {x.dtype} [{weight.shape[0]}], got {bias.dtype} {tuple(bias.shape)}")
+    if forward_ad._current_level >= 0 and any(v is not None and forward_ad.unpack_dual(v).tangent is not None for v in (x, weight, bias)):
+        raise RuntimeError("linear has no forward-mode derivative; an operand has a tangent")
     relu = int(bool(relu))
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _Linear.apply(x, weight, bias, relu, f)

@@ -59,3 +59,19 @@ def test_a_write_on_another_stream_outlives_its_cache_object():
     torch.cuda.synchronize()
     same(lb().RowCache.from_buffers(codes, scales, 64).read(), want)
     assert all((o == 2 ** 30).all().item() for o in others)
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_linear_refuses_operands_with_tangents(needs_grad):
+    from torch.autograd import forward_ad
+    x, w, b = (t.cuda().requires_grad_(needs_grad) for t in make(6, 8, 4, torch.float32)[:3])
+    y = lb().linear(x, w, b)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [x, w, b]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                lb().linear(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                lb().linear(*args)
+        assert torch.equal(lb().linear(x, w, b), y)                   # without a tangent: as ever
