@@ -263,7 +263,7 @@ class _DeformFunction(torch.autograd.Function):
             ws = kept
         ctx.cfg = cfg
         ctx.plan = plan
-        ctx.kept8 = kept8
+        ctx.kept8, ctx.chunks = kept8, chunks      # the backward reads the checkpoint where this forward put it
         if plan is not None:
             # the parameters are not re-read through saved_tensors (50 unpacks per step); their versions are kept
             # instead, so that an in-place update between forward and backward is still refused
@@ -318,7 +318,7 @@ class _DeformFunction(torch.autograd.Function):
             g_shs = g_shs.clone()
         d_xyz, d_sc, d_rot = (torch.empty_like(t) for t in (points_, scales_, rot_))
         d_shs = g_shs            # shs' = shs + delta: the input gradient IS the upstream gradient (the C ABI allows the alias)
-        chunks = _DeformFunction._chunks(L, d, P) if ctx.kept8 else [(0, P, 0)]
+        chunks = ctx.chunks
         most = chunks[0][1]
         scratch = torch.empty(max(int(L.gs4d_deform_backward_scratch_bytes(C.byref(d), C.c_int(most))), 256),
                               dtype=torch.uint8, device=dev)
