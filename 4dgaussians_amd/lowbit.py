@@ -273,14 +273,20 @@ class _Linear(torch.autograd.Function):
 def linear(x, weight, bias=None, relu=False, fmt="int8"):
     """act(x) @ weight.T + bias with act = relu or nothing: x [..., K], weight [M, K], bias [M], all of one dtype (float32,
     bfloat16 or float16; sums in float32).  For the backward it keeps act(x) in 8 bits in groups of 64 columns ("int8": 255
-    levels of a rectified input, 127 each way of a signed one) and, with relu, the signs of x -- a byte or so per number
-    instead of x.  The input gradient is exact; the weight gradient is taken with the kept values.  No forward-mode derivative.  At most 2^28 weights, K and M at most 2^20."""
+    levels of a rectified input, 127 each way of a signed one) and, with relu, the signs of x, instead of x.  The input gradient
+    is exact; the weight gradient is taken with the kept values.  Operands of several types are cast to autocast's under autocast
+    and refused outside of it; operands of one type are taken as they are.  No forward-mode derivative.  At most 2^28 weights, K
+    and M at most 2^20."""
     f = _format(fmt)
     _on_device("x", x)
     _on_device("weight", weight, x.device)
     _dtype("x", x)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise RuntimeError(f"linear: x [..., K] and weight [M, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if (weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype)) and torch.is_autocast_enabled("cuda") \
+            and all(v is None or v.dtype in DTYPES for v in (weight, bias)):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
     if weight.dtype != x.dtype:
         raise RuntimeError(f"linear: x is {x.dtype}, weight {weight.dtype}")
     if bias is not None:

@@ -75,3 +75,25 @@ def test_linear_refuses_operands_with_tangents(needs_grad):
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 lb().linear(*args)
         assert torch.equal(lb().linear(x, w, b), y)                   # without a tangent: as ever
+
+
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+def test_linear_under_autocast(low):
+    x, w, b, dy = make(70, 40, 20, torch.float32)
+    xs, ws, bs = leaf(x), leaf(w), leaf(b)
+    cast = [t.detach().to(low).requires_grad_(True) for t in (xs, ws, bs)]
+    y0 = lb().linear(*cast, relu=True)
+    want = torch.autograd.grad(y0, cast, dy.cuda().to(low))
+    with torch.autocast("cuda", low):
+        for args in ((cast[0], ws, bs), (xs, cast[1], bs), (xs, cast[1], cast[2]), (cast[0], cast[1], bs)):
+            y = lb().linear(*args, relu=True)
+            assert y.dtype is low and torch.equal(y, y0)
+            got = torch.autograd.grad(y, args, dy.cuda().to(low))
+            assert all(g.dtype is a.dtype and torch.equal(g.to(low), v) for g, a, v in zip(got, args, want))
+        assert lb().linear(xs, ws, bs).dtype is torch.float32         # one type: as it is
+        for bad in ((xs.double(), ws, bs), (xs, ws.double(), bs), (xs, ws, bs.double())):
+            with pytest.raises(RuntimeError):
+                lb().linear(*bad)
+    for args in ((cast[0], ws, bs), (xs, ws, cast[2])):
+        with pytest.raises(RuntimeError):
+            lb().linear(*args)
