@@ -674,6 +674,7 @@ int gs4d_rows8_read(const gs4d_rows8* c, void* out, int dtype, long long ld, lon
  *   GS4D_KEEP_CODES  act(x) in 8 bits in groups of 64 columns (int8 becomes uint8 with relu): the weight gradient's operand
  *   GS4D_KEEP_SIGNS  a bit per value, x > 0 (relu only): the input gradient's mask
  * as `what` says (0: nothing, keep may be NULL).
+ * K counts as a multiple of 64: 64 bytes of codes, a scale of 4 bytes and 8 bytes of signs per row and group.
  */
 #define GS4D_KEEP_CODES 1
 #define GS4D_KEEP_SIGNS 2
