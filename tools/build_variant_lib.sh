@@ -8,7 +8,7 @@ cd 4dgaussians_amd/csrc
 make -s
 base=${file%.hip}
 strict=""
-case "$base" in preprocess|geom_bwd|knn|binning|train_step) strict="-ffp-contract=off";; esac
+case "$base" in preprocess|geom_bwd|knn|binning|train_step|lowbit) strict="-ffp-contract=off";; hexplane) strict="-fno-slp-vectorize";; esac   # as csrc/Makefile has them
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wall -Wno-unused-function -I../../include $strict $extra -c $file -o /tmp/${base}_$suffix.o
 objs=$(ls *.o | grep -v "^$base.o$")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../libgs4d_$suffix.so $objs /tmp/${base}_$suffix.o
