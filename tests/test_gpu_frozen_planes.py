@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from conftest import pkg
+from oracle import deformation_ref as R
+from oracle import lowbit_ref as Q
 from test_gpu_lowbit_field import field, inputs, step
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +150,35 @@ def test_a_captured_frame_keeps_its_cache():
         step(net, x, t, f, ws)
     assert copy.deepcopy(net).deformation_net.__dict__.get("_captured") is None
     del others
+
+
+@pytest.mark.parametrize("channels,P,copies", [(32, 65_600, 1), (64, 32_800, 1), (16, 70_001, 2)])
+@pytest.mark.parametrize("use_time,use_force", [(True, False), (True, True), (False, True), (False, False)])
+def test_frozen_frames_of_so_many_points_that_lines_are_blended(channels, P, copies, use_time, use_force, monkeypatch):
+    """One time and one force for all rows, of one view and of several, against the network on what the cache holds at some rows, and
+    against the query with a time per row at all of them."""
+    kw = dict(use_time=use_time, use_force=use_force)
+    net = field(32, 1, channels, (1, 2), **kw)
+    x, t, f, _ = inputs(P)
+    many = [torch.cat([x[k]] * copies) for k in NAMES]
+    n = P * copies
+    with torch.no_grad():
+        cache = net.freeze_planes(x["points"])
+        one = net.forward_dynamic(*many, t[:1].expand(n, 1), f[:1].expand(n, 1), None)
+        each = net.forward_dynamic(*many, t[:1].repeat(n, 1), f[:1].repeat(n, 1), None)
+    at = torch.cat([torch.arange(400), torch.arange(n - 400, n), torch.randint(0, n, (700,), generator=torch.Generator().manual_seed(P))])
+    held = cache.read(at.cuda() % P).cpu().double().numpy()
+    sd = {k: v.detach().cpu().double() for k, v in net.state_dict().items()}
+    cfg = R.DeformConfig(plane_channels=channels, resolution=[24, 20, 16, 9], multires=[1, 2], defor_depth=1, **kw)
+    G = "deformation_net.grid."
+    times = [sd[f"{G}grids.{lv}.{i}"][0].numpy() for lv in range(2) for i in (2, 4, 5)]
+    monkeypatch.setattr(R, "hexplane_features", lambda sd_, cfg_, xyz, tp: torch.from_numpy(
+        Q.frame_features(held, times, sd[G + "aabb"].numpy(), xyz.numpy(), tp[:, 0].numpy())))
+    sub = [a.cpu()[at].double() for a in many]
+    want = R.forward_dynamic(sd, cfg, *sub, torch.full((len(at), 1), float(t[0])).double(), torch.full((len(at), 1), float(f[0])).double())
+    for k, (a, e, w) in enumerate(zip(one, each, want)):
+        tol = 1e-5 * max(1.0, float(w.abs().max()))                   # the float32 path's forward tolerance
+        if k == 2:                                                    # a rotation is divided by the norm of what the head gives
+            tol *= 20
+        assert float((a.cpu()[at].double() - w).abs().max()) <= tol, k
+        assert float((a - e).abs().max()) <= 2 * tol, k

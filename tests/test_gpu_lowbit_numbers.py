@@ -9,7 +9,7 @@ import torch
 
 from conftest import pkg
 from oracle import lowbit_ref as R
-from test_gpu_lowbit import DTYPES, leaf, lb, np64, rows
+from test_gpu_lowbit import DTYPES, leaf, lb, make, near, np64, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -233,3 +233,86 @@ def test_numbers_next_to_the_largest(n, c, f):
     x3[0, :], w3[1 % f, :] = big.max, float("inf")
     x3[1, :] = float("-inf")
     assert (_plain(x3, w3).cpu()[0, 1 % f] == float("inf")) and (_plain(x3, w3).cpu()[1, 1 % f] == float("-inf"))
+
+
+def chunk_rows(n, k, m):
+    groups, tiles = -(-k // 64), -(-m // 64)
+    gw = 8 if groups >= 8 else 4 if groups >= 4 else 2 if groups >= 2 else 1
+    chunks = max(1, min(256 // (tiles * -(-groups // gw)), -(-n // 128)))
+    return -(-(-(-n // chunks)) // 128) * 128
+
+
+SUMS = [(70_001, 64, 64), (40_007, 200, 70), (33_000, 520, 20), (5000, 64, 64), (129, 70, 33), (17, 64, 64), (16, 64, 5), (15, 64, 2), (1, 64, 1)]
+
+
+@pytest.mark.parametrize("n,k,m", SUMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_row_is_in_the_weight_gradient_once(n, k, m, dtype):
+    """Whole numbers: scales of 1, codes of at most 127, dy of -1, 0 and 1.  Every partial sum is below 2^24 (70 001 x 127), so the
+    result does not depend on the order and is compared for equality, in the 16-bit types after its one rounding."""
+    g = torch.Generator().manual_seed(n + k + m)
+    x = torch.randint(-127, 128, (n, k), generator=g).float()
+    x[:, ::64] = 127                                                  # every group's largest: a scale of 1
+    dy = torch.randint(-1, 2, (n, m), generator=g).float()
+    dy[-1] = 1
+    ws, bs = leaf(torch.zeros(m, k, dtype=dtype)), leaf(torch.zeros(m, dtype=dtype))
+    dw, db = torch.autograd.grad(lb().linear(x.to(dtype).cuda(), ws, bs), (ws, bs), dy.to(dtype).cuda())
+    assert torch.equal(dw.cpu(), (dy.double().T @ x.double()).to(dtype)) and torch.equal(db.cpu(), dy.double().sum(0).to(dtype))
+    db1, = torch.autograd.grad(lb().linear(x.to(dtype).cuda(), ws.detach(), bs), bs, dy.to(dtype).cuda())
+    assert torch.equal(db1, db)
+
+
+@pytest.mark.parametrize("n,k,m", SUMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_rows_at_every_border_are_whole(n, k, m, dtype):
+    """One row per column of dy is not zero -- the first and last of steps of 16 and of chunks, and of all -- with a number of all the
+    type's bits; codes are powers of two, so the sum is exact: a lost row, or a lost term of dy, is all of the result or its last bits."""
+    per = chunk_rows(n, k, m)
+    at = {0, n - 1, n - 2, n - 15, n - 16, n - 17, 15, 16}
+    for b in range(per, n + per, per):
+        at |= {b - 17, b - 16, b - 1, b, b + 15, b + 16}
+    at = sorted(r for r in at if 0 <= r < n)
+    bits = {torch.float32: 24, torch.bfloat16: 8, torch.float16: 11}[dtype]
+    x = 2.0 ** ((torch.arange(n)[:, None] * 5 + torch.arange(k)) % 7).float()
+    x[:, ::64] = 127
+    for i in range(0, len(at), m):
+        dy, want = torch.zeros(n, m), torch.zeros(m, k, dtype=torch.float64)
+        for c, r in enumerate(at[i:i + m]):
+            dy[r, c] = (2 ** bits - 1 - 2 * (c % 50)) * 2.0 ** (-bits)
+            want[c] = dy[r, c].double() * x[r].double()
+        ws, bs = leaf(torch.zeros(m, k, dtype=dtype)), leaf(torch.zeros(m, dtype=dtype))
+        dw, db = torch.autograd.grad(lb().linear(x.to(dtype).cuda(), ws, bs), (ws, bs), dy.to(dtype).cuda())
+        exact = torch.ones(k, dtype=torch.bool)
+        exact[::64] = False                                           # times 127: rounded
+        assert torch.equal(dw.cpu()[:, exact], want[:, exact].to(dtype)) and torch.equal(db.cpu(), dy.sum(0).to(dtype))
+
+
+@pytest.mark.parametrize("n,k,m", [(70_001, 64, 64), (40_007, 200, 70), (33_000, 520, 20)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_of_many_rows(n, k, m, dtype):
+    g = torch.Generator().manual_seed(n)
+    x, dy = rows(n, k, dtype, seed=n), (1e-2 * torch.randn(n, m, generator=g)).to(dtype)
+    ws, bs = leaf(torch.zeros(m, k, dtype=dtype)), leaf(torch.zeros(m, dtype=dtype))
+    dw, db = torch.autograd.grad(lb().linear(x.cuda(), ws, bs, relu=True), (ws, bs), dy.cuda())
+    kept, D = R.quantise(np.maximum(np64(x), 0), "uint8", 64)[0], np64(dy)
+    depth = weight_gradient_roundings(n, k, m)
+    for got, want, most in ((dw, D.T @ kept, np.abs(D).T @ kept), (db, D.sum(0), np.abs(D).sum(0))):
+        tol = depth * 2.0 ** -24 * most
+        if dtype is not torch.float32:
+            tol = tol + np.abs(want) * torch.finfo(dtype).eps / 2 + float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
+        assert (np.abs(np64(got) - want) <= tol).all(), (np.abs(np64(got) - want) / tol).max()
+        if dtype is torch.float32:                                    # what a lost step of 16 rows would be is well above the tolerance
+            assert (np.abs(D[-17:-1].T @ kept[-17:-1]) > 3 * tol).mean() > 0.5 if got is dw else True
+
+
+@pytest.mark.parametrize("n,k,m,dtype", [(20_000, 450, 450, torch.float32), (70_000, 512, 66, torch.float32), (70_000, 66, 450, torch.float32),
+                                         (45_000, 700, 300, torch.bfloat16), (45_000, 300, 700, torch.float16)])
+def test_a_weight_that_does_not_fit_over_several_rounds(n, k, m, dtype):
+    """The contraction's groups pass through LDS in portions, again for each round of rows: every one of forward and input gradient."""
+    x, w, b, dy = make(n, k, m, dtype)
+    xs = leaf(x)
+    y = lb().linear(xs, w.cuda(), b.cuda(), relu=True)
+    dx, = torch.autograd.grad(y, xs, dy.cuda())
+    X, W, D = np.maximum(np64(x), 0), np64(w), np64(dy)
+    near(y, X @ W.T + np64(b), X @ np.abs(W).T + np.abs(np64(b)), k)
+    near(dx, np.where(X > 0, D @ W, 0), np.abs(D) @ np.abs(W), m)

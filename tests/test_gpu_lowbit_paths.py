@@ -97,3 +97,28 @@ def test_linear_under_autocast(low):
     for args in ((cast[0], ws, bs), (xs, ws, cast[2])):
         with pytest.raises(RuntimeError):
             lb().linear(*args)
+
+
+@pytest.mark.parametrize("levels,ch,res,res_t,n", [(1, 4, 1, 1, 524_289), (2, 128, 1, 5, 16_385), (1, 256, 1, 1, 8200), (1, 64, 5000, 3, 32_769),
+                                                   (4, 4, 6000, 2, 524_300), (1, 32, 2500, 4, 65_540)])
+def test_frame_features_of_axes_of_one_and_of_lines_that_do_not_fit(levels, ch, res, res_t, n):
+    """Enough points for blended lines: axes of one texel, lines that leave few channels at once, and lines too long for any."""
+    g = torch.Generator().manual_seed(n)
+    static = 0.1 + torch.rand(n, levels * ch, generator=g) * 2
+    c = lb().RowCache(n, levels * ch, "int8", 64)
+    c.write(static.cuda())
+    planes = [(0.5 + torch.rand(1, res_t, res, ch, generator=g)).permute(0, 3, 1, 2) for _ in range(3 * levels)]
+    aabb = torch.tensor([[1.3, 1.2, 1.1], [-1.3, -1.2, -1.0]])
+    pts = (torch.rand(n, 3, generator=g) * 2 - 1) * 1.6
+    args = [p.cuda() for p in planes], aabb.cuda(), pts.cuda()
+    at = torch.cat([torch.arange(300), torch.arange(n - 300, n), torch.randint(0, n, (400,), generator=g)])
+    held = R.quantise(np64(static[at]), "int8", 64)[0]
+    # a coordinate of at most 4 in units of the axis is off by 8 roundings; a plane of values in [0.5, 1.5] turns an error of d texels
+    # into at most 2 d relative, three planes, two coordinates each; 20 roundings in the products
+    tol = (12 * 8 * 4 * max(res, res_t) + 20) * 2.0 ** -24
+    for t in (torch.tensor([0.3721]), torch.tensor([-2.0])):
+        got = lb().frame_features(c, *args, t.cuda())
+        want = R.frame_features(held, [p[0].numpy() for p in planes], aabb.numpy(), pts[at].numpy(), t.expand(len(at)).numpy())
+        assert np.abs(np64(got.cpu()[at]) / want - 1).max() <= tol
+        each = lb().frame_features(c, *args, t.expand(n).contiguous().cuda())
+        assert (got / each - 1).abs().max().item() <= 2 * tol
