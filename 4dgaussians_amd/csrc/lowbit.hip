@@ -599,17 +599,15 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
                 }
                 if constexpr (sizeof(T) == 4) {
                     float x[8];
-                    bool fit = true;
 #pragma unroll
                     for (int q = 0; q < 8; q++) {
                         v[u][q] = f < F && c + q < C ? v[u][q] : 0u;
                         x[q] = __uint_as_float(v[u][q]);
-                        fit = fit && fits(v[u][q]);
                     }
                     uint4 o[TERMS];
-                    if (fit) {
-                        split8<TERMS, true>(x, o);
-                    } else {                              // a weight has no term to spare: its leading bits and two terms of what is left
+                    split8<TERMS, true>(x, o);
+                    const unsigned top2 = max_u16x2(max_u16x2(o[0].x & 0x7fff7fffu, o[0].y & 0x7fff7fffu), max_u16x2(o[0].z & 0x7fff7fffu, o[0].w & 0x7fff7fffu));
+                    if (max(top2 & 0xffffu, top2 >> 16) >= 0x7f80u) {      // not all fits(): a weight has no term to spare: its leading bits and two terms of what is left
                         auto join = [](const uint4& a, const uint4& b) { return make_uint4(a.x | b.x, a.y | b.y, a.z | b.z, a.w | b.w); };
                         auto first = [](unsigned b) {     // (what rounding gives, but for numbers that do not fit)
                             const float x = __uint_as_float(b);
