@@ -969,16 +969,21 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 
 // A few rows (a single query): 16 lanes per feature read its weights once, 4 columns each, and multiply them with
 // all the rows.  No staging, so the latency is one round trip to memory (one row of 64 -> 64: 2.5 us, with the matrix cores 10).
-// These kernels take 1 us per 7 M products forward and per 16 M backward, the others have to split and stage the weight first, for
-// as long as some hundred rows take here: hence the rules.  Measured, these against those, in us: float32 forward 64 rows of 2048 ->
-// 1024 25 : 145, 2048 of 64 -> 512 20 : 27, 4096 of 64 -> 512 37 : 28; backward 1024 of 512 -> 512 18 : 30, 2048 33 : 31.  16-bit
-// forward 256 of 512 -> 512 13 : 18, 1024 of 64 -> 512 11 : 15, 2048 20 : 15, 4096 of 64 -> 64 7.0 : 6.3; backward 2048 of 512 -> 64
-// 9 : 19, 512 of 2048 -> 1024 71 : 40.
+// These kernels take 1 us per 7 M products forward and per 15 M backward (per 5 M and 6 M where the weight is read from memory), the
+// others first stage and split the weight, which takes 0.08 us (forward float32; 16 bits 0.03, backward 0.055 and 0.037) per column of
+// the contraction however few the rows, and then go as many rows at once: hence the first rule of each line for the row count and
+// the second for weights so large that the rows, times the features, are read or multiplied longer than that.  Measured, these
+// against those, in us: float32 forward 64 rows of 2048 -> 1024 25 : 160, 2048 of 64 -> 512 20 : 20, 4096 of 64 -> 512 37 : 21, 64 of
+// 16384 -> 16384 3865 : 1290; backward 1024 of 512 -> 512 18 : 35, 2048 33 : 33, 64 of 16384 -> 16384 2792 : 917.  16-bit forward 256 of
+// 512 -> 512 12 : 18, 1024 of 64 -> 512 11 : 15, 2048 20 : 16, 200 of 2048 -> 1024 63 : 61, 64 of 16384 -> 16384 3365 : 545; backward 2048
+// of 512 -> 64 8 : 19, 512 of 2048 -> 1024 71 : 40, 64 of 16384 -> 16384 2362 : 610.
 #define FEW_ROWS 4            // per workgroup
 static bool few(int dtype, bool dx, long long N, int K, int M)
 {
-    if (dx) return N <= 4096 && (N - 200) * K * M <= 1ll << (dtype == GS4D_F32 ? 28 : 27);
-    return dtype == GS4D_F32 ? N <= 4096 && (N - 500) * K * M <= 1ll << 26 : N <= 2048 && (N - 200) * K * M <= 1ll << 25;
+    const bool f32 = dtype == GS4D_F32;
+    if (dx) return N <= 4096 && (N - 200) * K * M <= 1ll << (f32 ? 28 : 27) && N * K <= (f32 ? 350000 : 120000) + (1ll << 28) / M;
+    return f32 ? N <= 4096 && (N - 500) * K * M <= 1ll << 26 && N * M <= 400000 + (1ll << 26) / K
+               : N <= 2048 && (N - 200) * K * M <= 1ll << 25 && N * M <= 130000 + (1ll << 25) / K;
 }
 template <typename T>
 __global__ __launch_bounds__(256) void linear8_few_kernel(RowsArgs a)

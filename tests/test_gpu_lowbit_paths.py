@@ -122,3 +122,30 @@ def test_frame_features_of_axes_of_one_and_of_lines_that_do_not_fit(levels, ch, 
         assert np.abs(np64(got.cpu()[at]) / want - 1).max() <= tol
         each = lb().frame_features(c, *args, t.expand(n).contiguous().cuda())
         assert (got / each - 1).abs().max().item() <= 2 * tol
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 23, 24, 25, 64])
+@pytest.mark.parametrize("k,m", [(70, 16_500), (16_500, 70), (2100, 2000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_few_rows_and_a_large_weight(n, k, m, dtype):
+    """On both sides of what the large dimension leaves to the kernels for few rows."""
+    check_linear(*make(n, k, m, dtype), True, "int8")
+
+
+def test_few_rows_of_a_large_weight_take_no_longer_than_many():
+    """200 rows of 8192 -> 8192 against 512 of them: the time of the kernels for few rows grows with the rows."""
+    w = torch.randn(8192, 8192, device="cuda")
+
+    def time(n):
+        x = torch.randn(n, 8192, device="cuda")
+        with torch.no_grad():
+            for _ in range(2):
+                lb().linear(x, w)
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                lb().linear(x, w)
+            b.record()
+            torch.cuda.synchronize()
+        return a.elapsed_time(b)
+    assert time(200) <= 1.25 * time(512)
