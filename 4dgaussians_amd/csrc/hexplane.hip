@@ -258,9 +258,10 @@ __global__ __launch_bounds__(256) void static_features_kernel(int P, int C, int 
 // workgroup blends the lines of its `slice` channels into LDS once and walks the points with half the corner rows, all of them in
 // LDS: what is left to memory is the cache row, the point and the result.  slice / 4 lanes per point, 4 channels of every level
 // each; workgroups that share points (other slices) differ by 8 in their number, i.e. sit behind one L2.  Bound by memory for wide
-// rows: 1 M points of 2 x 128 channels 308 us (1.38 GB: 4.5 TB/s).
-// The lines cost 3 to 6 us before the first point.  2 levels of 128 channels: 8192 points 10 us (frame_features_kernel: 7), 16384
-// points 12.5 (11.5), 32768 points 17 (20), 131072 points 40 (70); of 32 channels: 32768 points 8.4 (7.0), 131072 points 16 (20).
+// rows: 1 M points of 2 x 128 channels 307 to 324 us (1.38 GB: 4.3 to 4.5 TB/s).
+// The lines cost 3 to 6 us before the first point.  2 levels of 128 channels: 8192 points 8.4 us (frame_features_kernel: 7.2), 16384
+// points 11.5 (11.6), 32768 points 16 (21), 131072 points 38 (70); of 32 channels: 32768 points 8.0 (6.9), 65536 10.1 (11.2), 131072
+// points 15 (20).  (A time per point, in no order, costs that kernel 31 us for 131072 points of 2 x 32 channels, 213 of 2 x 128.)
 #define FRAME_LINES_MIN (1 << 21)     // points * channels from which they pay
 struct FrameArgs {
     gs4d_rows8 c; int L, C, slice, nslices, nwg, gshift;

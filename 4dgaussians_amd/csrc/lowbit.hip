@@ -20,8 +20,8 @@ template <typename T> __device__ __forceinline__ float high16(unsigned w)
 // Both directions move 16 bytes of the caller's rows per lane and step (COLS = 4 float32 or 8 16-bit numbers, neighbouring lanes
 // neighbouring addresses, at any alignment: gfx950 loads and stores 16 bytes from any address) and their codes as one word or two.
 // FULL: width is a multiple of COLS, so that no lane has a shorter share (1 M x 256 float32 read back: 217 us, without 327).
-// Bound by memory: 1 M x 256 float32 is written in 278 us (4.7 TB/s of rows and codes, a copy's rate) and read in 214; 333 k scattered
-// rows of 64 are read in 25 us (4.5 TB/s), odd widths at about 3 TB/s.
+// Bound by memory: 1 M x 256 float32 is written in 273 to 279 us (4.7 TB/s of rows and codes, a copy's rate) and read in 214 to 217; 333 k
+// scattered rows of 64 are read in 25 us (4.5 TB/s).  Odd widths (5, 17, 257) are written at 2.5 to 4.4 TB/s and read at 2.9 to 3.3.
 // A workgroup owns rpb rows, i.e. about ROWS8_ITEMS (row, columns) items; item e of it is row e / cpr by a multiply-high (exact:
 // e * cpr < 2^32).
 #define ROWS8_ITEMS 2048
@@ -366,8 +366,9 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&o)[TERMS])
 
 // An infinity or a NaN of either operand of the float32 products.  Among three terms it would meet lower terms that are 0 and give a
 // NaN where the product is an infinity.  So it is represented by its sign as a leading term, 1 or -1, and stands itself where it
-// meets the other operand's leading term alone: a weight's as its third term, one of x in a product of its own.  What the
-// representatives add to the sum is finite and of no account beside an infinity; the sums of other rows and features come out the same.
+// meets the other operand's leading term alone: a weight's as its third term, one of x in a product of its own (where there is one
+// group of columns, its row is done again instead: AGAIN).  What the representatives add to the sum is finite and of no account beside
+// an infinity; the sums of other rows and features come out the same.
 // A number that would be rounded to an infinity has its leading 8 bits as a term beside the three of what is left.
 __device__ __forceinline__ bool is_finite(unsigned bits) { return (bits & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool fits(unsigned bits) { return (bits & 0x7fffffffu) < 0x7f7f8000u; }
@@ -495,10 +496,10 @@ __device__ __forceinline__ void positive_nans(Group<T>& g)
 
 // How the groups of the contraction and the column blocks are walked:
 //   ROWS_ONE   one group, one column block (64 x 64 layers): nothing to prefetch within a tile, 16 waves of 128 registers
-//              (100 k rows: 23 us; as ROWS_MANY 26)
+//              (100 k rows: 21 us)
 //   ROWS_WIDE  one group, several column blocks: the group's operands stay in registers for all of them
-//   ROWS_MANY  several groups: the next one is in flight while this one is multiplied, 8 waves (1.2 M x 256: 463 us; 16 waves
-//              without the prefetch 503)
+//   ROWS_MANY  several groups: the next one is in flight while this one is multiplied, 8 waves (1.2 M x 256 -> 64: 476 to 496 us; 16
+//              waves without the prefetch took 503 when this took 463)
 //   ROWS_SPLIT several groups, few rows: the waves of a workgroup share a tile of rows, each takes groups of it, and the sums meet in
 //              LDS (SPLIT)
 enum { ROWS_ONE, ROWS_WIDE, ROWS_MANY, ROWS_SPLIT };
@@ -973,10 +974,10 @@ __global__ __launch_bounds__((kRowsThreads<T, NT, VEC, MODE>)) void linear8_rows
 // others first stage and split the weight, which takes 0.08 us (forward float32; 16 bits 0.03, backward 0.055 and 0.037) per column of
 // the contraction however few the rows, and then go as many rows at once: hence the first rule of each line for the row count and
 // the second for weights so large that the rows, times the features, are read or multiplied longer than that.  Measured, these
-// against those, in us: float32 forward 64 rows of 2048 -> 1024 25 : 160, 2048 of 64 -> 512 20 : 20, 4096 of 64 -> 512 37 : 21, 64 of
-// 16384 -> 16384 3865 : 1290; backward 1024 of 512 -> 512 18 : 35, 2048 33 : 33, 64 of 16384 -> 16384 2792 : 917.  16-bit forward 256 of
-// 512 -> 512 12 : 18, 1024 of 64 -> 512 11 : 15, 2048 20 : 16, 200 of 2048 -> 1024 63 : 61, 64 of 16384 -> 16384 3365 : 545; backward 2048
-// of 512 -> 64 8 : 19, 512 of 2048 -> 1024 71 : 40, 64 of 16384 -> 16384 2362 : 610.
+// against those, in us: float32 forward 64 rows of 2048 -> 1024 25 : 156, 2048 of 64 -> 512 20 : 19, 4096 of 64 -> 512 37 : 21, 64 of
+// 16384 -> 16384 3869 : 1263; backward 1024 of 512 -> 512 19 : 33, 2048 33 : 32, 64 of 16384 -> 16384 2794 : 898.  16-bit forward 256 of
+// 512 -> 512 13 : 18, 1024 of 64 -> 512 11 : 15, 2048 20 : 16, 200 of 2048 -> 1024 63 : 61, 64 of 16384 -> 16384 3370 : 542; backward 2048
+// of 512 -> 64 8 : 19, 512 of 2048 -> 1024 71 : 40, 64 of 16384 -> 16384 2358 : 610.
 #define FEW_ROWS 4            // per workgroup
 static bool few(int dtype, bool dx, long long N, int K, int M)
 {
@@ -1119,8 +1120,8 @@ __global__ __launch_bounds__(256) void linear8_few_dx_kernel(RowsArgs a)
 // lies in dy s alone, a float32 number, whose 24 bits are three bfloat16 numbers, for every type of dy.
 // A workgroup: 64 columns m, GW groups of 64 columns k (a wave each) and 8 / GW row slices per group, summed through LDS;
 // one slab of partial sums per workgroup.  Bound by the vector instructions that form and split dy s, once per group of columns:
-// 180 of them and 12 MFMAs a step of 16 rows (float32, int8).  1.2 M x 256 -> 64: 238 us (reading once: 135), 65536 x 512 -> 512
-// fp16 118 us, 100 k x 64 -> 64 12 us.
+// 180 of them and 12 MFMAs a step of 16 rows (float32, int8).  1.2 M x 256 -> 64: 238 to 244 us (reading once: 135), 65536 x 512 -> 512
+// fp16 142 to 148 us (two terms of dy s, which lose up to 2^-15 of a product, 116 to 126), 100 k x 64 -> 64 13 us.
 struct DwArgs {
     long long N; int K, M;
     const void* dy; Keep keep;

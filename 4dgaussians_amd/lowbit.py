@@ -180,8 +180,8 @@ class RowCache:
 def frame_features(cache, planes, aabb, points, t):
     """The features [P, L * C] (float32) of points [P, 3] in the frame at the normalised time t (a tensor of one or of P values):
     row p of the cache -- the product of a level's three spatial planes, levels side by side -- times the bilinear samples of
-    the level's three planes over (axis, t).  planes: 3 per level in the order x, y, z, each [1, C, T, axis] float32 (channels
-    last in memory, or it is copied so); aabb [2, 3] as HexPlaneField keeps it.  Rendering only: no gradient."""
+    the level's three planes over (axis, t).  planes: 3 per level in the order x, y, z, each [1, C, T, axis] float32, C a power of
+    two from 4 to 256 (channels last in memory, or it is copied so); aabb [2, 3] as HexPlaneField keeps it.  Rendering only: no gradient."""
     if not isinstance(cache, RowCache):
         raise RuntimeError("frame_features: cache must be a RowCache")
     dev = cache.device
