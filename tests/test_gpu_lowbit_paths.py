@@ -133,7 +133,8 @@ def test_linear_of_few_rows_and_a_large_weight(n, k, m, dtype):
 
 
 def test_few_rows_of_a_large_weight_take_no_longer_than_many():
-    """200 rows of 8192 -> 8192 against 512 of them: the time of the kernels for few rows grows with the rows."""
+    """200 rows of 8192 -> 8192 against 512 of them: the time of the kernels for few rows grows with the rows (they took four times
+    as long; a factor of two leaves room for clocks)."""
     w = torch.randn(8192, 8192, device="cuda")
 
     def time(n):
@@ -148,4 +149,4 @@ def test_few_rows_of_a_large_weight_take_no_longer_than_many():
             b.record()
             torch.cuda.synchronize()
         return a.elapsed_time(b)
-    assert time(200) <= 1.25 * time(512)
+    assert time(200) <= 2 * time(512)
